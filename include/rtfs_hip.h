@@ -535,6 +535,50 @@ int rtfs_gateway_fwd(const float* x, const float* w, const float* bias, float sl
 int rtfs_cl_to_nchw(const float* src, float* dst, int B, int P, int C, void* stream);
 int rtfs_nchw_to_cl(const float* src, float* dst, int B, int P, int C, void* stream);
 
+/* ---- sequences that go on: causal convolution and selective state-space scan (csrc/ssm_conv.hip, ssm_scan.hip, ssm_bwd.hip) --------------------------------------
+ * The uni-directional counterpart of the SRU entry points: a prompt of any length, its gradient, and one token at a time.  `type`: 0 fp32, 1 bf16 (x, B, C, y
+ * and their gradients; the convolution's state too); parameters, scan states and all sums are fp32.  *_row / *_tok: elements from row to row of the batch and
+ * from token to token (the values of one token are contiguous).  lengths [B] or NULL: tokens of each row (clamped to 0 .. L); behind them outputs are zero,
+ * inputs are not read and the state stays.
+ *   causal_conv: pre[t] = bias + sum_k w[d][k] x[t-K+1+k], y = silu ? silu(pre) : pre; K <= 8; x [B][L][D], w [D][K], state / last [B][K-1][D] (NULL: zeros / none).
+ *   ssm_scan:    d = softplus(dt + dt_bias) (softplus == 0: dt + dt_bias), S[t] = e^{d A} S[t-1] + d x[t] B[t]^T, y[t] = S[t] C[t] + D x[t]; x [B][L][H][P],
+ *                dt [B][L][H] (dt_type as type), Bm, C [B][L][G][N] (H a multiple of G), A, D, dt_bias [H], state / last [B][H][P][N]; P, N <= 128.
+ * Workspaces (fp32, uninitialised): scan forward B*H*segments*(tile+1) when rtfs_ssm_scan_segments > 1; backward starts: twice that, front / behind:
+ * B*ceil(L/64)*H*tile each, parts: 2*bwd_parts*B*L*G*N when rtfs_ssm_scan_bwd_parts > 1, sums: B*ceil(L/64)*H*3; tile = rtfs_ssm_tile(P, N). */
+int rtfs_causal_conv_fwd(const void* x, long long x_row, long long x_tok, const float* w, const float* bias, const void* state, const int* lengths, void* y,
+                         void* last, int B, int L, int D, int K, int silu, int type, void* stream);
+int rtfs_causal_conv_bwd_work_floats(int D, int K, int type);
+/* dy, dlast (or NULL) -> dx [B][L][D], dstate (or NULL), dw [D][K], dbias (or NULL), all written */
+int rtfs_causal_conv_bwd(const void* x, long long x_row, long long x_tok, const float* w, const float* bias, const void* state, const int* lengths,
+                         const void* dy, const void* dlast, void* dx, void* dstate, float* dw, float* dbias, float* work, int B, int L, int D, int K, int silu,
+                         int type, void* stream);
+/* one token per row: x [B][D] (x_row), state [B][K-1][D] moves on in place */
+int rtfs_causal_conv_step(const void* x, long long x_row, void* state, const float* w, const float* bias, void* y, int B, int D, int K, int silu, int type,
+                          void* stream);
+int rtfs_ssm_scan_segments(int B, int L, int H);
+int rtfs_ssm_tile(int P, int N);
+int rtfs_ssm_scan_fwd(const void* x, long long x_row, long long x_tok, const void* dt, long long dt_row, long long dt_tok, int dt_type, const float* A,
+                      const void* Bm, long long b_row, long long b_tok, const void* C, long long c_row, long long c_tok, const float* D, const float* dt_bias,
+                      int softplus, const float* state, const int* lengths, void* y, float* last, float* work, int B, int L, int H, int P, int G, int N, int type,
+                      void* stream);
+int rtfs_ssm_scan_bwd_parts(int B, int L, int H, int G);
+/* dy [B][L][H][P], dlast (or NULL) -> dx, ddt (contiguous, dt's type), dA, dB, dC, dD / dbias / dstate (or NULL), all written */
+int rtfs_ssm_scan_bwd(const void* x, long long x_row, long long x_tok, const void* dt, long long dt_row, long long dt_tok, int dt_type, const float* A,
+                      const void* Bm, long long b_row, long long b_tok, const void* C, long long c_row, long long c_tok, const float* D, const float* dt_bias,
+                      int softplus, const float* state, const int* lengths, const void* dy, const float* dlast, void* dx, void* ddt, float* dA, void* dB, void* dC,
+                      float* dD, float* dbias, float* dstate, float* starts, float* front, float* behind, float* parts, float* sums, int B, int L, int H, int P, int G,
+                      int N, int type, void* stream);
+/* one token per row: x [B][H][P], dt [B][H], Bm, C [B][G][N]; state [B][H][P][N] (16-byte aligned) is updated in place */
+int rtfs_ssm_step(const void* x, long long x_row, const void* dt, long long dt_row, int dt_type, const float* A, const void* Bm, long long b_row, const void* C,
+                  long long c_row, const float* D, const float* dt_bias, int softplus, float* state, void* y, int B, int H, int P, int G, int N, int type,
+                  void* stream);
+
+/* ---- global gradient norm and clipping for any optimizer (csrc/clip.hip): torch.nn.utils.clip_grad_norm_'s arithmetic over n tensors -------------------------------
+ * grads / sizes / types: HOST arrays of device addresses, element counts and types (0 fp32, 1 bf16, 2 fp16); norm_kind 2 (root of the sum of squares, summed in
+ * fp64) or 0 (largest magnitude); norm: one float; parts: n_parts >= 2048 + n doubles of workspace.  g *= min(1, max_norm / (norm + 1e-6)) in place. */
+int rtfs_clip_grad_norm(const long long* grads, const long long* sizes, const int* types, int n, double max_norm, int norm_kind, double* parts, int n_parts,
+                        float* norm, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

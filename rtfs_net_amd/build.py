@@ -11,7 +11,8 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 SOURCES = ["gemm.hip", "dualpath.hip", "attention.hip", "tfar.hip", "stft.hip", "bwd_elem.hip", "bwd_gemm.hip", "bwd_seq.hip", "bwd_attn.hip",
-           "bwd_misc.hip", "spread.hip", "loss.hip", "vp.hip", "vp_train.hip", "vp_attn.hip", "lip.hip", "optim.hip", "views.hip", "bwd_dw.hip"]
+           "bwd_misc.hip", "spread.hip", "loss.hip", "vp.hip", "vp_train.hip", "vp_attn.hip", "lip.hip", "optim.hip", "views.hip", "bwd_dw.hip",
+           "ssm_conv.hip", "ssm_scan.hip", "ssm_bwd.hip", "clip.hip"]
 LIB = os.path.join(HERE, "librtfs_hip.so")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=fast"]
 # The video-branch kernels run on a SIDE stream, i.e. next to the main stream's bf16 MFMA kernels on the same CUs in the bf16 / split-bf16
@@ -21,6 +22,8 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=f
 # with these files built without the SLP vectoriser (vp_block_kernel: 256 -> 0 such instructions, caf_video_kernel: 55 -> 0).  The depth-wise
 # kernels of tfar.hip use native 4-vectors for their packed FMAs and are not affected by the switch.
 EXTRA_FLAGS = {src: ["-fno-slp-vectorize"] for src in ("vp.hip", "tfar.hip", "vp_train.hip", "vp_attn.hip")}
+# The state-space and clip kernels run bf16 MFMA next to scalar fp32 code in the same kernel: no packed-fp32 instruction in them at all.
+EXTRA_FLAGS.update({src: ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] for src in ("ssm_conv.hip", "ssm_scan.hip", "ssm_bwd.hip", "clip.hip")})
 
 
 def _stale() -> bool:

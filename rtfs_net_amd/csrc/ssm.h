@@ -1,0 +1,277 @@
+// Device helpers of the selective scan (ssm_scan.hip, ssm_bwd.hip): chunk staging, matrix-core fragments, decays.
+//
+// A chunk is 64 tokens.  With s[t] = sum_{j <= t} dt[j] A (this head's log decay inside the chunk) everything inside it is a matrix product:
+//   y[t]  = sum_{j <= t} (C[t].B[j]) e^{s[t]-s[j]} dt[j] x[j] + e^{s[t]} S_in C[t],     S_out = e^{s[63]} S_in + sum_j e^{s[63]-s[j]} dt[j] x[j] B[j]^T,
+// and only S, the P x N state, goes from chunk to chunk.
+#pragma once
+#include "common.h"
+
+namespace rtfs {
+namespace ssm {
+
+constexpr int kQ = 64;  // tokens per chunk
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// ---- fragments ------------------------------------------------------------------------------------------------------------------------------------------
+// One fragment is a 16 x 32 operand of D[16x16] += A[16x32] B[32x16]: lane l holds 8 values of row (A) or column (B) l & 15; which 8 of the 32 products it
+// holds is free as long as A and B agree.  Two choices are used, with g = l >> 4: "run" k = 8 g + j, and "pair" k = 4 g + j, 16 + 4 g + j (j < 4), which is
+// how two accumulator tiles lie in registers (lane l: column l & 15, rows 4 g + i), so an accumulator becomes an operand without leaving its lane.
+// fp32 goes through v_mfma_f32_16x16x4_f32 (exact products, one value per lane and step), bf16 through one v_mfma_f32_16x16x32_bf16.
+template <typename T> struct Frag;
+template <> struct Frag<float> { f32x4 a, b; };
+template <> struct Frag<__bf16> { bf16x8 v; };
+
+__device__ __forceinline__ f32x4 mma(const Frag<float>& x, const Frag<float>& y, f32x4 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x.a[j], y.a[j], c, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x.b[j], y.b[j], c, 0, 0, 0);
+    return c;
+}
+__device__ __forceinline__ f32x4 mma(const Frag<__bf16>& x, const Frag<__bf16>& y, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, y.v, c, 0, 0, 0);
+}
+// 4 + 4 values in the operand type; two runs of four in LDS (8- or 16-byte aligned), or fp32 values rounded to it
+__device__ __forceinline__ Frag<float> frag(const float* p, const float* q) {
+    return {*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(q)};
+}
+__device__ __forceinline__ Frag<__bf16> frag(const __bf16* p, const __bf16* q) {
+    const bf16x4 a = *reinterpret_cast<const bf16x4*>(p), b = *reinterpret_cast<const bf16x4*>(q);
+    return {__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7)};
+}
+// 8 neighbours ("run")
+__device__ __forceinline__ Frag<float> frag(const float* p) { return frag(p, p + 4); }
+__device__ __forceinline__ Frag<__bf16> frag(const __bf16* p) { return {*reinterpret_cast<const bf16x8*>(p)}; }
+
+template <typename T> __device__ __forceinline__ Frag<T> frag_of(f32x4 a, f32x4 b);
+template <> __device__ __forceinline__ Frag<float> frag_of<float>(f32x4 a, f32x4 b) { return {a, b}; }
+template <> __device__ __forceinline__ Frag<__bf16> frag_of<__bf16>(f32x4 a, f32x4 b) {
+    Frag<__bf16> f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f.v[j] = (__bf16)a[j], f.v[4 + j] = (__bf16)b[j];
+    return f;
+}
+// An fp32 operand kept to 16 bits of mantissa as the sum of two bf16 (error 2^-17 of it): states and what feeds them are not rounded to 8 bits, nor are the
+// sums that the gradients of dt and A are differences of.  fp32 operands are themselves.
+template <typename T> struct Split { Frag<T> hi, lo; };
+template <> struct Split<float> { Frag<float> hi; };
+__device__ __forceinline__ void split(f32x4 a, f32x4 b, Split<float>& s) { s.hi = {a, b}; }
+__device__ __forceinline__ void split(f32x4 a, f32x4 b, Split<__bf16>& s) {
+    s.hi = frag_of<__bf16>(a, b);
+    f32x4 c, d;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[j] = a[j] - (float)s.hi.v[j], d[j] = b[j] - (float)s.hi.v[4 + j];
+    s.lo = frag_of<__bf16>(c, d);
+}
+__device__ __forceinline__ f32x4 mma(const Split<float>& x, const Frag<float>& y, f32x4 c) { return mma(x.hi, y, c); }
+__device__ __forceinline__ f32x4 mma(const Split<__bf16>& x, const Frag<__bf16>& y, f32x4 c) { return mma(x.lo, y, mma(x.hi, y, c)); }
+__device__ __forceinline__ f32x4 mma(const Frag<float>& x, const Split<float>& y, f32x4 c) { return mma(x, y.hi, c); }
+__device__ __forceinline__ f32x4 mma(const Frag<__bf16>& x, const Split<__bf16>& y, f32x4 c) { return mma(x, y.lo, mma(x, y.hi, c)); }
+
+__device__ __forceinline__ void widen(const Frag<float>& f, f32x4& a, f32x4& b) { a = f.a, b = f.b; }
+__device__ __forceinline__ void widen(const Frag<__bf16>& f, f32x4& a, f32x4& b) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] = (float)f.v[j], b[j] = (float)f.v[4 + j];
+}
+
+// ---- staging --------------------------------------------------------------------------------------------------------------------------------------------
+// Row pitch of a tile in LDS with `n` values per row: 16 bytes of padding keep the 16-byte alignment and move neighbouring rows to other banks.
+template <typename T> __host__ __device__ constexpr int pitch(int n) { return n + 16 / (int)sizeof(T); }
+
+template <typename T> struct Vec8;
+template <> struct Vec8<float> {
+    f32x4 a, b;
+    __device__ __forceinline__ float get(int i) const { return i < 4 ? a[i] : b[i - 4]; }
+    __device__ __forceinline__ void set(int i, float v) { if (i < 4) a[i] = v; else b[i - 4] = v; }
+};
+template <> struct Vec8<__bf16> {
+    bf16x8 v;
+    __device__ __forceinline__ __bf16 get(int i) const { return v[i]; }
+    __device__ __forceinline__ void set(int i, __bf16 x) { v[i] = x; }
+};
+template <typename T> __device__ __forceinline__ Vec8<T> zero8() {
+    Vec8<T> v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v.set(i, (T)0.f);
+    return v;
+}
+
+// A 64-token tile of up to COLS values per token, read by THREADS threads in units of 4 tokens x 8 values; what lies past `rows` tokens or `cols` values is
+// zero (never read: a padded batch may hold anything there).  `fast`: 16-byte loads (addresses, pitches and `cols` allow them).
+template <typename T, int COLS, int THREADS>
+struct Tile {
+    static constexpr int kUnits = 16 * (COLS / 8), kPer = (kUnits + THREADS - 1) / THREADS;
+    Vec8<T> r[kPer][4];
+
+    __device__ __forceinline__ void load(const T* src, long long row, int rows, int cols, bool fast) {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const int u = threadIdx.x + k * THREADS, c = (u >> 4) * 8;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = (u & 15) * 4 + i;
+                r[k][i] = zero8<T>();
+                if ((kUnits % THREADS == 0 || u < kUnits) && t < rows && c < cols) {
+                    const T* p = src + t * row + c;
+                    if (fast) {
+                        r[k][i] = *reinterpret_cast<const Vec8<T>*>(p);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (c + j < cols) r[k][i].set(j, p[j]);
+                    }
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void rows(T* dst) const {  // dst[token][value]
+        constexpr int ld = pitch<T>(COLS);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const int u = threadIdx.x + k * THREADS, c = (u >> 4) * 8, t = (u & 15) * 4;
+            if (kUnits % THREADS == 0 || u < kUnits) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) *reinterpret_cast<Vec8<T>*>(dst + (t + i) * ld + c) = r[k][i];
+            }
+        }
+    }
+    __device__ __forceinline__ void columns(T* dst) const {  // dst[value][token]
+        constexpr int ld = pitch<T>(kQ);
+        typedef T T4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const int u = threadIdx.x + k * THREADS, c = (u >> 4) * 8, t = (u & 15) * 4;
+            if (kUnits % THREADS == 0 || u < kUnits) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    T4 v;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = r[k][i].get(j);
+                    *reinterpret_cast<T4*>(dst + (c + j) * ld + t) = v;
+                }
+            }
+        }
+    }
+};
+
+// ---- decays ---------------------------------------------------------------------------------------------------------------------------------------------
+constexpr float kLog2e = 1.4426950408889634f;
+
+// log(1 + e^v), and its derivative
+__device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.f) + log1pf(expf(-fabsf(v))); }
+
+struct Steps {
+    const void* dt;
+    long long row, tok;
+    int type;           // 0 fp32, 1 bf16
+    const float* bias;  // [H] or none
+    int softplus;
+    __device__ __forceinline__ float raw(int b, long long t, int h) const {
+        const long long i = b * row + t * tok + h;
+        const float v = type == 0 ? static_cast<const float*>(dt)[i] : (float)static_cast<const __bf16*>(dt)[i];
+        return bias ? v + bias[h] : v;
+    }
+};
+
+// sums over the tokens up to and including this lane's, in fp64: the differences s[t] - s[j] are what counts, and behind a strong decay both are large
+__device__ __forceinline__ double running_sum(double v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double u = __shfl_up(v, o, 64);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+// One wave, one token per lane: step and log2 decay (as two floats whose sum is the fp64 value to 48 bits).
+__device__ __forceinline__ void chunk_decay(float step, float A, float& hi, float& lo) {
+    const double s = running_sum((double)step * (double)A * 1.4426950408889634074);
+    hi = (float)s;
+    lo = (float)(s - (double)hi);
+}
+__device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// blocks that follow each other share inputs (heads of a group): hand each XCD a contiguous part of them (workgroup i runs on XCD i % 8)
+__device__ __forceinline__ unsigned xcd_block(unsigned i, unsigned n) {
+    const unsigned q = n >> 3, r = n & 7, x = i & 7, k = i >> 3;
+    return x * q + (x < r ? x : r) + k;
+}
+
+// ---- arguments and host side (ssm_scan.hip) --------------------------------------------------------------------------------------------------------------
+struct ScanArgs {
+    const void *x, *B, *C;
+    long long x_row, x_tok, b_row, b_tok, c_row, c_tok;
+    Steps dt;
+    const float *A, *D, *state;
+    const int* lengths;
+    int rows, L, H, P, G, N;
+    int segs, seg_chunks, chunks;  // segments per row, chunks per segment and per row
+    int fast_x, fast_b, fast_c;
+};
+
+__device__ __forceinline__ int row_length(const int* lengths, int b, int L) {
+    if (!lengths) return L;
+    const int n = lengths[b];
+    return n < 0 ? 0 : n < L ? n : L;
+}
+
+struct WalkOut {
+    const float* starts;  // [row][head][segment][PP][NP], or none: segments start from zero
+    float *ends, *decays;
+    float* tiles;         // [row][chunk][head][PP * NP]
+    float* last;          // [row][head][P][N]
+    int backwards;
+};
+
+
+template <int PP> struct Waves {
+    static constexpr int kWaves = PP / 16 < 4 ? PP / 16 : 4, kThreads = 64 * kWaves, kTiles = PP / 16 / kWaves;  // 16-wide slices of P per wave
+};
+
+// P and N are padded to 32, 64 or 128 in LDS and registers (the padding is zero, in memory there is none)
+inline int padded(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : 128; }
+inline bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+inline bool scan_sizes(int B, int L, int H, int P, int G, int N) {
+    return B > 0 && L > 0 && L <= (1 << 30) && H > 0 && P > 0 && P <= 128 && G > 0 && H % G == 0 && N > 0 && N <= 128 && (long long)B * H <= (1 << 24);
+}
+
+void scan_cut(ScanArgs& a);
+int scan_starts(const ScanArgs& a0, const ScanArgs& a1, const float* state1, float* ws, int both, int type, hipStream_t st);
+int scan_walks(const ScanArgs& a0, const WalkOut& o0, const ScanArgs& a1, const WalkOut& o1, int both, int type, hipStream_t st);
+
+inline ScanArgs scan_args(const void* x, long long x_row, long long x_tok, const Steps& dt, const float* A, const void* B, long long b_row, long long b_tok,
+                          const void* C, long long c_row, long long c_tok, const float* D, const float* state, const int* lengths, int rows, int L, int H, int P,
+                          int G, int N, int type) {
+    ScanArgs a{x, B, C, x_row, x_tok, b_row, b_tok, c_row, c_tok, dt, A, D, state, lengths, rows, L, H, P, G, N, 1, 0, 0, 0, 0, 0};
+    const int v = type == 0 ? 4 : 8;
+    a.fast_x = P % 8 == 0 && x_row % v == 0 && x_tok % v == 0 && on16(x);
+    a.fast_b = N % 8 == 0 && b_row % v == 0 && b_tok % v == 0 && on16(B);
+    a.fast_c = N % 8 == 0 && c_row % v == 0 && c_tok % v == 0 && on16(C);
+    scan_cut(a);
+    return a;
+}
+
+#define RTFS_SSM_PP(T, NP, P, F, ARGS)         \
+    do {                                       \
+        if ((P) <= 32) return F<T, NP, 32> ARGS; \
+        if ((P) <= 64) return F<T, NP, 64> ARGS; \
+        return F<T, NP, 128> ARGS;             \
+    } while (0)
+#define RTFS_SSM_NP(T, N, P, F, ARGS)                      \
+    do {                                                   \
+        if ((N) <= 32) RTFS_SSM_PP(T, 32, P, F, ARGS);     \
+        else if ((N) <= 64) RTFS_SSM_PP(T, 64, P, F, ARGS); \
+        else RTFS_SSM_PP(T, 128, P, F, ARGS);              \
+    } while (0)
+#define RTFS_SSM_DISPATCH(type, N, P, F, ARGS)         \
+    do {                                               \
+        if ((type) == 0) RTFS_SSM_NP(float, N, P, F, ARGS); \
+        else RTFS_SSM_NP(__bf16, N, P, F, ARGS);       \
+    } while (0)
+
+}  // namespace ssm
+}  // namespace rtfs

@@ -161,6 +161,18 @@ SIGNATURES = {
     "rtfs_proj_gateway_bwd_bf16": [P, P, P, P, P, P, F, P, I, P, I, P, P, P, LL, I, P],
     "rtfs_fold_gemm_bwd_bf16": [P, P, P, I, I, I, I, P],
     "rtfs_convt_bwd_input_bf16": [P, P, P, I, I, I, I, P],
+    # ---- causal convolution, selective scan, gradient clip (rtfs_net_amd.ssm, rtfs_net_amd.optim) ----
+    "rtfs_causal_conv_fwd": [P, LL, LL, P, P, P, P, P, P, I, I, I, I, I, I, P],
+    "rtfs_causal_conv_bwd_work_floats": [I, I, I],
+    "rtfs_causal_conv_bwd": [P, LL, LL] + [P] * 11 + [I] * 6 + [P],
+    "rtfs_causal_conv_step": [P, LL, P, P, P, P, I, I, I, I, I, P],
+    "rtfs_ssm_scan_segments": [I, I, I],
+    "rtfs_ssm_tile": [I, I],
+    "rtfs_ssm_scan_fwd": [P, LL, LL, P, LL, LL, I, P, P, LL, LL, P, LL, LL, P, P, I, P, P, P, P, P] + [I] * 7 + [P],
+    "rtfs_ssm_scan_bwd_parts": [I, I, I, I],
+    "rtfs_ssm_scan_bwd": [P, LL, LL, P, LL, LL, I, P, P, LL, LL, P, LL, LL, P, P, I] + [P] * 17 + [I] * 7 + [P],
+    "rtfs_ssm_step": [P, LL, P, LL, I, P, P, LL, P, LL, P, P, I, P, P] + [I] * 6 + [P],
+    "rtfs_clip_grad_norm": [P, P, P, I, D, I, P, I, P, P],
 }
 
 _lib = None

@@ -8,9 +8,12 @@ moment updates, bias-corrected update, in torch.optim.AdamW's own operation orde
 `FusedAdamW` is a `torch.optim.Optimizer`: param groups, `zero_grad`, `state_dict` / `load_state_dict` behave as usual and the per-parameter state
 (`step`, `exp_avg`, `exp_avg_sq`) has torch.optim.AdamW's keys, so optimizer checkpoints interchange with it.  One group's hyper-parameters apply per
 launch pair; parameters must be contiguous fp32 CUDA tensors (RTFS-Net's are).  `amsgrad`, `maximize`, sparse gradients: not supported (raise).
+
+`clip_grad_norm_` is the clip alone (csrc/clip.hip), for any other optimizer and for fp32, bf16 and fp16 gradients.
 """
 from __future__ import annotations
 
+import array
 import math
 
 import torch
@@ -126,3 +129,65 @@ class FusedAdamW(torch.optim.Optimizer):
             g_np[i] = g.data_ptr()
         plan["dev"][1].copy_(row, non_blocking=True)
         return group, ps, plan
+
+
+_CLIP_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0):
+    """torch.nn.utils.clip_grad_norm_ as HIP launches: the norm of all gradients of `parameters` (a tensor or an iterable of them; those without a gradient are
+    passed over) taken as one vector, and every gradient scaled in place by min(1, max_norm / (norm + 1e-6)).
+
+    norm_type 2 or inf.  fp32, bf16 and fp16 gradients in any mix, dense in any order of their dimensions, on one device; the same tensor listed twice counts
+    once.  The norm's squares are summed in fp64 in a fixed order.  -> the norm before clipping, a 0-dim fp32 tensor on the gradients' device (nothing is copied
+    to the host; a norm that is not finite is not an error: a NaN goes through to every gradient).  Every gradient is written, also where the factor is 1."""
+    max_norm, norm_type = float(max_norm), float(norm_type)
+    if not max_norm >= 0.0:
+        raise ValueError("clip_grad_norm_: max_norm must not be negative")
+    if norm_type not in (2.0, math.inf):
+        raise ValueError(f"clip_grad_norm_: norm_type 2 or inf, got {norm_type}")
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads, device, seen = [], None, set()
+    at, sizes, types = array.array("q"), array.array("q"), array.array("i")
+    for p in parameters:
+        g = p.grad
+        if g is None or id(g) in seen:
+            continue
+        kind = _CLIP_TYPES.get(g.dtype)
+        if kind is None or g.layout != torch.strided or not g.is_cuda:
+            raise ValueError(f"clip_grad_norm_: gradients must be dense fp32, bf16 or fp16 HIP tensors, got {g.dtype}, {g.layout}, {g.device}")
+        if device is None:
+            device = g.device
+        elif g.device != device:
+            raise ValueError(f"clip_grad_norm_: gradients on {device} and {g.device}")
+        if not g.is_contiguous() and not _fills_its_span(g):
+            raise ValueError("clip_grad_norm_: a gradient has gaps or overlaps in memory")
+        seen.add(id(g))
+        grads.append(g)
+        if g.numel():
+            at.append(g.data_ptr())
+            sizes.append(g.numel())
+            types.append(kind)
+    if device is None:
+        return torch.zeros(())
+    if not at:
+        return torch.zeros((), device=device)
+    norm = torch.empty((), device=device)
+    n = len(at) + sum(s >> 30 for s in sizes)  # a tensor of over 2^30 elements is listed in pieces
+    parts = torch.empty(2048 + n, dtype=torch.float64, device=device)
+    lib.call("rtfs_clip_grad_norm", at.buffer_info()[0], sizes.buffer_info()[0], types.buffer_info()[0], len(at), max_norm, 2 if norm_type == 2.0 else 0, parts,
+             parts.numel(), norm)
+    torch.autograd.graph.increment_version(grads)  # written through their addresses
+    return norm
+
+
+def _fills_its_span(t):
+    """whether t's elements are a gap-free stretch of memory, in whatever order of its dimensions"""
+    size = 1
+    for stride, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != size:
+            return False
+        size *= n
+    return True

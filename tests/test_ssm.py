@@ -1,0 +1,494 @@
+"""rtfs_net_amd.ssm (csrc/ssm_conv.hip, ssm_scan.hip, ssm_bwd.hip) against token-by-token definitions in float64.
+
+Tolerances (relative L2 error of a whole tensor), from the roundings counted: u = finfo.eps / 2 of the type.
+  fp32: sums of at most 128 + 64 + a few products, each rounded once: below 256 u = 1.6e-5.
+  bf16: y and dx: scores (or weights), state and result are rounded once each, 3 u; dB, dC: scores and result, 2 u; all inputs are exact.
+  fp32 results of bf16 inputs (states, parameter gradients, dt's gradient): operands split to 2^-17, twice on the way: 256 u(fp32) + 2 * 2^-17 = 3.1e-5."""
+import pytest
+import torch
+
+gpu = pytest.mark.gpu
+U16, U32 = torch.finfo(torch.bfloat16).eps / 2, torch.finfo(torch.float32).eps / 2
+
+
+def tol(kind, roundings=0):
+    """`roundings` to bf16 when the inputs are; 0: a result that stays fp32"""
+    if kind == torch.float32:
+        return 256 * U32
+    return roundings * U16 if roundings else 256 * U32 + 2 * 2.0 ** -17
+
+
+def off(got, want):
+    got, want = got.detach().double().cpu(), want.detach().double().cpu()
+    assert got.shape == want.shape
+    return float((got - want).norm() / want.norm().clamp_min(1e-30)) if want.numel() else 0.0
+
+
+def alive_of(lengths, B, L):
+    ends = torch.full((B,), L) if lengths is None else lengths.clamp(0, L).long()
+    return ends, torch.arange(L) < ends[:, None]
+
+
+def ref_conv(x, w, bias, state, lengths, silu):
+    B, L, D = x.shape
+    K = w.shape[1]
+    ends, alive = alive_of(lengths, B, L)
+    x = torch.where(alive[..., None], x, torch.zeros((), dtype=x.dtype))
+    line = torch.cat([x.new_zeros(B, K - 1, D) if state is None else state, x], 1)
+    pre = sum(line[:, k:k + L] * w[:, k] for k in range(K))
+    if bias is not None:
+        pre = pre + bias
+    y = pre * torch.sigmoid(pre) if silu else pre
+    return torch.where(alive[..., None], y, torch.zeros((), dtype=y.dtype)), torch.stack([line[b, e:e + K - 1] for b, e in enumerate(ends.tolist())])
+
+
+def ref_scan(x, dt, A, Bm, C, D, bias, softplus, state, lengths):
+    B, L, H, P = x.shape
+    G, N = Bm.shape[2:]
+    _, alive = alive_of(lengths, B, L)
+    zero = torch.zeros((), dtype=x.dtype)
+    x, Bm, C = (torch.where(alive[..., None, None], v, zero) for v in (x, Bm, C))
+    d = torch.where(alive[..., None], dt, zero)
+    d = d if bias is None else d + bias
+    d = torch.nn.functional.softplus(d, threshold=60) if softplus else d
+    d = torch.where(alive[..., None], d, zero)
+    Bm, C = Bm.repeat_interleave(H // G, 2), C.repeat_interleave(H // G, 2)
+    S = x.new_zeros(B, H, P, N) if state is None else state
+    ys = []
+    for t in range(L):
+        S = torch.exp(d[:, t] * A)[..., None, None] * S + (d[:, t, :, None] * x[:, t])[..., None] * Bm[:, t, :, None]
+        ys.append((S * C[:, t, :, None]).sum(-1))
+    y = torch.stack(ys, 1)
+    y = y if D is None else y + D[:, None] * x
+    return torch.where(alive[..., None, None], y, zero), S
+
+
+def scan_inputs(B, L, H, G, P, N, kind, seed=0, fp32_dt=False, pad=0):
+    """on the CPU; `pad`: extra values per token, so that the tensors are slices"""
+    r = torch.Generator().manual_seed(seed)
+
+    def normal(*shape, scale=1.0, dtype=kind):
+        return (torch.randn(*shape, generator=r) * scale).to(dtype)
+
+    v = {"x": normal(B, L, H * P + pad)[..., pad // 2:pad // 2 + H * P].unflatten(-1, (H, P)),
+         "dt": normal(B, L, H + pad, scale=0.5, dtype=torch.float32 if fp32_dt else kind)[..., :H],
+         "A": -(0.5 + 8 * torch.rand(H, generator=r)),
+         "Bm": normal(B, L, G * N + pad)[..., :G * N].unflatten(-1, (G, N)), "C": normal(B, L, G * N + pad)[..., pad:].unflatten(-1, (G, N)),
+         "D": 1 + normal(H, scale=0.1, dtype=torch.float32), "bias": normal(H, dtype=torch.float32) - 2,
+         "state": normal(B, H, P, N, dtype=torch.float32)}
+    return v
+
+
+def gpu_scan(v, lengths=None, softplus=True, want_state=True):
+    from rtfs_net_amd.ssm import selective_scan
+
+    return selective_scan(v["x"], v["dt"], v["A"], v["Bm"], v["C"], v["D"], dt_bias=v["bias"], softplus=softplus, state=v["state"],
+                          lengths=None if lengths is None else lengths.cuda(), return_state=want_state)
+
+
+def cuda(v, leaf=False):
+    """to the GPU with the same strides (slices stay slices)"""
+    out = {}
+    for k, t in v.items():
+        if t is None:
+            out[k] = None
+            continue
+        base = torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device="cuda")
+        out[k] = base.copy_(t).requires_grad_(leaf)
+    return out
+
+
+SHAPES = [  # B, L, H, G, P, N
+    (1, 1, 1, 1, 1, 1), (2, 2, 4, 2, 32, 32), (3, 63, 2, 1, 17, 5), (2, 64, 4, 4, 64, 64), (1, 65, 2, 1, 128, 128), (2, 130, 6, 2, 48, 40),
+    (5, 200, 3, 1, 33, 128), (1, 64 * 9 + 5, 2, 2, 64, 16), (2, 320, 4, 1, 20, 65), (1, 1030, 1, 1, 100, 33),
+]
+
+
+@gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_scan_matches_the_recurrence(shape, kind):
+    B, L, H, G, P, N = shape
+    for pad, ragged in ((0, False), (24, True)):
+        v = scan_inputs(*shape, kind, seed=L, pad=pad)
+        lengths = torch.randint(0, L + 1, (B,), generator=torch.Generator().manual_seed(1), dtype=torch.int32) if ragged else None
+        want, last = ref_scan(*(v[k].double() for k in ("x", "dt", "A", "Bm", "C", "D", "bias")), True, v["state"].double(), lengths)
+        y, s = gpu_scan(cuda(v), lengths)
+        assert y.dtype == kind and s.dtype == torch.float32
+        assert off(y, want) <= tol(kind, 3) and off(s, last) <= tol(kind), (pad, off(y, want), off(s, last))
+
+
+@gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_scan_gradients_match_the_recurrences(shape, kind):
+    B, L, H, G, P, N = shape
+    v = scan_inputs(*shape, kind, seed=L + 1, fp32_dt=L % 2 == 0)
+    r = torch.Generator().manual_seed(2)
+    lengths = torch.randint(0, L + 1, (B,), generator=r, dtype=torch.int32) if B > 2 else None
+    dy, ds = torch.randn(B, L, H, P, generator=r).to(kind), torch.randn(B, H, P, N, generator=r)
+    leaves = {k: t.double().requires_grad_() for k, t in v.items()}
+    y, s = ref_scan(*(leaves[k] for k in ("x", "dt", "A", "Bm", "C", "D", "bias")), True, leaves["state"], lengths)
+    want = dict(zip(leaves, torch.autograd.grad((y, s), list(leaves.values()), (dy.double(), ds.double()))))
+    here = cuda(v, leaf=True)
+    got = dict(zip(here, torch.autograd.grad(gpu_scan(here, lengths), list(here.values()), (dy.cuda(), ds.cuda()))))
+    # One number has no random signs to average: dC = e^s S dy + (V E d) B with the second factor rounded is off by u |V E d B| + u |dC|, and |dC| may be as small
+    # as the two terms happen to cancel.  Its error counts against the sum of the terms' magnitudes, which the same gradients of |inputs| give.
+    size = want
+    if B * L * H * P * N == 1:
+        mag = {k: t.double().abs().requires_grad_() if k in ("x", "Bm", "C", "state", "D") else t.double().requires_grad_() for k, t in v.items()}
+        m = ref_scan(*(mag[k] for k in ("x", "dt", "A", "Bm", "C", "D", "bias")), True, mag["state"], lengths)
+        size = dict(zip(mag, torch.autograd.grad(m, list(mag.values()), (dy.double().abs(), ds.double().abs()))))
+    bad = {}
+    for k in want:
+        assert got[k].dtype == v[k].dtype
+        bound = {"x": tol(kind, 3), "Bm": tol(kind, 2), "C": tol(kind, 2), "dt": tol(kind, 0) if got[k].dtype == torch.float32 else tol(kind, 1) * 1.01}.get(k, tol(kind))
+        # a sum over all tokens may cancel: its error counts against the sum of magnitudes, which for these inputs is below sqrt(tokens) of its value
+        if k in ("A", "D", "bias"):
+            bound *= max(1.0, (B * L * P) ** 0.5 / 8)
+        err = off(got[k], want[k]) * float(want[k].norm() / size[k].norm())
+        if err > bound:
+            bad[k] = (err, bound)
+    assert not bad, bad
+
+
+@gpu
+def test_scan_gradient_against_differences():
+    """the loss moves along a random direction as the gradients say, by central differences of the float64 definition"""
+    v = scan_inputs(2, 70, 4, 2, 24, 12, torch.float32, seed=5)
+    r = torch.Generator().manual_seed(3)
+    dy, way = torch.randn(2, 70, 4, 24, generator=r).double(), {k: torch.randn(t.shape, generator=r).double() * 0.3 for k, t in v.items()}
+    here = cuda(v, leaf=True)
+    grads = torch.autograd.grad(gpu_scan(here, want_state=False), list(here.values()), dy.float().cuda())
+    got = sum(float((g.double().cpu() * way[k]).sum()) for k, g in zip(here, grads))
+
+    def loss(h):
+        w = {k: t.double() + h * way[k] for k, t in v.items()}
+        return float((ref_scan(*(w[k] for k in ("x", "dt", "A", "Bm", "C", "D", "bias")), True, w["state"], None)[0] * dy).sum())
+
+    want = (8 * (loss(1e-4) - loss(-1e-4)) - (loss(2e-4) - loss(-2e-4))) / 12e-4
+    scale = sum(float((g.double().cpu() * way[k]).norm()) for k, g in zip(here, grads))
+    assert abs(got - want) <= 256 * U32 * scale + 1e-7 * abs(want)
+
+
+@gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("B,H,G,P,N", [(1, 4, 1, 32, 32), (3, 6, 2, 48, 40), (2, 3, 3, 33, 7), (2, 2, 1, 128, 128), (1, 1, 1, 1, 1)])
+def test_prompt_in_pieces_then_single_tokens(kind, B, H, G, P, N):
+    """a prompt cut anywhere, then one token at a time, is the whole sequence; the conv goes on the same way"""
+    from rtfs_net_amd.ssm import causal_conv, causal_conv_step, selective_scan, selective_scan_step
+
+    L = 150
+    v = scan_inputs(B, L, H, G, P, N, kind, seed=9)
+    want, last = ref_scan(*(v[k].double() for k in ("x", "dt", "A", "Bm", "C", "D", "bias")), True, v["state"].double(), None)
+    c = cuda(v)
+    ys, state = [], c["state"]
+    with torch.no_grad():
+        for a, b in ((0, 64), (64, 65), (65, 147)):
+            y, state = selective_scan(c["x"][:, a:b], c["dt"][:, a:b], c["A"], c["Bm"][:, a:b], c["C"][:, a:b], c["D"], dt_bias=c["bias"], softplus=True, state=state,
+                                      return_state=True)
+            ys.append(y)
+        for t in range(147, L):
+            ys.append(selective_scan_step(c["x"][:, t], c["dt"][:, t], c["A"], c["Bm"][:, t], c["C"][:, t], state, c["D"], dt_bias=c["bias"], softplus=True)[:, None])
+    assert off(torch.cat(ys, 1), want) <= tol(kind, 3) and off(state, last) <= 2 * tol(kind)
+    r = torch.Generator().manual_seed(4)
+    D, K = H * P, 4
+    x, w, b = torch.randn(B, 20, D, generator=r).to(kind), torch.randn(D, K, generator=r), torch.randn(D, generator=r)
+    want, last = ref_conv(x.double(), w.double(), b.double(), None, None, True)
+    xc, wc, bc = x.cuda(), w.cuda(), b.cuda()
+    y0, s = causal_conv(xc[:, :2], wc, bc, return_state=True)
+    y1, s = causal_conv(xc[:, 2:17], wc, bc, state=s, return_state=True)
+    y2 = [causal_conv_step(xc[:, t], s, wc, bc)[:, None] for t in range(17, 20)]
+    assert off(torch.cat([y0, y1, *y2], 1), want) <= tol(kind, 1) and torch.equal(s.cpu(), last.to(kind))
+
+
+@gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("B,L,D,K,silu,pad", [(1, 1, 1, 1, True, 0), (2, 3, 5, 8, True, 0), (3, 70, 64, 4, True, 0), (2, 33, 40, 3, False, 8), (1, 300, 24, 4, True, 3),
+                                              (4, 129, 512, 2, True, 0), (2, 2, 16, 5, True, 0), (7, 37, 192, 6, False, 0), (1, 40, 700, 7, True, 0)])
+def test_conv_and_its_gradients(kind, B, L, D, K, silu, pad):
+    from rtfs_net_amd.ssm import causal_conv
+
+    r = torch.Generator().manual_seed(L)
+    for ragged, with_state in ((False, False), (True, True)):
+        x = torch.randn(B, L, D + pad, generator=r).to(kind)[..., pad:]
+        w, b = torch.randn(D, K, generator=r) / K ** 0.5, torch.randn(D, generator=r)
+        state = torch.randn(B, K - 1, D, generator=r).to(kind) if with_state else None
+        lengths = torch.randint(0, L + 1, (B,), generator=r, dtype=torch.int32) if ragged else None
+        dy, dl = torch.randn(B, L, D, generator=r).to(kind), torch.randn(B, K - 1, D, generator=r).to(kind)
+        leaves = {"x": x, "w": w, "b": b, **({"state": state} if with_state else {})}
+        ref = {k: t.double().requires_grad_() for k, t in leaves.items()}
+        y, last = ref_conv(ref["x"], ref["w"], ref["b"], ref.get("state"), lengths, silu)
+        want = torch.autograd.grad((y, last), list(ref.values()), (dy.double(), dl.double()), allow_unused=True)
+        here = cuda(leaves, leaf=True)
+        out = causal_conv(here["x"], here["w"], here["b"], silu=silu, state=here.get("state"), lengths=None if lengths is None else lengths.cuda(), return_state=True)
+        assert off(out[0], y) <= tol(kind, 1) and torch.equal(out[1].cpu().double(), last.detach())
+        got = torch.autograd.grad(out, list(here.values()), (dy.cuda(), dl.cuda()))
+        for k, g, q in zip(leaves, got, want):
+            # w and b: fp32 sums over B L tokens whose magnitudes add up to at most sqrt(B L) of the result for random signs
+            bound = tol(kind, 1) if k in ("x", "state") else 64 * U32 * max(1.0, (B * L) ** 0.5)
+            assert off(g, torch.zeros_like(g, device="cpu") if q is None else q) <= bound, (k, ragged, off(g, q))
+
+
+@gpu
+def test_nothing_behind_a_rows_end_is_read():
+    """a padded batch may hold anything there: outputs, gradients and states are those of a batch of zeros there"""
+    from rtfs_net_amd.ssm import causal_conv
+
+    v = scan_inputs(4, 100, 2, 1, 16, 8, torch.float32, seed=1)
+    lengths = torch.tensor([100, 37, 0, 64], dtype=torch.int32)
+    _, alive = alive_of(lengths, 4, 100)
+    results = []
+    for filler in (0.0, float("nan"), float("inf")):
+        w = {k: t.clone() for k, t in v.items()}
+        for k in ("x", "dt", "Bm", "C"):
+            w[k][~alive] = filler
+        here = cuda(w, leaf=True)
+        dy = torch.randn(4, 100, 2, 16, generator=torch.Generator().manual_seed(0))
+        dy[~alive] = filler
+        y, s = gpu_scan(here, lengths)
+        results.append([y.detach(), s.detach(), *torch.autograd.grad((y, s), list(here.values()), (dy.cuda(), torch.ones_like(s)))])
+        x = here["x"].detach().flatten(2).requires_grad_()
+        wt = torch.randn(32, 4, generator=torch.Generator().manual_seed(1)).cuda().requires_grad_()
+        y, s = causal_conv(x, wt, lengths=lengths.cuda(), return_state=True)
+        results[-1] += [y.detach(), s.detach(), *torch.autograd.grad((y, s), (x, wt), (dy.flatten(2).cuda(), torch.ones_like(s)))]
+    for other in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(results[0], other))
+    assert not results[0][0].cpu()[~alive].any()
+
+
+@gpu
+def test_rows_are_independent_and_runs_repeat():
+    """a NaN in one row stays in it; the same inputs give the same bits, gradients included"""
+    v = scan_inputs(3, 700, 2, 1, 32, 32, torch.bfloat16, seed=2)
+    here = cuda(v, leaf=True)
+    dy = torch.randn(3, 700, 2, 32, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16).cuda()
+
+    def once(v):
+        y, s = gpu_scan(v)
+        return [y.detach(), s.detach(), *torch.autograd.grad((y, s), list(v.values()), (dy, torch.ones_like(s)))]
+
+    a, b = once(here), once(here)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    w = {k: t.clone() for k, t in v.items()}
+    w["x"][1, 300, 0, 3] = float("nan")
+    c = once(cuda(w, leaf=True))
+    for p, q in zip(a[:2], c[:2]):
+        assert torch.equal(p[0], q[0]) and torch.equal(p[2], q[2]) and q[1].isnan().any()
+
+
+@gpu
+def test_strong_decay_and_growth_stay_finite():
+    """steps so large that every state is forgotten at once, and steps of zero: no NaN from differences of large sums, values by the definition"""
+    v = scan_inputs(2, 200, 2, 1, 16, 16, torch.float32, seed=3)
+    v["bias"] = torch.tensor([40.0, -300.0])
+    want, last = ref_scan(*(v[k].double() for k in ("x", "dt", "A", "Bm", "C", "D", "bias")), True, v["state"].double(), None)
+    y, s = gpu_scan(cuda(v))
+    assert off(y, want) <= tol(torch.float32) and off(s, last) <= tol(torch.float32)
+    v = scan_inputs(1, 130, 2, 1, 16, 16, torch.float32, seed=4)
+    v["A"], v["bias"] = torch.tensor([0.05, 0.0]), torch.zeros(2)  # a state that grows, one that only adds up
+    want, last = ref_scan(*(v[k].double() for k in ("x", "dt", "A", "Bm", "C", "D", "bias")), True, v["state"].double(), None)
+    y, s = gpu_scan(cuda(v))
+    assert off(y, want) <= 4 * tol(torch.float32) and off(s, last) <= 4 * tol(torch.float32)
+
+
+@gpu
+def test_optional_arguments():
+    """without D, bias, softplus, state; one output alone wanted, one gradient alone given"""
+    from rtfs_net_amd.ssm import selective_scan
+
+    v = scan_inputs(2, 90, 2, 1, 16, 16, torch.float32, seed=6)
+    v["dt"] = v["dt"].abs() * 0.1
+    leaves = {k: v[k].double().requires_grad_() for k in ("x", "dt", "A", "Bm", "C")}
+    y, s = ref_scan(*leaves.values(), None, None, False, None, None)
+    here = cuda({k: v[k] for k in leaves}, leaf=True)
+    for pick in (0, 1):
+        want = torch.autograd.grad((y, s)[pick].square().sum(), list(leaves.values()), retain_graph=True, allow_unused=True)
+        out = selective_scan(*here.values(), return_state=True)[pick]
+        got = torch.autograd.grad(out.square().sum(), list(here.values()))
+        for k, a, b in zip(leaves, got, want):
+            assert off(a, torch.zeros(a.shape) if b is None else b) <= 8 * tol(torch.float32), (pick, k)
+    assert torch.equal(selective_scan(*(t.detach() for t in here.values())), selective_scan(*here.values()).detach())
+
+
+@gpu
+@pytest.mark.parametrize("B,L", [(0, 5), (2, 0)])
+def test_no_tokens(B, L):
+    from rtfs_net_amd.ssm import causal_conv, causal_conv_step, selective_scan_step
+
+    v = cuda(scan_inputs(B, L, 2, 1, 4, 4, torch.float32))
+    y, s = gpu_scan(v)
+    assert y.shape == (B, L, 2, 4) and torch.equal(s, v["state"])
+    w = torch.ones(8, 4, device="cuda")
+    y, s = causal_conv(v["x"].flatten(2), w, return_state=True)
+    assert y.shape == (B, L, 8) and s.shape == (B, 3, 8) and not s.any()
+    if B == 0:
+        assert causal_conv_step(v["x"].new_zeros(0, 8), w.new_zeros(0, 3, 8), w).shape == (0, 8)
+        assert selective_scan_step(w.new_zeros(0, 2, 4), w.new_zeros(0, 2), v["A"], w.new_zeros(0, 1, 4), w.new_zeros(0, 1, 4), v["state"]).shape == (0, 2, 4)
+
+
+@gpu
+def test_captured_steps_and_prompts_replay():
+    """two graphs captured from the same calls, replayed in turn with eager work between, give the eager results each time"""
+    from rtfs_net_amd.ssm import causal_conv_step, selective_scan_step
+
+    r = torch.Generator(device="cuda").manual_seed(0)
+    x, dt = torch.empty(2, 1, 4, 16, device="cuda"), torch.empty(2, 1, 4, device="cuda")
+    A, w = -torch.rand(4, device="cuda", generator=r), torch.randn(64, 4, device="cuda", generator=r)
+    bc = torch.randn(2, 1, 1, 8, device="cuda", generator=r)
+    long = cuda(scan_inputs(1, 64 * 12, 2, 1, 32, 32, torch.float32, seed=8))
+
+    def token(conv, state):
+        y = causal_conv_step(x.view(2, 64), conv, w)
+        return selective_scan_step(y.view(2, 4, 16), dt[:, 0], A, bc[:, 0], bc[:, 0], state, softplus=True)
+
+    def fresh():
+        return torch.zeros(2, 3, 64, device="cuda"), torch.zeros(2, 4, 16, 8, device="cuda")
+
+    eager, held = fresh(), fresh()
+    x.normal_(generator=r), dt.normal_(generator=r)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side), torch.no_grad():
+        token(*fresh()), gpu_scan(long)
+    torch.cuda.synchronize()
+    one, two = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.no_grad():
+        with torch.cuda.graph(one):
+            out = token(*held)
+        with torch.cuda.graph(two):
+            prompt = gpu_scan(long)
+    held[0].zero_(), held[1].zero_()
+    for i in range(4):
+        x.normal_(generator=r), dt.normal_(generator=r)
+        long["x"].normal_(generator=r)
+        one.replay()
+        want = token(*eager)
+        two.replay()
+        y, s = gpu_scan(long)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(held[0], eager[0]) and torch.equal(held[1], eager[1]), i
+        assert torch.equal(prompt[0], y) and torch.equal(prompt[1], s), i
+
+
+@gpu
+def test_a_layer_of_them_trains_and_serves():
+    """projection -> convolution -> scan, a training step with the clip, on a side stream; then the trained layer frame by frame gives the prompt's outputs"""
+    from rtfs_net_amd.optim import clip_grad_norm_
+    from rtfs_net_amd.ssm import causal_conv, causal_conv_step, selective_scan, selective_scan_step
+
+    torch.manual_seed(0)
+    H, P, N, dim = 4, 32, 16, 64
+    width = H * P + 2 * N
+    into, weight, A = torch.nn.Linear(dim, width + H).cuda(), torch.nn.Parameter(torch.randn(width, 4, device="cuda") / 2), torch.nn.Parameter(torch.zeros(H, device="cuda"))
+    params = [*into.parameters(), weight, A]
+    opt = torch.optim.SGD(params, lr=0.1)
+
+    def layer(x):
+        xbc, dt = into(x).split([width, H], -1)
+        xs, b, c = causal_conv(xbc, weight).split([H * P, N, N], -1)
+        return selective_scan(xs.unflatten(-1, (H, P)), dt, -A.exp(), b[:, :, None], c[:, :, None], softplus=True)
+
+    x = torch.randn(3, 150, dim, device="cuda")
+    before = [p.detach().clone() for p in params]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer(x).square().mean().backward()
+        grads = [p.grad.clone() for p in params]
+        norm = clip_grad_norm_(params, 1e-3)
+        opt.step()
+    torch.cuda.current_stream().wait_stream(side)
+    want = torch.stack([g.double().norm() for g in grads]).norm()
+    assert abs(float(norm) / float(want) - 1) < 4 * U32 and float(want) > 1e-3
+    for p, q, g in zip(params, before, grads):
+        assert g.abs().max() > 0 and off(p.grad, g * (1e-3 / (norm + 1e-6))) <= 4 * U32
+        assert torch.equal(p.detach(), torch.add(q, p.grad, alpha=-0.1))
+    with torch.no_grad():
+        want = layer(x)
+        xbc, dt = into(x).split([width, H], -1)
+        conv, state, got = torch.zeros(3, 3, width, device="cuda"), torch.zeros(3, H, P, N, device="cuda"), []
+        for t in range(150):
+            xs, b, c = causal_conv_step(xbc[:, t], conv, weight).split([H * P, N, N], -1)
+            got.append(selective_scan_step(xs.unflatten(-1, (H, P)), dt[:, t], -A.exp(), b[:, None], c[:, None], state, softplus=True))
+    assert off(torch.stack(got, 1), want) <= 2 * tol(torch.float32)
+
+
+@gpu
+def test_broadcast_inputs_get_summed_gradients():
+    """B and C expanded over the rows (stride 0) are read in place and their gradients summed"""
+    v = scan_inputs(3, 70, 2, 1, 16, 16, torch.float32, seed=7)
+    one = {**v, "Bm": v["Bm"][:1], "C": v["C"][:1]}
+    leaves = {k: t.double().requires_grad_() for k, t in one.items()}
+    full = {**leaves, "Bm": leaves["Bm"].expand(3, -1, -1, -1), "C": leaves["C"].expand(3, -1, -1, -1)}
+    y, _ = ref_scan(*(full[k] for k in ("x", "dt", "A", "Bm", "C", "D", "bias")), True, full["state"], None)
+    want = torch.autograd.grad(y.sum(), [leaves["Bm"], leaves["C"]])
+    here = cuda(one, leaf=True)
+    out, _ = gpu_scan({**here, "Bm": here["Bm"].expand(3, -1, -1, -1), "C": here["C"].expand(3, -1, -1, -1)})
+    got = torch.autograd.grad(out.sum(), [here["Bm"], here["C"]])
+    assert all(off(a, b) <= tol(torch.float32) for a, b in zip(got, want))
+
+
+def test_refusals_of_the_convolution():
+    from rtfs_net_amd.ssm import causal_conv, causal_conv_step
+
+    x, w, s = torch.zeros(2, 5, 6), torch.zeros(6, 4), torch.zeros(2, 3, 6)
+    for bad in (lambda: causal_conv(x[0], w), lambda: causal_conv(x.half(), w), lambda: causal_conv(x, torch.zeros(6, 9)), lambda: causal_conv(x, w[:5]),
+                lambda: causal_conv(x, w.double()), lambda: causal_conv(x, w, torch.zeros(5)), lambda: causal_conv(x, w, state=s[:, :2]),
+                lambda: causal_conv(x, w, state=s.bfloat16()), lambda: causal_conv(x, w, lengths=torch.zeros(2)),
+                lambda: causal_conv(x, w, lengths=torch.zeros(3, dtype=torch.int32)), lambda: causal_conv_step(x[:, 0], s[:1], w),
+                lambda: causal_conv_step(x[:, 0], s.transpose(1, 2).contiguous().transpose(1, 2), w), lambda: causal_conv_step(x, s, w)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(TypeError):
+        causal_conv([1.0], w)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        causal_conv_step(x[:, 0], s, w.clone().requires_grad_())
+    with pytest.raises(RuntimeError, match="HIP"):
+        causal_conv(x, w)
+    with pytest.raises(RuntimeError, match="HIP"):
+        causal_conv_step(x[:, 0], s, w)
+
+
+def test_refusals_of_the_scan():
+    from rtfs_net_amd.ssm import selective_scan, selective_scan_step
+
+    x, dt, A, bc, s = torch.zeros(2, 5, 4, 8), torch.zeros(2, 5, 4), torch.zeros(4), torch.zeros(2, 5, 2, 3), torch.zeros(2, 4, 8, 3)
+    wide = torch.zeros(2, 5, 2, 129)
+    for bad in (lambda: selective_scan(x[0], dt, A, bc, bc), lambda: selective_scan(x.half(), dt, A, bc, bc), lambda: selective_scan(x, dt[:, :4], A, bc, bc),
+                lambda: selective_scan(x, dt.bfloat16(), A, bc, bc), lambda: selective_scan(x, dt, A[:3], bc, bc), lambda: selective_scan(x, dt, A.double(), bc, bc),
+                lambda: selective_scan(x, dt, A, bc, bc[..., :2]), lambda: selective_scan(x, dt, A, bc[:, :, :0], bc[:, :, :0]), lambda: selective_scan(x, dt, A, wide, wide),
+                lambda: selective_scan(x[:, :, :3], dt[..., :3], A[:3], bc, bc), lambda: selective_scan(torch.zeros(2, 5, 4, 129), dt, A, bc, bc),
+                lambda: selective_scan(x, dt, A, bc, bc, A[:2]), lambda: selective_scan(x, dt, A, bc, bc, dt_bias=A.bfloat16()),
+                lambda: selective_scan(x, dt, A, bc, bc, state=s[:1]), lambda: selective_scan(x, dt, A, bc, bc, state=s.bfloat16()),
+                lambda: selective_scan(x, dt, A, bc, bc, lengths=torch.zeros(2, dtype=torch.int64)), lambda: selective_scan(x, dt, A, bc.bfloat16(), bc),
+                lambda: selective_scan_step(x[:, 0], dt[:, 0], A, bc[:, 0], bc[:, 0], None), lambda: selective_scan_step(x[:, 0], dt[:, 0], A, bc[:, 0], bc[:, 0], s.bfloat16()),
+                lambda: selective_scan_step(x[:, 0], dt[:, 0], A, bc[:, 0], bc[:, 0], torch.zeros(2, 4, 3, 8).transpose(2, 3)),
+                lambda: selective_scan_step(x[:, 0], dt[:, 0], A, bc[:, 0], bc[:, 0], torch.zeros(193)[1:].view(2, 4, 8, 3)),
+                lambda: selective_scan(torch.zeros(1 << 23, 1, 4, 1), torch.zeros(1 << 23, 1, 4), A, torch.zeros(1 << 23, 1, 1, 1), torch.zeros(1 << 23, 1, 1, 1))):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(TypeError):
+        selective_scan(x, None, A, bc, bc)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        selective_scan_step(x[:, 0], dt[:, 0], A, bc[:, 0], bc[:, 0], s.clone().requires_grad_())
+    with pytest.raises(RuntimeError, match="HIP"):
+        selective_scan(x, dt, A, bc, bc)
+    with pytest.raises(RuntimeError, match="HIP"):
+        selective_scan_step(x[:, 0], dt[:, 0], A, bc[:, 0], bc[:, 0], s)
+
+
+def test_the_library_refuses_what_its_kernels_cannot_take():
+    """sizes and types outside the contract come back as an error before anything is launched (no device is touched)"""
+    from rtfs_net_amd import lib
+
+    h = lib.load()
+    one = 16  # an address that is never followed: the sizes are refused first
+    scan = lambda *dims: h.rtfs_ssm_scan_fwd(one, 1, 1, one, 1, 1, 0, one, one, 1, 1, one, 1, 1, None, None, 0, None, None, one, None, None, *dims, None)  # noqa: E731
+    for dims in ((0, 1, 1, 1, 1, 1, 0), (1, 0, 1, 1, 1, 1, 0), (1, 1, 3, 1, 2, 1, 0), (1, 1, 1, 129, 1, 1, 0), (1, 1, 1, 1, 1, 129, 0), (1, 1, 1, 1, 1, 1, 2)):
+        assert scan(*dims) == -1
+    assert scan(1, 4096, 1, 1, 1, 1, 0) == -1  # cut into segments, and no workspace for them
+    conv = lambda *dims: h.rtfs_causal_conv_fwd(one, 1, 1, one, None, None, None, one, None, *dims, None)  # noqa: E731
+    for dims in ((0, 1, 1, 1, 1, 0), (1, 1, 1, 9, 1, 0), (1, 1, 1, 0, 1, 0), (1, 1, 1, 1, 1, 3)):
+        assert conv(*dims) == -1
+    assert h.rtfs_ssm_tile(129, 1) == -1 and h.rtfs_ssm_tile(33, 65) == 64 * 128 and h.rtfs_causal_conv_bwd_work_floats(0, 4, 0) == -1
+    assert h.rtfs_ssm_scan_segments(1, 64 * 100, 1) == 25 and h.rtfs_ssm_scan_segments(512, 64 * 100, 1) == 1 and h.rtfs_ssm_scan_bwd_parts(1, 64, 8, 3) == -1
