@@ -54,22 +54,24 @@ template <> __device__ __forceinline__ Frag<__bf16> frag_of<__bf16>(f32x4 a, f32
     for (int j = 0; j < 4; ++j) f.v[j] = (__bf16)a[j], f.v[4 + j] = (__bf16)b[j];
     return f;
 }
-// An fp32 operand kept to 16 bits of mantissa as the sum of two bf16 (error 2^-17 of it): states and what feeds them are not rounded to 8 bits, nor are the
-// sums that the gradients of dt and A are differences of.  fp32 operands are themselves.
-template <typename T> struct Split { Frag<T> hi, lo; };
+// An fp32 operand as the sum of three bf16 (8 bits of mantissa each, error 2^-25 of it): states, what builds them, and the sums that the gradients of dt and A
+// are differences of keep fp32's precision for bf16 tensors too.  fp32 operands are themselves.
+template <typename T> struct Split { Frag<T> hi, mid, lo; };
 template <> struct Split<float> { Frag<float> hi; };
 __device__ __forceinline__ void split(f32x4 a, f32x4 b, Split<float>& s) { s.hi = {a, b}; }
 __device__ __forceinline__ void split(f32x4 a, f32x4 b, Split<__bf16>& s) {
     s.hi = frag_of<__bf16>(a, b);
-    f32x4 c, d;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c[j] = a[j] - (float)s.hi.v[j], d[j] = b[j] - (float)s.hi.v[4 + j];
-    s.lo = frag_of<__bf16>(c, d);
+    for (int j = 0; j < 4; ++j) a[j] -= (float)s.hi.v[j], b[j] -= (float)s.hi.v[4 + j];
+    s.mid = frag_of<__bf16>(a, b);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] -= (float)s.mid.v[j], b[j] -= (float)s.mid.v[4 + j];
+    s.lo = frag_of<__bf16>(a, b);
 }
 __device__ __forceinline__ f32x4 mma(const Split<float>& x, const Frag<float>& y, f32x4 c) { return mma(x.hi, y, c); }
-__device__ __forceinline__ f32x4 mma(const Split<__bf16>& x, const Frag<__bf16>& y, f32x4 c) { return mma(x.lo, y, mma(x.hi, y, c)); }
+__device__ __forceinline__ f32x4 mma(const Split<__bf16>& x, const Frag<__bf16>& y, f32x4 c) { return mma(x.hi, y, mma(x.mid, y, mma(x.lo, y, c))); }
 __device__ __forceinline__ f32x4 mma(const Frag<float>& x, const Split<float>& y, f32x4 c) { return mma(x, y.hi, c); }
-__device__ __forceinline__ f32x4 mma(const Frag<__bf16>& x, const Split<__bf16>& y, f32x4 c) { return mma(x, y.lo, mma(x, y.hi, c)); }
+__device__ __forceinline__ f32x4 mma(const Frag<__bf16>& x, const Split<__bf16>& y, f32x4 c) { return mma(x, y.hi, mma(x, y.mid, mma(x, y.lo, c))); }
 
 __device__ __forceinline__ void widen(const Frag<float>& f, f32x4& a, f32x4& b) { a = f.a, b = f.b; }
 __device__ __forceinline__ void widen(const Frag<__bf16>& f, f32x4& a, f32x4& b) {
@@ -99,14 +101,40 @@ template <typename T> __device__ __forceinline__ Vec8<T> zero8() {
     return v;
 }
 
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+// 8 values at byte offset `at`; an offset past every tensor (bounds are below 2^31) where there are none
+__device__ __forceinline__ void buffer_vec8(Vec8<__bf16>& v, __amdgpu_buffer_rsrc_t r, unsigned at, bool any, bool) {
+    v.v = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(r, any ? at : 0x80000000u, 0, 0));
+}
+__device__ __forceinline__ void buffer_vec8(Vec8<float>& v, __amdgpu_buffer_rsrc_t r, unsigned at, bool any, bool more) {
+    v.a = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, any ? at : 0x80000000u, 0, 0));
+    v.b = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, more ? at + 16 : 0x80000000u, 0, 0));
+}
+
 // A 64-token tile of up to COLS values per token, read by THREADS threads in units of 4 tokens x 8 values; what lies past `rows` tokens or `cols` values is
-// zero (never read: a padded batch may hold anything there).  `fast`: 16-byte loads (addresses, pitches and `cols` allow them).
+// zero (never read: a padded batch may hold anything there).  `fast` (addresses and pitches on 16 bytes, `cols` a multiple of 16 bytes): buffer loads, whose
+// bounds check supplies the zeros without a branch; else 16-byte loads at any address, and element by element where a unit crosses `cols`.
+// The loads stay in flight in `r` until rows() or columns() stores them to LDS: a tile is asked for one chunk ahead.
 template <typename T, int COLS, int THREADS>
 struct Tile {
     static constexpr int kUnits = 16 * (COLS / 8), kPer = (kUnits + THREADS - 1) / THREADS;
     Vec8<T> r[kPer][4];
 
     __device__ __forceinline__ void load(const T* src, long long row, int rows, int cols, bool fast) {
+        if (fast) {
+            // without a token the bound is 0: nothing is read (below 0 it would be no bound at all)
+            const int bytes = rows > 0 ? (int)(((rows - 1) * row + cols) * (long long)sizeof(T)) : 0;
+            const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(src), 0, bytes, 0x00027000);
+            const unsigned pitch = (unsigned)row * sizeof(T);
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) {
+                const int u = threadIdx.x + k * THREADS, c = (u >> 4) * 8;
+                unsigned at = (u & 15) * 4 * pitch + c * sizeof(T);
+#pragma unroll
+                for (int i = 0; i < 4; ++i, at += pitch) buffer_vec8(r[k][i], rsrc, at, c < cols, c + 4 < cols);
+            }
+            return;
+        }
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
             const int u = threadIdx.x + k * THREADS, c = (u >> 4) * 8;
@@ -116,11 +144,11 @@ struct Tile {
                 r[k][i] = zero8<T>();
                 if ((kUnits % THREADS == 0 || u < kUnits) && t < rows && c < cols) {
                     const T* p = src + t * row + c;
-                    if (fast) {
-                        r[k][i] = *reinterpret_cast<const Vec8<T>*>(p);
+                    if (c + 8 <= cols) {
+                        __builtin_memcpy(&r[k][i], p, sizeof(Vec8<T>));
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
+                        for (int j = 0; j < 7; ++j)
                             if (c + j < cols) r[k][i].set(j, p[j]);
                     }
                 }
@@ -157,6 +185,17 @@ struct Tile {
     }
 };
 
+// A product over tokens needs its operands with 8 neighbouring TOKENS per lane.  bf16 tiles are stored a second time with tokens innermost (16-byte reads);
+// fp32 ones are read across their rows, one value at a time: as many bytes per cycle, and LDS for one copy.
+template <typename T> constexpr bool kTwice = sizeof(T) == 2;
+__device__ __forceinline__ Frag<float> frag_down(const float* rows, int ld, const float*, int col, int t) {
+    Frag<float> f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f.a[j] = rows[(t + j) * ld + col], f.b[j] = rows[(t + 4 + j) * ld + col];
+    return f;
+}
+__device__ __forceinline__ Frag<__bf16> frag_down(const __bf16*, int, const __bf16* cols, int col, int t) { return frag(cols + col * pitch<__bf16>(kQ) + t); }
+
 // ---- decays ---------------------------------------------------------------------------------------------------------------------------------------------
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -186,13 +225,28 @@ __device__ __forceinline__ double running_sum(double v) {
     }
     return v;
 }
-// One wave, one token per lane: step and log2 decay (as two floats whose sum is the fp64 value to 48 bits).
+// One wave, one token per lane: log2 decay (as two floats whose sum is the fp64 value to 48 bits).
 __device__ __forceinline__ void chunk_decay(float step, float A, float& hi, float& lo) {
     const double s = running_sum((double)step * (double)A * 1.4426950408889634074);
     hi = (float)s;
     lo = (float)(s - (double)hi);
 }
+// What the products of a chunk take from its decays, per token: s as two floats, d, e^{s[t]}, e^{s[63]-s[t]}
+struct Decays {
+    float hi[kQ], lo[kQ], step[kQ], from[kQ], to[kQ];
+};
+
 __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// by one wave for one chunk; `raw`: this lane's dt (with bias), `alive`: whether its token is within the row
+__device__ __forceinline__ void put_decays(Decays& o, float raw, bool alive, bool plus, float A) {
+    const int lane = threadIdx.x & 63;
+    const float d = !alive ? 0.f : plus ? softplus(raw) : raw;
+    float hi, lo;
+    chunk_decay(d, A, hi, lo);
+    const float eh = __shfl(hi, 63, 64), el = __shfl(lo, 63, 64);
+    o.hi[lane] = hi, o.lo[lane] = lo, o.step[lane] = d, o.from[lane] = exp2_fast(hi), o.to[lane] = exp2_fast((eh - hi) + (el - lo));
+}
 
 // blocks that follow each other share inputs (heads of a group): hand each XCD a contiguous part of them (workgroup i runs on XCD i % 8)
 __device__ __forceinline__ unsigned xcd_block(unsigned i, unsigned n) {
@@ -247,10 +301,11 @@ inline ScanArgs scan_args(const void* x, long long x_row, long long x_tok, const
                           const void* C, long long c_row, long long c_tok, const float* D, const float* state, const int* lengths, int rows, int L, int H, int P,
                           int G, int N, int type) {
     ScanArgs a{x, B, C, x_row, x_tok, b_row, b_tok, c_row, c_tok, dt, A, D, state, lengths, rows, L, H, P, G, N, 1, 0, 0, 0, 0, 0};
-    const int v = type == 0 ? 4 : 8;
-    a.fast_x = P % 8 == 0 && x_row % v == 0 && x_tok % v == 0 && on16(x);
-    a.fast_b = N % 8 == 0 && b_row % v == 0 && b_tok % v == 0 && on16(B);
-    a.fast_c = N % 8 == 0 && c_row % v == 0 && c_tok % v == 0 && on16(C);
+    const int v = type == 0 ? 4 : 8;  // values in 16 bytes; 64 tokens must lie within 2^31 bytes of each other
+    auto fast = [&](const void* p, int width, long long row, long long tok) {
+        return width % v == 0 && row % v == 0 && tok % v == 0 && tok >= 0 && tok < (1ll << 23) && on16(p);
+    };
+    a.fast_x = fast(x, P, x_row, x_tok), a.fast_b = fast(B, N, b_row, b_tok), a.fast_c = fast(C, N, c_row, c_tok);
     scan_cut(a);
     return a;
 }

@@ -22,13 +22,23 @@ __device__ __forceinline__ void scan_place(const ScanArgs& a, int& b, int& seg, 
 // C B^T is shared out by tiles of the lower triangle and meets the decays on its way to LDS; D joins its diagonal.
 // Roundings (bf16): the scores times decay and step, and the state as it enters the product with C, once each to bf16 - y is rounded to that anyway; the
 // weighted inputs that build the state are kept as two bf16 (ssm.h), so the state that is handed on is good to 2^-17.
+template <typename T, int NP, int PP> struct ScanTiles {
+    static constexpr int kN = pitch<T>(NP), kP = pitch<T>(PP), kT = pitch<T>(kQ);
+    static constexpr int kBt = kTwice<T> ? NP * kT : 0, kX = kTwice<T> ? PP * kT : kQ * kP;
+    static constexpr int kBytes = (2 * kQ * kN + kBt + kX + kQ * kT) * (int)sizeof(T) + Waves<PP>::kWaves * (int)sizeof(Decays);
+    // waves per SIMD: two (256 registers each) where a CU's LDS holds as many workgroups, else one
+    static constexpr int kWavesPerSimd = kBytes * 2 <= 160 * 1024 ? 2 : 1;
+};
+
 template <typename T, int NP, int PP>
-__global__ __launch_bounds__(Waves<PP>::kThreads) void scan_kernel(ScanArgs a, const float* __restrict__ starts, T* __restrict__ y, float* __restrict__ last) {
+__global__ __launch_bounds__(Waves<PP>::kThreads, (ScanTiles<T, NP, PP>::kWavesPerSimd)) void scan_kernel(ScanArgs a, const float* __restrict__ starts,
+                                                                                                         T* __restrict__ y, float* __restrict__ last) {
     typedef Waves<PP> W;
+    typedef ScanTiles<T, NP, PP> S_;
     typedef T T4 __attribute__((ext_vector_type(4)));
-    constexpr int kN = pitch<T>(NP), kT = pitch<T>(kQ);
-    __shared__ __attribute__((aligned(16))) T Bs[kQ * kN], Cs[kQ * kN], Bt[NP * kT], Xt[PP * kT], Ms[kQ * kT];
-    __shared__ __attribute__((aligned(16))) float hi[kQ], lo[kQ], step[kQ], from[kQ], to[kQ];
+    constexpr int kN = S_::kN, kP = S_::kP, kT = S_::kT;
+    __shared__ __attribute__((aligned(16))) T Bs[kQ * kN], Cs[kQ * kN], Bt[S_::kBt + 1], Xs[S_::kX], Ms[kQ * kT];
+    __shared__ __attribute__((aligned(16))) Decays decays[W::kWaves];
     int b, seg, h;
     scan_place(a, b, seg, h);
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, lc = lane & 15, g = lane >> 4;
@@ -55,34 +65,37 @@ __global__ __launch_bounds__(Waves<PP>::kThreads) void scan_kernel(ScanArgs a, c
         }
     for (int i = threadIdx.x; i < kQ * kT; i += W::kThreads) Ms[i] = (T)0.f;
 
-    const int c0 = seg * a.seg_chunks, c1 = c0 + a.seg_chunks < a.chunks ? c0 + a.seg_chunks : a.chunks;
-    for (int c = c0; c < c1; ++c) {
-        const int t0 = c * kQ, rows = len - t0 < kQ ? len - t0 : kQ, all = a.L - t0 < kQ ? a.L - t0 : kQ;
-        T* out = y + (((long long)b * a.L + t0) * a.H + h) * a.P;
-        if (rows <= 0) {  // behind this row's end: nothing but zeros
-            for (int i = threadIdx.x; i < all * a.P; i += W::kThreads) out[(long long)(i / a.P) * a.H * a.P + i % a.P] = (T)0.f;
-            continue;
-        }
-        Tile<T, NP, W::kThreads> tb, tc;
-        Tile<T, PP, W::kThreads> tx;
+    const int c0 = seg * a.seg_chunks, c_all = c0 + a.seg_chunks < a.chunks ? c0 + a.seg_chunks : a.chunks;
+    const int c_len = (len + kQ - 1) / kQ, c1 = c_all < c_len ? c_all : c_len;
+    Tile<T, NP, W::kThreads> tb, tc;
+    Tile<T, PP, W::kThreads> tx;
+    float raw = 0.f;
+    auto ask = [&](int c) {
+        const long long t0 = (long long)c * kQ;
+        const int rows = len - t0 < kQ ? (int)(len - t0) : kQ;
         tb.load(Bg + t0 * a.b_tok, a.b_tok, rows, a.N, a.fast_b);
         tc.load(Cg + t0 * a.c_tok, a.c_tok, rows, a.N, a.fast_c);
         tx.load(x + t0 * a.x_tok, a.x_tok, rows, a.P, a.fast_x);
-        float d = 0.f, dh, dl;
-        if (w == 0) {
-            if (lane < rows) {
-                d = a.dt.raw(b, t0 + lane, h);
-                if (a.dt.softplus) d = softplus(d);
-            }
-            chunk_decay(d, A, dh, dl);
-        }
+    };
+    auto ask_step = [&](int c) {  // the steps of as many chunks as there are waves, one chunk per wave
+        const int t = (c + w) * kQ + lane;
+        raw = t < len ? a.dt.raw(b, t, h) : 0.f;
+    };
+    if (c0 < c1) ask(c0), ask_step(c0);
+    for (int c = c0; c < c1; ++c) {
+        const int t0 = c * kQ, rows = len - t0 < kQ ? len - t0 : kQ, all = a.L - t0 < kQ ? a.L - t0 : kQ, which = (c - c0) % W::kWaves;
+        T* out = y + (((long long)b * a.L + t0) * a.H + h) * a.P;
         __syncthreads();  // the chunk before has been read
-        tb.rows(Bs), tb.columns(Bt), tc.rows(Cs), tx.columns(Xt);
-        if (w == 0) {
-            const float eh = __shfl(dh, 63, 64), el = __shfl(dl, 63, 64);
-            hi[lane] = dh, lo[lane] = dl, step[lane] = d, from[lane] = exp2_fast(dh), to[lane] = exp2_fast((eh - dh) + (el - dl)) * d;
+        tb.rows(Bs), tc.rows(Cs);
+        if constexpr (kTwice<T>) tb.columns(Bt), tx.columns(Xs);
+        else tx.rows(Xs);
+        if (which == 0) {
+            put_decays(decays[w], raw, (c + w) * kQ + lane < len, a.dt.softplus, A);
+            if (c + W::kWaves < c1) ask_step(c + W::kWaves);
         }
+        if (c + 1 < c1) ask(c + 1);
         __syncthreads();
+        const Decays& e = decays[which];
         // scores of the tiles on and below the diagonal: lane l holds token t = its column, four tokens j = its rows
         for (int i = w; i < 10; i += W::kWaves) {
             const int tt = i < 1 ? 0 : i < 3 ? 1 : i < 6 ? 2 : 3, ss = i - tt * (tt + 1) / 2;
@@ -91,11 +104,12 @@ __global__ __launch_bounds__(Waves<PP>::kThreads) void scan_kernel(ScanArgs a, c
             for (int k = 0; k < NP / 32; ++k)
                 m = mma(frag(Bs + (16 * ss + lc) * kN + 32 * k + 8 * g), frag(Cs + (16 * tt + lc) * kN + 32 * k + 8 * g), m);
             const int t = 16 * tt + lc, j = 16 * ss + 4 * g;
-            const float th = hi[t], tl = lo[t];
+            const float th = e.hi[t], tl = e.lo[t];
+            const f32x4 jh = *reinterpret_cast<const f32x4*>(e.hi + j), jl = *reinterpret_cast<const f32x4*>(e.lo + j), d = *reinterpret_cast<const f32x4*>(e.step + j);
             T4 v;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float s = m[i] * exp2_fast((th - hi[j + i]) + (tl - lo[j + i])) * step[j + i];
+                const float s = m[i] * exp2_fast((th - jh[i]) + (tl - jl[i])) * d[i];
                 v[i] = (T)(j + i < t ? s : j + i == t ? s + D : 0.f);
             }
             *reinterpret_cast<T4*>(Ms + t * kT + j) = v;
@@ -119,26 +133,29 @@ __global__ __launch_bounds__(Waves<PP>::kThreads) void scan_kernel(ScanArgs a, c
         }
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
-            const float f = from[16 * tt + lc];
+            const float f = e.from[16 * tt + lc];
 #pragma unroll
             for (int pt = 0; pt < W::kTiles; ++pt) acc[pt][tt] *= f;
         }
         // the state, before the barrier that the scores wait for
-        const float whole = from[kQ - 1];
+        const float whole = e.from[kQ - 1];
 #pragma unroll
         for (int pt = 0; pt < W::kTiles; ++pt) {
             Split<T> xs[2];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 f32x4 u, v;
-                widen(frag(Xt + (16 * (w * W::kTiles + pt) + lc) * kT + 32 * k + 8 * g), u, v);
-                split(u * *reinterpret_cast<const f32x4*>(to + 32 * k + 8 * g), v * *reinterpret_cast<const f32x4*>(to + 32 * k + 8 * g + 4), xs[k]);
+                widen(frag_down(Xs, kP, Xs, 16 * (w * W::kTiles + pt) + lc, 32 * k + 8 * g), u, v);
+                const float *to = e.to + 32 * k + 8 * g, *d = e.step + 32 * k + 8 * g;
+                u *= *reinterpret_cast<const f32x4*>(to) * *reinterpret_cast<const f32x4*>(d);
+                v *= *reinterpret_cast<const f32x4*>(to + 4) * *reinterpret_cast<const f32x4*>(d + 4);
+                split(u, v, xs[k]);
             }
 #pragma unroll
             for (int nt = 0; nt < NP / 16; ++nt) {
                 f32x4 s = S[nt][pt] * whole;
 #pragma unroll
-                for (int k = 0; k < 2; ++k) s = mma(frag(Bt + (16 * nt + lc) * kT + 32 * k + 8 * g), xs[k], s);
+                for (int k = 0; k < 2; ++k) s = mma(frag_down(Bs, kN, Bt, 16 * nt + lc, 32 * k + 8 * g), xs[k], s);
                 S[nt][pt] = s;
             }
         }
@@ -147,7 +164,7 @@ __global__ __launch_bounds__(Waves<PP>::kThreads) void scan_kernel(ScanArgs a, c
         for (int pt = 0; pt < W::kTiles; ++pt) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const Frag<T> q = frag(Xt + (16 * (w * W::kTiles + pt) + lc) * kT + 32 * k + 8 * g);
+                const Frag<T> q = frag_down(Xs, kP, Xs, 16 * (w * W::kTiles + pt) + lc, 32 * k + 8 * g);
 #pragma unroll
                 for (int tt = 2 * k; tt < 4; ++tt) acc[pt][tt] = mma(q, frag(Ms + (16 * tt + lc) * kT + 32 * k + 8 * g), acc[pt][tt]);
             }
@@ -171,6 +188,12 @@ __global__ __launch_bounds__(Waves<PP>::kThreads) void scan_kernel(ScanArgs a, c
             }
         }
     }
+    // chunks behind this row's end: nothing but zeros
+    for (int c = c0 > c1 ? c0 : c1; c < c_all; ++c) {
+        const int t0 = c * kQ, all = a.L - t0 < kQ ? a.L - t0 : kQ;
+        T* out = y + (((long long)b * a.L + t0) * a.H + h) * a.P;
+        for (int i = threadIdx.x; i < all * a.P; i += W::kThreads) out[(long long)(i / a.P) * a.H * a.P + i % a.P] = (T)0.f;
+    }
     if (last && seg == a.segs - 1) {
 #pragma unroll
         for (int nt = 0; nt < NP / 16; ++nt)
@@ -192,10 +215,21 @@ __global__ __launch_bounds__(Waves<PP>::kThreads) void scan_kernel(ScanArgs a, c
 // state, from the gradient of the next chunk's)  S <- e^{s[63]} S + sum_t e^{s[t]} dy[t] C[t]^T.  `x` and `B` of the arguments are dy and C then.
 // Two uses: a first pass over the segments of a row when rows and heads are too few to fill the chip (`ends`, `decays`: each segment's own state from zero,
 // which scan_join_kernel chains), and the states in front of every chunk for the gradients (`tiles`: accumulator tiles as they lie, 1 KB each).
+template <typename T, int NP, int PP> struct WalkTiles {
+    static constexpr int kN = pitch<T>(NP), kP = pitch<T>(PP), kT = pitch<T>(kQ);
+    static constexpr int kB = kTwice<T> ? NP * kT : kQ * kN, kX = kTwice<T> ? PP * kT : kQ * kP;
+};
+
+// two walks in one launch (blockIdx.y): the gradients need both directions at once
 template <typename T, int NP, int PP>
-__device__ __forceinline__ void scan_walk(const ScanArgs& a, const WalkOut& o, T* Bt, T* Xt, float* to, float* end) {
+__global__ __launch_bounds__(Waves<PP>::kThreads, 2) void scan_walk_kernel(ScanArgs a0, WalkOut o0, ScanArgs a1, WalkOut o1) {
     typedef Waves<PP> W;
-    constexpr int kT = pitch<T>(kQ);
+    constexpr int kN = pitch<T>(NP), kP = pitch<T>(PP);
+    __shared__ __attribute__((aligned(16))) T Bs[WalkTiles<T, NP, PP>::kB], Xs[WalkTiles<T, NP, PP>::kX];
+    __shared__ __attribute__((aligned(16))) Decays decays[W::kWaves];
+    ScanArgs a = a0;
+    WalkOut o = o0;
+    if (blockIdx.y) a = a1, o = o1;
     int b, seg, h;
     scan_place(a, b, seg, h);
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, lc = lane & 15, g = lane >> 4;
@@ -219,10 +253,27 @@ __device__ __forceinline__ void scan_walk(const ScanArgs& a, const WalkOut& o, T
                 S[pt][nt][i] = v;
             }
         }
-    double sum = 0.0;
+    // step k of the walk is chunk k, or the k-th from the back
     const int k0 = seg * a.seg_chunks, k1 = k0 + a.seg_chunks < a.chunks ? k0 + a.seg_chunks : a.chunks;
+    auto chunk = [&](int k) { return o.backwards ? a.chunks - 1 - k : k; };
+    Tile<T, NP, W::kThreads> tb;
+    Tile<T, PP, W::kThreads> tx;
+    float raw = 0.f;
+    double sum = 0.0;
+    auto ask = [&](int k) {
+        const long long t0 = (long long)chunk(k) * kQ;
+        if (t0 >= len) return;
+        const int rows = len - t0 < kQ ? (int)(len - t0) : kQ;
+        tb.load(Bg + t0 * a.b_tok, a.b_tok, rows, a.N, a.fast_b);
+        tx.load(x + t0 * a.x_tok, a.x_tok, rows, a.P, a.fast_x);
+    };
+    auto ask_step = [&](int k) {
+        const long long t = (long long)chunk(k + w) * kQ + lane;
+        raw = k + w < k1 && t < len ? a.dt.raw(b, t, h) : 0.f;
+    };
+    ask(k0), ask_step(k0);
     for (int k = k0; k < k1; ++k) {
-        const int c = o.backwards ? a.chunks - 1 - k : k, t0 = c * kQ, rows = len - t0 < kQ ? len - t0 : kQ;
+        const int c = chunk(k), t0 = c * kQ, which = (k - k0) % W::kWaves;
         if (o.tiles) {
             float* to_tile = o.tiles + (((long long)b * a.chunks + c) * a.H + h) * PP * NP;
 #pragma unroll
@@ -231,43 +282,42 @@ __device__ __forceinline__ void scan_walk(const ScanArgs& a, const WalkOut& o, T
                 for (int nt = 0; nt < NP / 16; ++nt)
                     *reinterpret_cast<f32x4*>(to_tile + ((w * W::kTiles + pt) * (NP / 16) + nt) * 256 + lane * 4) = S[pt][nt];
         }
-        if (rows <= 0) continue;
-        Tile<T, NP, W::kThreads> tb;
-        Tile<T, PP, W::kThreads> tx;
-        tb.load(Bg + t0 * a.b_tok, a.b_tok, rows, a.N, a.fast_b);
-        tx.load(x + t0 * a.x_tok, a.x_tok, rows, a.P, a.fast_x);
-        float d = 0.f, dh, dl;
-        if (w == 0) {
-            if (lane < rows) {
-                d = a.dt.raw(b, t0 + lane, h);
-                if (a.dt.softplus) d = softplus(d);
-            }
-            chunk_decay(d, A, dh, dl);
-            sum += (double)__shfl(dh, 63, 64) + (double)__shfl(dl, 63, 64);
-        }
         __syncthreads();
-        tb.columns(Bt), tx.columns(Xt);
-        if (w == 0) {
-            const float eh = __shfl(dh, 63, 64), el = __shfl(dl, 63, 64);
-            to[lane] = o.backwards ? (lane < rows ? exp2_fast(dh) : 0.f) : exp2_fast((eh - dh) + (el - dl)) * d;
-            if (lane == 63) *end = exp2_fast(dh);
+        if (t0 < len) {
+            if constexpr (kTwice<T>) tb.columns(Bs), tx.columns(Xs);
+            else tb.rows(Bs), tx.rows(Xs);
         }
+        if (which == 0) {
+            put_decays(decays[w], raw, k + w < k1 && (long long)chunk(k + w) * kQ + lane < len, a.dt.softplus, A);
+            if (k + W::kWaves < k1) ask_step(k + W::kWaves);
+        }
+        if (k + 1 < k1) ask(k + 1);
         __syncthreads();
-        const float whole = *end;
+        if (t0 >= len) continue;
+        const Decays& e = decays[which];
+        sum += (double)e.hi[kQ - 1] + (double)e.lo[kQ - 1];
+        const float whole = e.from[kQ - 1];
 #pragma unroll
         for (int pt = 0; pt < W::kTiles; ++pt) {
             Split<T> xs[2];
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
                 f32x4 u, v;
-                widen(frag(Xt + (16 * (w * W::kTiles + pt) + lc) * kT + 32 * q + 8 * g), u, v);
-                split(u * *reinterpret_cast<const f32x4*>(to + 32 * q + 8 * g), v * *reinterpret_cast<const f32x4*>(to + 32 * q + 8 * g + 4), xs[q]);
+                widen(frag_down(Xs, kP, Xs, 16 * (w * W::kTiles + pt) + lc, 32 * q + 8 * g), u, v);
+                const int t = 32 * q + 8 * g;
+                if (o.backwards) {
+                    u *= *reinterpret_cast<const f32x4*>(e.from + t), v *= *reinterpret_cast<const f32x4*>(e.from + t + 4);
+                } else {
+                    u *= *reinterpret_cast<const f32x4*>(e.to + t) * *reinterpret_cast<const f32x4*>(e.step + t);
+                    v *= *reinterpret_cast<const f32x4*>(e.to + t + 4) * *reinterpret_cast<const f32x4*>(e.step + t + 4);
+                }
+                split(u, v, xs[q]);
             }
 #pragma unroll
             for (int nt = 0; nt < NP / 16; ++nt) {
                 f32x4 s = S[pt][nt] * whole;
 #pragma unroll
-                for (int q = 0; q < 2; ++q) s = mma(xs[q], frag(Bt + (16 * nt + lc) * kT + 32 * q + 8 * g), s);
+                for (int q = 0; q < 2; ++q) s = mma(xs[q], frag_down(Bs, kN, Bs, 16 * nt + lc, 32 * q + 8 * g), s);
                 S[pt][nt] = s;
             }
         }
@@ -286,17 +336,6 @@ __device__ __forceinline__ void scan_walk(const ScanArgs& a, const WalkOut& o, T
             }
         }
     if (o.decays && threadIdx.x == 0) o.decays[((long long)b * a.H + h) * a.segs + seg] = exp2_fast((float)sum);
-}
-
-// two walks in one launch (blockIdx.y): the gradients need both directions at once
-template <typename T, int NP, int PP>
-__global__ __launch_bounds__(Waves<PP>::kThreads) void scan_walk_kernel(ScanArgs a0, WalkOut o0, ScanArgs a1, WalkOut o1) {
-    constexpr int kT = pitch<T>(kQ);
-    __shared__ __attribute__((aligned(16))) T Bt[NP * kT], Xt[PP * kT];
-    __shared__ __attribute__((aligned(16))) float to[kQ];
-    __shared__ float end;
-    if (blockIdx.y == 0) scan_walk<T, NP, PP>(a0, o0, Bt, Xt, to, &end);
-    else scan_walk<T, NP, PP>(a1, o1, Bt, Xt, to, &end);
 }
 
 // Chains the segments' own states: ends[i] becomes the state in front of segment i.  One thread per state element walks the segments.
