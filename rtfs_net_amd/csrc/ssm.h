@@ -120,7 +120,9 @@ struct Tile {
     static constexpr int kUnits = 16 * (COLS / 8), kPer = (kUnits + THREADS - 1) / THREADS;
     Vec8<T> r[kPer][4];
 
-    __device__ __forceinline__ void load(const T* src, long long row, int rows, int cols, bool fast) {
+    __device__ __forceinline__ void load(int thread, const T* src, long long row, int rows, int cols, bool fast) {
+        // formed anew at every call: hoisted out of the chunk loop, the addresses of the element-wise path alone take a hundred registers
+        asm volatile("" : "+v"(thread));
         if (fast) {
             // without a token the bound is 0: nothing is read (below 0 it would be no bound at all)
             const int bytes = rows > 0 ? (int)(((rows - 1) * row + cols) * (long long)sizeof(T)) : 0;
@@ -128,7 +130,7 @@ struct Tile {
             const unsigned pitch = (unsigned)row * sizeof(T);
 #pragma unroll
             for (int k = 0; k < kPer; ++k) {
-                const int u = threadIdx.x + k * THREADS, c = (u >> 4) * 8;
+                const int u = thread + k * THREADS, c = (u >> 4) * 8;
                 unsigned at = (u & 15) * 4 * pitch + c * sizeof(T);
 #pragma unroll
                 for (int i = 0; i < 4; ++i, at += pitch) buffer_vec8(r[k][i], rsrc, at, c < cols, c + 4 < cols);
@@ -137,7 +139,7 @@ struct Tile {
         }
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
-            const int u = threadIdx.x + k * THREADS, c = (u >> 4) * 8;
+            const int u = thread + k * THREADS, c = (u >> 4) * 8;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int t = (u & 15) * 4 + i;
@@ -155,23 +157,23 @@ struct Tile {
             }
         }
     }
-    __device__ __forceinline__ void rows(T* dst) const {  // dst[token][value]
+    __device__ __forceinline__ void rows(int thread, T* dst) const {  // dst[token][value]
         constexpr int ld = pitch<T>(COLS);
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
-            const int u = threadIdx.x + k * THREADS, c = (u >> 4) * 8, t = (u & 15) * 4;
+            const int u = thread + k * THREADS, c = (u >> 4) * 8, t = (u & 15) * 4;
             if (kUnits % THREADS == 0 || u < kUnits) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) *reinterpret_cast<Vec8<T>*>(dst + (t + i) * ld + c) = r[k][i];
             }
         }
     }
-    __device__ __forceinline__ void columns(T* dst) const {  // dst[value][token]
+    __device__ __forceinline__ void columns(int thread, T* dst) const {  // dst[value][token]
         constexpr int ld = pitch<T>(kQ);
         typedef T T4 __attribute__((ext_vector_type(4)));
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
-            const int u = threadIdx.x + k * THREADS, c = (u >> 4) * 8, t = (u & 15) * 4;
+            const int u = thread + k * THREADS, c = (u >> 4) * 8, t = (u & 15) * 4;
             if (kUnits % THREADS == 0 || u < kUnits) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -194,7 +196,28 @@ __device__ __forceinline__ Frag<float> frag_down(const float* rows, int ld, cons
     for (int j = 0; j < 4; ++j) f.a[j] = rows[(t + j) * ld + col], f.b[j] = rows[(t + 4 + j) * ld + col];
     return f;
 }
+// the same across the rows of a tile whatever its type (one value at a time: for products outside the loops)
+template <typename T>
+__device__ __forceinline__ Frag<T> frag_across(const T* rows, int ld, int col, int t) {
+    f32x4 a, b;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] = (float)rows[(t + j) * ld + col], b[j] = (float)rows[(t + 4 + j) * ld + col];
+    return frag_of<T>(a, b);
+}
+// "pair" order: tokens t .. t + 3 and t + 16 .. t + 19
+__device__ __forceinline__ Frag<float> frag_down_pair(const float* rows, int ld, const float*, int col, int t) {
+    Frag<float> f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f.a[j] = rows[(t + j) * ld + col], f.b[j] = rows[(t + 16 + j) * ld + col];
+    return f;
+}
+__device__ __forceinline__ Frag<__bf16> frag_down_pair(const __bf16*, int, const __bf16* cols, int col, int t) {
+    return frag(cols + col * pitch<__bf16>(kQ) + t, cols + col * pitch<__bf16>(kQ) + t + 16);
+}
 __device__ __forceinline__ Frag<__bf16> frag_down(const __bf16*, int, const __bf16* cols, int col, int t) { return frag(cols + col * pitch<__bf16>(kQ) + t); }
+
+// this wave's index, known to the compiler to be the same in all its lanes
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // ---- decays ---------------------------------------------------------------------------------------------------------------------------------------------
 constexpr float kLog2e = 1.4426950408889634f;

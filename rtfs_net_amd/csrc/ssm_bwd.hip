@@ -23,20 +23,39 @@ struct GradArgs {
 };
 
 // One workgroup takes a chunk for a group's heads (or a part of them, where rows, chunks and groups are too few): C B^T is formed once, and the gradients of B
-// and C are summed over the heads in registers, in order.  Wave w owns tokens 16 w .. 16 w + 15 as the columns j of the score tiles - their accumulators are
-// then operands of dx as they lie - and every fourth 16-wide slice of N for the products with H and G, whose tiles it loads from memory as operands.  P goes
-// through in blocks of 64.  What a and d(step) need is summed in fp32 from products of split operands (ssm.h); what only dx, dB and dC need is rounded to the
-// tensors' type once on its way into a product.
+// and C are summed over the heads in registers, in order.  Two shares of work per wave:
+//   scores: wave w owns tokens 16 (w % 4) .. as the columns j of the score tiles (with eight waves, every other one of their row tiles) - these accumulators
+//           are operands of dx as they lie;
+//   states: the first half of the waves forms U = dy H, the other V = x G, each for its 16-wide slices of N; the tiles of H and G come from memory as operands.
+// P goes through in blocks of 64.  Steps and decays are made for four heads at a time, one per wave, and the per-token sums of four heads are finished at a
+// time likewise: on one wave they were a third of a head's time.  x and dy are asked for one block ahead.
+// What a and d(step) need is summed in fp32 from products of split operands (ssm.h); what only dx, dB and dC need is rounded to the tensors' type once on its
+// way into a product.
+constexpr int kRing = 4;  // heads per ring of decays and sums
+
+struct HeadSums {
+    float rowZ[4][kQ], dotU[4][kQ], dotV[4][kQ], colZ[2][kQ], diagZ[kQ], diagV[kQ], crossing[4];
+};
+
+template <typename T, int NP, int PP> struct GradTiles {
+    static constexpr int kWaves = NP == 128 ? 8 : 4, kThreads = 64 * kWaves, kHalf = kWaves / 2, kAlt = kWaves / 4;
+    static constexpr int kSlices = NP / 16 / kHalf;  // 16-wide slices of N per wave
+    static constexpr int PB = PP < 64 ? PP : 64, kBlocks = PP / PB;
+    static constexpr int kN = pitch<T>(NP), kT = pitch<T>(kQ), kP = pitch<T>(PB);
+    static constexpr int kYt = kTwice<T> ? PB * kT : 0, kMain = 2 * kQ * kP + kYt + PB * kN, kPool = kMain > kQ * kT ? kMain : kQ * kT;
+    static constexpr int kBytes = (2 * kQ * kN + kPool) * (int)sizeof(T) + kRing * (int)(sizeof(Decays) + sizeof(HeadSums));
+    static constexpr int kWavesPerSimd = kWaves == 8 || kBytes * 2 <= 160 * 1024 ? 2 : 1;
+};
+
 template <typename T, int NP, int PP>
-__global__ __launch_bounds__(256) void scan_grad_kernel(GradArgs q) {
+__global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP, PP>::kWavesPerSimd)) void scan_grad_kernel(GradArgs q) {
+    typedef GradTiles<T, NP, PP> S;
     typedef T T4 __attribute__((ext_vector_type(4)));
-    constexpr int PB = PP < 64 ? PP : 64, kN = pitch<T>(NP), kT = pitch<T>(kQ), kP = pitch<T>(PB);
-    constexpr int NT = NP / 64 > 0 ? NP / 64 : 1;  // slices of N per wave
-    constexpr int kMain = 2 * kQ * kP + PB * kT + PB * kN, kEnd = kQ * kT + NP * kT;
-    __shared__ __attribute__((aligned(16))) T Bs[kQ * kN], Cs[kQ * kN], pool[kMain > kEnd ? kMain : kEnd];
-    __shared__ __attribute__((aligned(16))) float hi[kQ], lo[kQ], step[kQ], from[kQ], to[kQ];
-    __shared__ float rowZ[4][kQ], dotU[4][kQ], dotV[4][kQ], colZ[kQ], diagZ[kQ], diagV[kQ], crossing[4];
-    T *Ys = pool, *Xs = Ys + kQ * kP, *Yt = Xs + kQ * kP, *Gt = Yt + PB * kT;
+    constexpr int PB = S::PB, kN = S::kN, kT = S::kT, kP = S::kP, NS = S::kSlices;
+    __shared__ __attribute__((aligned(16))) T Bs[kQ * kN], Cs[kQ * kN], pool[S::kPool];
+    __shared__ __attribute__((aligned(16))) Decays decays[kRing];
+    __shared__ __attribute__((aligned(16))) HeadSums sums[kRing];
+    T *Ys = pool, *Xs = Ys + kQ * kP, *Gt = Xs + kQ * kP, *Yt = Gt + PB * kN;
     const ScanArgs& a = q.a;
     unsigned i0 = xcd_block(blockIdx.x, gridDim.x);
     const int part = (int)(i0 % q.parts);
@@ -44,103 +63,96 @@ __global__ __launch_bounds__(256) void scan_grad_kernel(GradArgs q) {
     const int grp = (int)(i0 % a.G);
     i0 /= a.G;
     const int c = (int)(i0 % a.chunks), b = (int)(i0 / a.chunks);
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, lc = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, w = wave_index(), lc = lane & 15, g = lane >> 4;
     const int len = row_length(a.lengths, b, a.L), t0 = c * kQ, all = a.L - t0 < kQ ? a.L - t0 : kQ, rows = len - t0 < 0 ? 0 : len - t0 < kQ ? len - t0 : kQ;
     const int each = a.H / a.G, h0 = grp * each + part * q.part_heads, h1 = h0 + q.part_heads < (grp + 1) * each ? h0 + q.part_heads : (grp + 1) * each;
-    const T* Bg = static_cast<const T*>(a.B) + b * a.b_row + t0 * a.b_tok + (long long)grp * a.N;
-    const T* Cg = static_cast<const T*>(a.C) + b * a.c_row + t0 * a.c_tok + (long long)grp * a.N;
+    const int blocks = (a.P + PB - 1) / PB;  // of P that hold anything
+    const int jt = w & 3, alt = w >> 2, j = 16 * jt + lc;  // this lane's column of the score tiles
+    const bool role_v = w >= S::kHalf;
+    const int first = role_v ? w - S::kHalf : w;
+    const T *Rs = role_v ? Xs : Ys, *Ks = role_v ? Bs : Cs;
+    const float *mine = role_v ? q.behind : q.front;
     {
-        Tile<T, NP, 256> tile;
-        tile.load(Bg, a.b_tok, rows, a.N, a.fast_b);
-        tile.rows(Bs);
-        tile.load(Cg, a.c_tok, rows, a.N, a.fast_c);
-        tile.rows(Cs);
+        const T* Bg = static_cast<const T*>(a.B) + b * a.b_row + t0 * a.b_tok + (long long)grp * a.N;
+        const T* Cg = static_cast<const T*>(a.C) + b * a.c_row + t0 * a.c_tok + (long long)grp * a.N;
+        Tile<T, NP, S::kThreads> tile;
+        tile.load(threadIdx.x, Bg, a.b_tok, rows, a.N, a.fast_b);
+        tile.rows(threadIdx.x, Bs);
+        tile.load(threadIdx.x, Cg, a.c_tok, rows, a.N, a.fast_c);
+        tile.rows(threadIdx.x, Cs);
     }
+    Tile<T, PB, 128> ahead;  // x by waves 0 and 1, dy by waves 2 and 3
+    auto ask = [&](int h, int p0) {
+        const T* src = w < 2 ? static_cast<const T*>(a.x) + b * a.x_row + t0 * a.x_tok : static_cast<const T*>(q.dy) + ((long long)b * a.L + t0) * a.H * a.P;
+        if (w < 4)
+            ahead.load(threadIdx.x & 127, src + (long long)h * a.P + p0, w < 2 ? a.x_tok : (long long)a.H * a.P, rows, a.P - p0, w < 2 ? a.fast_x : q.fast_dy);
+    };
+    float raw = 0.f;
+    auto ask_step = [&](int h) { raw = w < kRing && h + w < h1 && lane < rows ? a.dt.raw(b, t0 + lane, h + w) : 0.f; };
+    ask(h0, 0), ask_step(h0);
     __syncthreads();
-    const int j = 16 * w + lc;  // this lane's column of the score tiles
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    f32x4 cb[4], dcb[4], dBa[4][NT], dCa[4][NT];  // rows t, columns j; rows t, columns n
+    f32x4 cb[4], dcb[4], sum[4][NS];  // rows t, columns j; rows t, columns n
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) {
         cb[tt] = dcb[tt] = zero;
-        if (tt >= w)
+        if (tt >= jt)
 #pragma unroll
             for (int k = 0; k < NP / 32; ++k) cb[tt] = mma(frag(Cs + (16 * tt + lc) * kN + 32 * k + 8 * g), frag(Bs + j * kN + 32 * k + 8 * g), cb[tt]);
 #pragma unroll
-        for (int s = 0; s < NT; ++s) dBa[tt][s] = dCa[tt][s] = zero;
+        for (int s = 0; s < NS; ++s) sum[tt][s] = zero;
     }
     for (int h = h0; h < h1; ++h) {
-        const float A = a.A[h], D = a.D ? a.D[h] : 0.f;
-        float raw = 0.f;
-        if (w == 0) {
-            float d = 0.f, dh, dl;
-            if (lane < rows) {
-                d = raw = a.dt.raw(b, t0 + lane, h);
-                if (a.dt.softplus) d = softplus(d);
-            }
-            chunk_decay(d, A, dh, dl);
-            const float eh = __shfl(dh, 63, 64), el = __shfl(dl, 63, 64);
-            hi[lane] = dh, lo[lane] = dl, step[lane] = d, from[lane] = exp2_fast(dh), to[lane] = exp2_fast((eh - dh) + (el - dl));
-        }
-        const T* x = static_cast<const T*>(a.x) + b * a.x_row + t0 * a.x_tok + (long long)h * a.P;
+        const int ring = (h - h0) % kRing;
+        const Decays& e = decays[ring];
+        HeadSums& hs = sums[ring];
+        const float D = a.D ? a.D[h] : 0.f;
         const long long at = (((long long)b * a.L + t0) * a.H + h) * a.P, tiles = (((long long)b * a.chunks + c) * a.H + h) * PP * NP;
-        f32x4 E[4], dM[4], U[4][NT], V[4][NT];
+        f32x4 dM[4], R[4][NS];
         Frag<T> wgt[2];
         float gh = 0.f;
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
             dM[tt] = zero;
 #pragma unroll
-            for (int s = 0; s < NT; ++s) U[tt][s] = V[tt][s] = zero;
+            for (int s = 0; s < NS; ++s) R[tt][s] = zero;
         }
-        for (int p0 = 0; p0 < PP; p0 += PB) {
-            if (p0 > 0) __syncthreads();
-            if (p0 >= a.P) break;
-            {
-                Tile<T, PB, 256> tile;
-                tile.load(static_cast<const T*>(q.dy) + at + p0, (long long)a.H * a.P, rows, a.P - p0, q.fast_dy);
-                tile.rows(Ys), tile.columns(Yt);
-                tile.load(x + p0, a.x_tok, rows, a.P - p0, a.fast_x);
-                tile.rows(Xs);
+        for (int pb = 0; pb < blocks; ++pb) {
+            const int p0 = pb * PB;
+            f32x4 tile[NS][PB / 16];
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int pt = 0; pt < PB / 16; ++pt)
+                    tile[s][pt] = *reinterpret_cast<const f32x4*>(mine + tiles + ((p0 / 16 + pt) * (NP / 16) + first + S::kHalf * s) * 256 + lane * 4);
+            __syncthreads();  // the block before has been read
+            if (w < 2) {
+                ahead.rows(threadIdx.x, Xs);
+            } else if (w < 4) {
+                ahead.rows(threadIdx.x - 128, Ys);
+                if constexpr (kTwice<T>) ahead.columns(threadIdx.x - 128, Yt);
             }
-            f32x4 H[NT][PB / 16], Gr[NT][PB / 16];
-#pragma unroll
-            for (int s = 0; s < NT; ++s) {
-                const int nt = w + 4 * s;
-#pragma unroll
-                for (int pt = 0; pt < PB / 16; ++pt) {
-                    H[s][pt] = Gr[s][pt] = zero;
-                    if (NP >= 64 || nt < NP / 16) {
-                        const long long o = tiles + ((p0 / 16 + pt) * (NP / 16) + nt) * 256 + lane * 4;
-                        H[s][pt] = *reinterpret_cast<const f32x4*>(q.front + o);
-                        Gr[s][pt] = *reinterpret_cast<const f32x4*>(q.behind + o);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            gh = fmaf(H[s][pt][i], Gr[s][pt][i], gh);
-                            Gt[(16 * pt + 4 * g + i) * kN + 16 * nt + lc] = (T)Gr[s][pt][i];
-                        }
-                    }
-                }
+            if (pb == 0 && ring == 0) {
+                if (w < kRing && h + w < h1) put_decays(decays[w], raw, lane < rows, a.dt.softplus, a.A[h + w]);
+                ask_step(h + kRing);
             }
+            const bool next = pb + 1 == blocks;  // head
+            if (!next || h + 1 < h1) ask(next ? h + 1 : h, next ? 0 : p0 + PB);
             __syncthreads();
-            if (p0 == 0) {
-                const float jh = hi[j], jl = lo[j], d = step[j];
-#pragma unroll
-                for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int t = 16 * tt + 4 * g + i;
-                        E[tt][i] = t >= j ? exp2_fast((hi[t] - jh) + (lo[t] - jl)) : 0.f;
-                    }
+            if (pb == 0) {
+                const float jh = e.hi[j], jl = e.lo[j], d = e.step[j];
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     f32x4 m[2];
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        m[r] = cb[2 * k + r] * E[2 * k + r] * d;
+                        const int t = 16 * (2 * k + r) + 4 * g;
+                        const f32x4 th = *reinterpret_cast<const f32x4*>(e.hi + t), tl = *reinterpret_cast<const f32x4*>(e.lo + t);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (16 * (2 * k + r) + 4 * g + i == j) m[r][i] += D;
+                        for (int i = 0; i < 4; ++i) {
+                            m[r][i] = t + i >= j ? cb[2 * k + r][i] * exp2_fast((th[i] - jh) + (tl[i] - jl)) * d : 0.f;
+                            if (t + i == j) m[r][i] += D;
+                        }
                     }
                     wgt[k] = frag_of<T>(m[0], m[1]);
                 }
@@ -150,32 +162,97 @@ __global__ __launch_bounds__(256) void scan_grad_kernel(GradArgs q) {
                 const Frag<T> xj = frag(Xs + j * kP + 32 * k + 8 * g);
 #pragma unroll
                 for (int tt = 0; tt < 4; ++tt)
-                    if (tt >= w) dM[tt] = mma(frag(Ys + (16 * tt + lc) * kP + 32 * k + 8 * g), xj, dM[tt]);
-                if (NP >= 64 || w < NP / 16) {
+                    if (tt >= jt && tt % S::kAlt == alt) dM[tt] = mma(frag(Ys + (16 * tt + lc) * kP + 32 * k + 8 * g), xj, dM[tt]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
-                    for (int s = 0; s < NT; ++s) {
-                        Split<T> hs, gs;
-                        split(H[s][2 * k], H[s][2 * k + 1], hs);
-                        split(Gr[s][2 * k], Gr[s][2 * k + 1], gs);
+            for (int s = 0; s < NS; ++s) {
+                if (role_v) {
 #pragma unroll
-                        for (int tt = 0; tt < 4; ++tt) {
-                            U[tt][s] = mma(frag(Ys + (16 * tt + lc) * kP + 32 * k + 4 * g, Ys + (16 * tt + lc) * kP + 32 * k + 16 + 4 * g), hs, U[tt][s]);
-                            V[tt][s] = mma(frag(Xs + (16 * tt + lc) * kP + 32 * k + 4 * g, Xs + (16 * tt + lc) * kP + 32 * k + 16 + 4 * g), gs, V[tt][s]);
+                    for (int pt = 0; pt < PB / 16; ++pt) {
+                        const int nt = first + S::kHalf * s;
+                        const f32x4 other = *reinterpret_cast<const f32x4*>(q.front + tiles + ((p0 / 16 + pt) * (NP / 16) + nt) * 256 + lane * 4);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            gh = fmaf(other[i], tile[s][pt][i], gh);
+                            Gt[(16 * pt + 4 * g + i) * kN + 16 * nt + lc] = (T)tile[s][pt][i];
                         }
                     }
                 }
+#pragma unroll
+                for (int k = 0; k < PB / 32; ++k) {
+                    Split<T> op;
+                    split(tile[s][2 * k], tile[s][2 * k + 1], op);
+#pragma unroll
+                    for (int tt = 0; tt < 4; ++tt)
+                        R[tt][s] = mma(frag(Rs + (16 * tt + lc) * kP + 32 * k + 4 * g, Rs + (16 * tt + lc) * kP + 32 * k + 16 + 4 * g), op, R[tt][s]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
-            const float end = to[j] * step[j];
+            __builtin_amdgcn_sched_barrier(0);
+            if (next) {
+                // per-token sums: over j (16 lanes, and the waves) for the rows, over t (this wave's registers) for the columns
+                float col = 0.f, diag = 0.f, dv = 0.f;
+                const float jh = e.hi[j], jl = e.lo[j], dj = e.step[j];
+#pragma unroll
+                for (int tt = 0; tt < 4; ++tt) {
+                    if (tt % S::kAlt != alt) continue;
+                    const int t = 16 * tt + 4 * g;
+                    f32x4 r = zero;
+                    if (tt >= jt) {
+                        const f32x4 th = *reinterpret_cast<const f32x4*>(e.hi + t), tl = *reinterpret_cast<const f32x4*>(e.lo + t);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float m = t + i >= j ? dM[tt][i] * exp2_fast((th[i] - jh) + (tl[i] - jl)) : 0.f, z = m * cb[tt][i];
+                            dcb[tt][i] = fmaf(m, dj, dcb[tt][i]);
+                            if (t + i == j) diag = z, dv = dM[tt][i];
+                            else col += z;
+                            r[i] = row16_sum(t + i == j ? 0.f : z * dj);
+                        }
+                    }
+                    if (lc == 0) *reinterpret_cast<f32x4*>(hs.rowZ[jt] + t) = r;
+                }
+                col += __shfl_xor(col, 16, 64), diag += __shfl_xor(diag, 16, 64), dv += __shfl_xor(dv, 16, 64);
+                col += __shfl_xor(col, 32, 64), diag += __shfl_xor(diag, 32, 64), dv += __shfl_xor(dv, 32, 64);
+                if (g == 0) {
+                    hs.colZ[alt][j] = col;
+                    if (jt % S::kAlt == alt) hs.diagZ[j] = diag, hs.diagV[j] = dv;
+                }
+#pragma unroll
+                for (int tt = 0; tt < 4; ++tt) {
+                    const int t = 16 * tt + 4 * g;
+                    f32x4 f = *reinterpret_cast<const f32x4*>((role_v ? e.to : e.from) + t), r = zero;
+                    if (role_v) f *= *reinterpret_cast<const f32x4*>(e.step + t);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                        for (int s = 0; s < NS; ++s) {
+                            r[i] = fmaf((float)Ks[(t + i) * kN + 16 * (first + S::kHalf * s) + lc], R[tt][s][i], r[i]);
+                            sum[tt][s][i] = fmaf(f[i], R[tt][s][i], sum[tt][s][i]);
+                        }
+                        r[i] = row16_sum(r[i]);
+                    }
+                    if (lc == 0) *reinterpret_cast<f32x4*>((role_v ? hs.dotV : hs.dotU)[first] + t) = r;
+                }
+                if (role_v) {
+                    gh = wave_sum(gh);
+                    if (lane == 0) hs.crossing[first] = gh;
+                }
+            }
+            __syncthreads();
+            const float end = e.to[j] * e.step[j];
             T* dx = static_cast<T*>(q.dx) + at + (long long)j * a.H * a.P + p0;
 #pragma unroll
             for (int pt = 0; pt < PB / 16; ++pt) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (pt % S::kAlt != alt) continue;
                 f32x4 acc = zero;  // rows p, columns j
 #pragma unroll
                 for (int k = 0; k < NP / 32; ++k) acc = mma(frag(Gt + (16 * pt + lc) * kN + 32 * k + 8 * g), frag(Bs + j * kN + 32 * k + 8 * g), acc);
                 acc *= end;
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
-                    if (2 * k + 1 >= w) acc = mma(frag(Yt + (16 * pt + lc) * kT + 32 * k + 4 * g, Yt + (16 * pt + lc) * kT + 32 * k + 16 + 4 * g), wgt[k], acc);
+                    if (2 * k + 1 >= jt) acc = mma(frag_down_pair(Ys, kP, Yt, 16 * pt + lc, 32 * k + 4 * g), wgt[k], acc);
                 const int p = 16 * pt + 4 * g;
                 if (j < all && p0 + p < a.P) {
                     T4 v;
@@ -191,120 +268,66 @@ __global__ __launch_bounds__(256) void scan_grad_kernel(GradArgs q) {
                 }
             }
         }
-        // per-token sums: over j (16 lanes and the waves) for the rows, over t (this wave's registers) for the columns
-        float col = 0.f, diag = 0.f, dv = 0.f;
-        const float dj = step[j];
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
-            if (tt >= w) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int t = 16 * tt + 4 * g + i;
-                    const float e = dM[tt][i] * E[tt][i], z = e * cb[tt][i];
-                    dcb[tt][i] = fmaf(e, dj, dcb[tt][i]);
-                    if (t == j) diag += z, dv += dM[tt][i];
-                    else col += z;
-                    const float r = row16_sum(t == j ? 0.f : z * dj);
-                    if (lc == 0) rowZ[w][t] = r;
-                }
-            } else if (lc == 0) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) rowZ[w][16 * tt + 4 * g + i] = 0.f;
+        if ((ring == kRing - 1 || h + 1 == h1) && w <= ring) {  // a wave per head of the ring, one token per lane
+            const int hw = h - ring + w;
+            const Decays& d = decays[w];
+            const HeadSums& s = sums[w];
+            const float step = d.step[lane], A = a.A[hw], v_all = S::kHalf == 4 ? s.dotV[2][lane] + s.dotV[3][lane] : 0.f;
+            const float u_all = S::kHalf == 4 ? s.dotU[2][lane] + s.dotU[3][lane] : 0.f, g_all = S::kHalf == 4 ? s.crossing[2] + s.crossing[3] : 0.f;
+            const float r = s.rowZ[0][lane] + s.rowZ[1][lane] + s.rowZ[2][lane] + s.rowZ[3][lane];
+            const float u = d.from[lane] * (s.dotU[0][lane] + s.dotU[1][lane] + u_all), v = d.to[lane] * (s.dotV[0][lane] + s.dotV[1][lane] + v_all);
+            const float col = S::kAlt == 2 ? s.colZ[0][lane] + s.colZ[1][lane] : s.colZ[0][lane];
+            const float cross = d.from[kQ - 1] * (s.crossing[0] + s.crossing[1] + g_all);
+            const double in = running_sum((double)(step * v)), out = running_sum((double)u + ((double)r - (double)step * col));
+            const double total = __shfl(out, 63, 64), before = __shfl_up(out, 1, 64), in_before = __shfl_up(in, 1, 64);
+            const float over = (float)((double)cross + (lane ? in_before : 0.0) + (total - (lane ? before : 0.0)));
+            float dstep = lane < rows ? fmaf(A, over, col + s.diagZ[lane] + v) : 0.f;
+            if (a.dt.softplus) dstep *= -expm1f(-step);  // softplus'(v) = 1 - e^{-softplus(v)}
+            if (lane < all) {
+                const long long o = ((long long)b * a.L + t0 + lane) * a.H + hw;
+                if (a.dt.type == 0) static_cast<float*>(q.ddt)[o] = dstep;
+                else static_cast<__bf16*>(q.ddt)[o] = (__bf16)dstep;
+            }
+            const float sA = wave_sum(lane < rows ? over * step : 0.f), sD = wave_sum(s.diagV[lane]), sb = wave_sum(dstep);
+            if (lane == 0) {
+                float* o = q.sums + (((long long)b * a.chunks + c) * a.H + hw) * 3;
+                o[0] = sA, o[1] = sD, o[2] = sb;
             }
         }
-        col += __shfl_xor(col, 16, 64), diag += __shfl_xor(diag, 16, 64), dv += __shfl_xor(dv, 16, 64);
-        col += __shfl_xor(col, 32, 64), diag += __shfl_xor(diag, 32, 64), dv += __shfl_xor(dv, 32, 64);
-        if (g == 0) colZ[j] = col, diagZ[j] = diag, diagV[j] = dv;
+    }
+    // dC += (V o E) d B, dB += (V o E)^T d C, summed over the heads before the product
+    T* Ms = pool;
+    __syncthreads();
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+        if (tt % S::kAlt == alt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) Ms[(16 * tt + 4 * g + i) * kT + j] = (T)dcb[tt][i];
+    __syncthreads();
+    T* grad = static_cast<T*>(role_v ? q.dB : q.dC);
+    float* wide = role_v ? q.pB : q.pC;
+    const T* Os = role_v ? Cs : Bs;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+        const int n = 16 * (first + S::kHalf * s) + lc;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const Frag<T> o = frag_across(Os, kN, n, 32 * k + 8 * g);
+#pragma unroll
+            for (int tt = 0; tt < 4; ++tt)
+                sum[tt][s] = mma(role_v ? frag_across(Ms, kT, 16 * tt + lc, 32 * k + 8 * g) : frag(Ms + (16 * tt + lc) * kT + 32 * k + 8 * g), o, sum[tt][s]);
+        }
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int t = 16 * tt + 4 * g + i;
-                float u = 0.f, v = 0.f;
-                if (NP >= 64 || w < NP / 16) {
-#pragma unroll
-                    for (int s = 0; s < NT; ++s) {
-                        const int n = 16 * (w + 4 * s) + lc;
-                        u = fmaf((float)Cs[t * kN + n], U[tt][s][i], u);
-                        v = fmaf((float)Bs[t * kN + n], V[tt][s][i], v);
-                        dCa[tt][s][i] = fmaf(from[t], U[tt][s][i], dCa[tt][s][i]);
-                        dBa[tt][s][i] = fmaf(to[t] * step[t], V[tt][s][i], dBa[tt][s][i]);
-                    }
-                }
-                u = row16_sum(u), v = row16_sum(v);
-                if (lc == 0) dotU[w][t] = u, dotV[w][t] = v;
-            }
-        gh = wave_sum(gh);
-        if (lane == 0) crossing[w] = gh;
-        __syncthreads();
-        if (w == 0) {  // one token per lane
-            const float d = step[lane];
-            const float r = rowZ[0][lane] + rowZ[1][lane] + rowZ[2][lane] + rowZ[3][lane];
-            const float u = from[lane] * (dotU[0][lane] + dotU[1][lane] + dotU[2][lane] + dotU[3][lane]);
-            const float v = to[lane] * (dotV[0][lane] + dotV[1][lane] + dotV[2][lane] + dotV[3][lane]);
-            const float cross = from[kQ - 1] * (crossing[0] + crossing[1] + crossing[2] + crossing[3]);
-            const double in = running_sum((double)(d * v)), out = running_sum((double)u + ((double)r - (double)d * colZ[lane]));
-            const double total = __shfl(out, 63, 64);
-            const double before = __shfl_up(out, 1, 64), in_before = __shfl_up(in, 1, 64);
-            const float over = (float)((double)cross + (lane ? in_before : 0.0) + (total - (lane ? before : 0.0)));
-            float dstep = fmaf(A, over, colZ[lane] + diagZ[lane] + v);
-            if (lane >= rows) dstep = 0.f;
-            if (a.dt.softplus) dstep = dstep / (1.f + expf(-raw));
-            if (lane < all) {
-                const long long o = ((long long)b * a.L + t0 + lane) * a.H + h;
-                if (a.dt.type == 0) static_cast<float*>(q.ddt)[o] = dstep;
-                else static_cast<__bf16*>(q.ddt)[o] = (__bf16)dstep;
-            }
-            const float sA = wave_sum(lane < rows ? over * d : 0.f), sD = wave_sum(diagV[lane]), sb = wave_sum(dstep);
-            if (lane == 0) {
-                float* s = q.sums + (((long long)b * a.chunks + c) * a.H + h) * 3;
-                s[0] = sA, s[1] = sD, s[2] = sb;
-            }
-        }
-        // what the next head writes before its first barrier (steps and decays, by this wave; the P-block tiles) nobody reads any more
-    }
-    // dC += (V o E) d B, dB += (V o E)^T d C, summed over the heads before the product
-    T *Ms = pool, *Kt = pool + kQ * kT;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        __syncthreads();
-        Tile<T, NP, 256> tile;
-        if (half == 0) tile.load(Bg, a.b_tok, rows, a.N, a.fast_b);
-        else tile.load(Cg, a.c_tok, rows, a.N, a.fast_c);
-        tile.columns(Kt);
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
-            T4 v;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[i] = (T)dcb[tt][i];
-                if (half == 0) Ms[(16 * tt + 4 * g + i) * kT + j] = v[i];
-            }
-            if (half == 1) *reinterpret_cast<T4*>(Ms + j * kT + 16 * tt + 4 * g) = v;
-        }
-        __syncthreads();
-        T* grad = static_cast<T*>(half == 0 ? q.dC : q.dB);
-        float* wide = half == 0 ? q.pC : q.pB;
-#pragma unroll
-        for (int s = 0; s < NT; ++s) {
-            const int nt = w + 4 * s, n = 16 * nt + lc;
-            if (NP < 64 && nt >= NP / 16) break;
-#pragma unroll
-            for (int tt = 0; tt < 4; ++tt) {
-                f32x4 acc = half == 0 ? dCa[tt][s] : dBa[tt][s];
-#pragma unroll
-                for (int k = 0; k < 2; ++k) acc = mma(frag(Ms + (16 * tt + lc) * kT + 32 * k + 8 * g), frag(Kt + n * kT + 32 * k + 8 * g), acc);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int t = 16 * tt + 4 * g + i;
-                    if (t < all && n < a.N) {
-                        const long long o = (((long long)b * a.L + t0 + t) * a.G + grp) * a.N + n;
-                        if (q.parts > 1) wide[(long long)part * a.rows * a.L * a.G * a.N + o] = acc[i];
-                        else grad[o] = (T)acc[i];
-                    }
+                if (t < all && n < a.N) {
+                    const long long o = (((long long)b * a.L + t0 + t) * a.G + grp) * a.N + n;
+                    if (q.parts > 1) wide[(long long)part * a.rows * a.L * a.G * a.N + o] = sum[tt][s][i];
+                    else grad[o] = (T)sum[tt][s][i];
                 }
             }
-        }
     }
 }
 
@@ -351,7 +374,7 @@ template <typename T, int NP, int PP>
 static int launch_grad(const GradArgs& q, hipStream_t st) {
     const long long blocks = (long long)q.a.rows * q.a.chunks * q.a.G * q.parts;
     if (blocks > 0x7fffffffll) return RTFS_EINVAL;
-    hipLaunchKernelGGL((scan_grad_kernel<T, NP, PP>), dim3((unsigned)blocks), dim3(256), 0, st, q);
+    hipLaunchKernelGGL((scan_grad_kernel<T, NP, PP>), dim3((unsigned)blocks), dim3(GradTiles<T, NP, PP>::kThreads), 0, st, q);
     RTFS_LAUNCH_CHECK();
     if (q.parts > 1) {
         const long long n = (long long)q.a.rows * q.a.L * q.a.G * q.a.N, wg = (n + 255) / 256;

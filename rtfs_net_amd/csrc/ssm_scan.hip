@@ -41,7 +41,7 @@ __global__ __launch_bounds__(Waves<PP>::kThreads, (ScanTiles<T, NP, PP>::kWavesP
     __shared__ __attribute__((aligned(16))) Decays decays[W::kWaves];
     int b, seg, h;
     scan_place(a, b, seg, h);
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, lc = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, w = wave_index(), lc = lane & 15, g = lane >> 4;
     const int len = row_length(a.lengths, b, a.L);
     const float A = a.A[h], D = a.D ? a.D[h] : 0.f;
     const T* x = static_cast<const T*>(a.x) + b * a.x_row + (long long)h * a.P;
@@ -73,9 +73,9 @@ __global__ __launch_bounds__(Waves<PP>::kThreads, (ScanTiles<T, NP, PP>::kWavesP
     auto ask = [&](int c) {
         const long long t0 = (long long)c * kQ;
         const int rows = len - t0 < kQ ? (int)(len - t0) : kQ;
-        tb.load(Bg + t0 * a.b_tok, a.b_tok, rows, a.N, a.fast_b);
-        tc.load(Cg + t0 * a.c_tok, a.c_tok, rows, a.N, a.fast_c);
-        tx.load(x + t0 * a.x_tok, a.x_tok, rows, a.P, a.fast_x);
+        tb.load(threadIdx.x, Bg + t0 * a.b_tok, a.b_tok, rows, a.N, a.fast_b);
+        tc.load(threadIdx.x, Cg + t0 * a.c_tok, a.c_tok, rows, a.N, a.fast_c);
+        tx.load(threadIdx.x, x + t0 * a.x_tok, a.x_tok, rows, a.P, a.fast_x);
     };
     auto ask_step = [&](int c) {  // the steps of as many chunks as there are waves, one chunk per wave
         const int t = (c + w) * kQ + lane;
@@ -86,9 +86,9 @@ __global__ __launch_bounds__(Waves<PP>::kThreads, (ScanTiles<T, NP, PP>::kWavesP
         const int t0 = c * kQ, rows = len - t0 < kQ ? len - t0 : kQ, all = a.L - t0 < kQ ? a.L - t0 : kQ, which = (c - c0) % W::kWaves;
         T* out = y + (((long long)b * a.L + t0) * a.H + h) * a.P;
         __syncthreads();  // the chunk before has been read
-        tb.rows(Bs), tc.rows(Cs);
-        if constexpr (kTwice<T>) tb.columns(Bt), tx.columns(Xs);
-        else tx.rows(Xs);
+        tb.rows(threadIdx.x, Bs), tc.rows(threadIdx.x, Cs);
+        if constexpr (kTwice<T>) tb.columns(threadIdx.x, Bt), tx.columns(threadIdx.x, Xs);
+        else tx.rows(threadIdx.x, Xs);
         if (which == 0) {
             put_decays(decays[w], raw, (c + w) * kQ + lane < len, a.dt.softplus, A);
             if (c + W::kWaves < c1) ask_step(c + W::kWaves);
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(Waves<PP>::kThreads, 2) void scan_walk_kernel(ScanA
     if (blockIdx.y) a = a1, o = o1;
     int b, seg, h;
     scan_place(a, b, seg, h);
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, lc = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, w = wave_index(), lc = lane & 15, g = lane >> 4;
     const int len = row_length(a.lengths, b, a.L);
     const float A = a.A[h];
     const T* x = static_cast<const T*>(a.x) + b * a.x_row + (long long)h * a.P;
@@ -264,8 +264,8 @@ __global__ __launch_bounds__(Waves<PP>::kThreads, 2) void scan_walk_kernel(ScanA
         const long long t0 = (long long)chunk(k) * kQ;
         if (t0 >= len) return;
         const int rows = len - t0 < kQ ? (int)(len - t0) : kQ;
-        tb.load(Bg + t0 * a.b_tok, a.b_tok, rows, a.N, a.fast_b);
-        tx.load(x + t0 * a.x_tok, a.x_tok, rows, a.P, a.fast_x);
+        tb.load(threadIdx.x, Bg + t0 * a.b_tok, a.b_tok, rows, a.N, a.fast_b);
+        tx.load(threadIdx.x, x + t0 * a.x_tok, a.x_tok, rows, a.P, a.fast_x);
     };
     auto ask_step = [&](int k) {
         const long long t = (long long)chunk(k + w) * kQ + lane;
@@ -284,8 +284,8 @@ __global__ __launch_bounds__(Waves<PP>::kThreads, 2) void scan_walk_kernel(ScanA
         }
         __syncthreads();
         if (t0 < len) {
-            if constexpr (kTwice<T>) tb.columns(Bs), tx.columns(Xs);
-            else tb.rows(Bs), tx.rows(Xs);
+            if constexpr (kTwice<T>) tb.columns(threadIdx.x, Bs), tx.columns(threadIdx.x, Xs);
+            else tb.rows(threadIdx.x, Bs), tx.rows(threadIdx.x, Xs);
         }
         if (which == 0) {
             put_decays(decays[w], raw, k + w < k1 && (long long)chunk(k + w) * kQ + lane < len, a.dt.softplus, A);
