@@ -19,7 +19,7 @@ struct GradArgs {
     float *pB, *pC;              // [parts][rows][L][G][N] when the heads of a group are spread over several workgroups
     float* sums;                 // [rows][chunk][head][3]: dA, dD, dbias
     int parts, part_heads;
-    int fast_dy;
+    int how_dy;
 };
 
 // One workgroup takes a chunk for a group's heads (or a part of them, where rows, chunks and groups are too few): C B^T is formed once, and the gradients of B
@@ -40,10 +40,13 @@ struct HeadSums {
 template <typename T, int NP, int PP> struct GradTiles {
     static constexpr int kWaves = NP == 128 ? 8 : 4, kThreads = 64 * kWaves, kHalf = kWaves / 2, kAlt = kWaves / 4;
     static constexpr int kSlices = NP / 16 / kHalf;  // 16-wide slices of N per wave
-    static constexpr int PB = PP < 64 ? PP : 64, kBlocks = PP / PB;
-    static constexpr int kN = pitch<T>(NP), kT = pitch<T>(kQ), kP = pitch<T>(PB);
-    static constexpr int kYt = kTwice<T> ? PB * kT : 0, kMain = 2 * kQ * kP + kYt + PB * kN, kPool = kMain > kQ * kT ? kMain : kQ * kT;
-    static constexpr int kBytes = (2 * kQ * kN + kPool) * (int)sizeof(T) + kRing * (int)(sizeof(Decays) + sizeof(HeadSums));
+    static constexpr int PB = PP < 64 ? PP : 64;
+    typedef Tile<T, kQ, NP> Wide;
+    typedef Tile<T, kQ, PB> Slim;
+    typedef Tile<T, NP, PB> States;
+    typedef Tile<T, kQ, kQ> Scores;
+    static constexpr int kMain = 2 * Slim::kBytes + States::kBytes, kPool = kMain > Scores::kBytes ? kMain : Scores::kBytes;
+    static constexpr int kBytes = 2 * Wide::kBytes + kPool + kRing * (int)(sizeof(Decays) + sizeof(HeadSums));
     static constexpr int kWavesPerSimd = kWaves == 8 || kBytes * 2 <= 160 * 1024 ? 2 : 1;
 };
 
@@ -51,11 +54,13 @@ template <typename T, int NP, int PP>
 __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP, PP>::kWavesPerSimd)) void scan_grad_kernel(GradArgs q) {
     typedef GradTiles<T, NP, PP> S;
     typedef T T4 __attribute__((ext_vector_type(4)));
-    constexpr int PB = S::PB, kN = S::kN, kT = S::kT, kP = S::kP, NS = S::kSlices;
-    __shared__ __attribute__((aligned(16))) T Bs[kQ * kN], Cs[kQ * kN], pool[S::kPool];
+    constexpr int PB = S::PB, NS = S::kSlices;
+    __shared__ __attribute__((aligned(16))) typename S::Wide Bs, Cs;
+    __shared__ __attribute__((aligned(16))) char pool[S::kPool];
     __shared__ __attribute__((aligned(16))) Decays decays[kRing];
     __shared__ __attribute__((aligned(16))) HeadSums sums[kRing];
-    T *Ys = pool, *Xs = Ys + kQ * kP, *Gt = Xs + kQ * kP, *Yt = Gt + PB * kN;
+    typename S::Slim &Ys = *reinterpret_cast<typename S::Slim*>(pool), &Xs = *reinterpret_cast<typename S::Slim*>(pool + S::Slim::kBytes);
+    typename S::States& Gs = *reinterpret_cast<typename S::States*>(pool + 2 * S::Slim::kBytes);  // rows n
     const ScanArgs& a = q.a;
     unsigned i0 = xcd_block(blockIdx.x, gridDim.x);
     const int part = (int)(i0 % q.parts);
@@ -70,35 +75,38 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
     const int jt = w & 3, alt = w >> 2, j = 16 * jt + lc;  // this lane's column of the score tiles
     const bool role_v = w >= S::kHalf;
     const int first = role_v ? w - S::kHalf : w;
-    const T *Rs = role_v ? Xs : Ys, *Ks = role_v ? Bs : Cs;
+    const typename S::Slim& Rs = role_v ? Xs : Ys;
+    const typename S::Wide& Ks = role_v ? Bs : Cs;
     const float *mine = role_v ? q.behind : q.front;
     {
         const T* Bg = static_cast<const T*>(a.B) + b * a.b_row + t0 * a.b_tok + (long long)grp * a.N;
         const T* Cg = static_cast<const T*>(a.C) + b * a.c_row + t0 * a.c_tok + (long long)grp * a.N;
-        Tile<T, NP, S::kThreads> tile;
-        tile.load(threadIdx.x, Bg, a.b_tok, rows, a.N, a.fast_b);
-        tile.rows(threadIdx.x, Bs);
-        tile.load(threadIdx.x, Cg, a.c_tok, rows, a.N, a.fast_c);
-        tile.rows(threadIdx.x, Cs);
+        Load<T, NP, S::kThreads> load;
+        load.ask(threadIdx.x, Bg, a.b_tok, rows, a.N, a.how_b);
+        load.put(threadIdx.x, Bs);
+        load.ask(threadIdx.x, Cg, a.c_tok, rows, a.N, a.how_c);
+        load.put(threadIdx.x, Cs);
     }
-    Tile<T, PB, 128> ahead;  // x by waves 0 and 1, dy by waves 2 and 3
+    Load<T, PB, 128> ahead;  // x by waves 0 and 1, dy by waves 2 and 3
     auto ask = [&](int h, int p0) {
         const T* src = w < 2 ? static_cast<const T*>(a.x) + b * a.x_row + t0 * a.x_tok : static_cast<const T*>(q.dy) + ((long long)b * a.L + t0) * a.H * a.P;
         if (w < 4)
-            ahead.load(threadIdx.x & 127, src + (long long)h * a.P + p0, w < 2 ? a.x_tok : (long long)a.H * a.P, rows, a.P - p0, w < 2 ? a.fast_x : q.fast_dy);
+            ahead.ask(threadIdx.x & 127, src + (long long)h * a.P + p0, w < 2 ? a.x_tok : (long long)a.H * a.P, rows, a.P - p0, w < 2 ? a.how_x : q.how_dy);
     };
     float raw = 0.f;
     auto ask_step = [&](int h) { raw = w < kRing && h + w < h1 && lane < rows ? a.dt.raw(b, t0 + lane, h + w) : 0.f; };
     ask(h0, 0), ask_step(h0);
     __syncthreads();
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    const typename S::Wide::Lane ln;
+    const typename S::Slim::Lane lp;
     f32x4 cb[4], dcb[4], sum[4][NS];  // rows t, columns j; rows t, columns n
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) {
         cb[tt] = dcb[tt] = zero;
         if (tt >= jt)
 #pragma unroll
-            for (int k = 0; k < NP / 32; ++k) cb[tt] = mma(frag(Cs + (16 * tt + lc) * kN + 32 * k + 8 * g), frag(Bs + j * kN + 32 * k + 8 * g), cb[tt]);
+            for (int k = 0; k < NP / 32; ++k) cb[tt] = mma(Cs.row(ln, 16 * tt, 32 * k), Bs.row(ln, 16 * jt, 32 * k), cb[tt]);
 #pragma unroll
         for (int s = 0; s < NS; ++s) sum[tt][s] = zero;
     }
@@ -123,15 +131,11 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
 #pragma unroll
             for (int s = 0; s < NS; ++s)
 #pragma unroll
-                for (int pt = 0; pt < PB / 16; ++pt)
-                    tile[s][pt] = *reinterpret_cast<const f32x4*>(mine + tiles + ((p0 / 16 + pt) * (NP / 16) + first + S::kHalf * s) * 256 + lane * 4);
+                for (int pt = 0; pt < PB / 16; ++pt)  // (the walks leave tiles behind P unwritten)
+                    tile[s][pt] = p0 + 16 * pt < a.P ? *reinterpret_cast<const f32x4*>(mine + tiles + ((p0 / 16 + pt) * (NP / 16) + first + S::kHalf * s) * 256 + lane * 4) : zero;
             __syncthreads();  // the block before has been read
-            if (w < 2) {
-                ahead.rows(threadIdx.x, Xs);
-            } else if (w < 4) {
-                ahead.rows(threadIdx.x - 128, Ys);
-                if constexpr (kTwice<T>) ahead.columns(threadIdx.x - 128, Yt);
-            }
+            if (w < 2) ahead.put(threadIdx.x, Xs);
+            else if (w < 4) ahead.put(threadIdx.x - 128, Ys);
             if (pb == 0 && ring == 0) {
                 if (w < kRing && h + w < h1) put_decays(decays[w], raw, lane < rows, a.dt.softplus, a.A[h + w]);
                 ask_step(h + kRing);
@@ -159,10 +163,10 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
             }
 #pragma unroll
             for (int k = 0; k < PB / 32; ++k) {
-                const Frag<T> xj = frag(Xs + j * kP + 32 * k + 8 * g);
+                const Frag<T> xj = Xs.row(lp, 16 * jt, 32 * k);
 #pragma unroll
                 for (int tt = 0; tt < 4; ++tt)
-                    if (tt >= jt && tt % S::kAlt == alt) dM[tt] = mma(frag(Ys + (16 * tt + lc) * kP + 32 * k + 8 * g), xj, dM[tt]);
+                    if (tt >= jt && tt % S::kAlt == alt) dM[tt] = mma(Ys.row(lp, 16 * tt, 32 * k), xj, dM[tt]);
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
@@ -171,12 +175,10 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
 #pragma unroll
                     for (int pt = 0; pt < PB / 16; ++pt) {
                         const int nt = first + S::kHalf * s;
-                        const f32x4 other = *reinterpret_cast<const f32x4*>(q.front + tiles + ((p0 / 16 + pt) * (NP / 16) + nt) * 256 + lane * 4);
+                        const f32x4 other = p0 + 16 * pt < a.P ? *reinterpret_cast<const f32x4*>(q.front + tiles + ((p0 / 16 + pt) * (NP / 16) + nt) * 256 + lane * 4) : zero;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            gh = fmaf(other[i], tile[s][pt][i], gh);
-                            Gt[(16 * pt + 4 * g + i) * kN + 16 * nt + lc] = (T)tile[s][pt][i];
-                        }
+                        for (int i = 0; i < 4; ++i) gh = fmaf(other[i], tile[s][pt][i], gh);
+                        Gs.put4(16 * nt + lc, 16 * pt + 4 * g, tile[s][pt]);
                     }
                 }
 #pragma unroll
@@ -185,7 +187,7 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
                     split(tile[s][2 * k], tile[s][2 * k + 1], op);
 #pragma unroll
                     for (int tt = 0; tt < 4; ++tt)
-                        R[tt][s] = mma(frag(Rs + (16 * tt + lc) * kP + 32 * k + 4 * g, Rs + (16 * tt + lc) * kP + 32 * k + 16 + 4 * g), op, R[tt][s]);
+                        R[tt][s] = mma(Rs.row(lp, 16 * tt, 32 * k), op, R[tt][s]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
@@ -227,7 +229,7 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
                     for (int i = 0; i < 4; ++i) {
 #pragma unroll
                         for (int s = 0; s < NS; ++s) {
-                            r[i] = fmaf((float)Ks[(t + i) * kN + 16 * (first + S::kHalf * s) + lc], R[tt][s][i], r[i]);
+                            r[i] = fmaf(Ks.get(t + i, 16 * (first + S::kHalf * s) + lc), R[tt][s][i], r[i]);
                             sum[tt][s][i] = fmaf(f[i], R[tt][s][i], sum[tt][s][i]);
                         }
                         r[i] = row16_sum(r[i]);
@@ -248,11 +250,11 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
                 if (pt % S::kAlt != alt) continue;
                 f32x4 acc = zero;  // rows p, columns j
 #pragma unroll
-                for (int k = 0; k < NP / 32; ++k) acc = mma(frag(Gt + (16 * pt + lc) * kN + 32 * k + 8 * g), frag(Bs + j * kN + 32 * k + 8 * g), acc);
+                for (int k = 0; k < NP / 32; ++k) acc = mma(Gs.down(lp, 32 * k, 16 * pt), Bs.row(ln, 16 * jt, 32 * k), acc);
                 acc *= end;
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
-                    if (2 * k + 1 >= jt) acc = mma(frag_down_pair(Ys, kP, Yt, 16 * pt + lc, 32 * k + 4 * g), wgt[k], acc);
+                    if (2 * k + 1 >= jt) acc = mma(Ys.down(lp, 32 * k, 16 * pt), wgt[k], acc);
                 const int p = 16 * pt + 4 * g;
                 if (j < all && p0 + p < a.P) {
                     T4 v;
@@ -296,26 +298,26 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
         }
     }
     // dC += (V o E) d B, dB += (V o E)^T d C, summed over the heads before the product
-    T* Ms = pool;
+    const typename S::Scores::Lane lq;
+    typename S::Scores& Ms = *reinterpret_cast<typename S::Scores*>(pool);
     __syncthreads();
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt)
         if (tt % S::kAlt == alt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) Ms[(16 * tt + 4 * g + i) * kT + j] = (T)dcb[tt][i];
+            for (int i = 0; i < 4; ++i) Ms.put(16 * tt + 4 * g + i, j, dcb[tt][i]);
     __syncthreads();
     T* grad = static_cast<T*>(role_v ? q.dB : q.dC);
     float* wide = role_v ? q.pB : q.pC;
-    const T* Os = role_v ? Cs : Bs;
+    const typename S::Wide& Os = role_v ? Cs : Bs;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
         const int n = 16 * (first + S::kHalf * s) + lc;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const Frag<T> o = frag_across(Os, kN, n, 32 * k + 8 * g);
+            const Frag<T> o = Os.down_any(32 * k, 16 * (first + S::kHalf * s));
 #pragma unroll
-            for (int tt = 0; tt < 4; ++tt)
-                sum[tt][s] = mma(role_v ? frag_across(Ms, kT, 16 * tt + lc, 32 * k + 8 * g) : frag(Ms + (16 * tt + lc) * kT + 32 * k + 8 * g), o, sum[tt][s]);
+            for (int tt = 0; tt < 4; ++tt) sum[tt][s] = mma(role_v ? Ms.down(lq, 32 * k, 16 * tt) : Ms.row(lq, 16 * tt, 32 * k), o, sum[tt][s]);
         }
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
@@ -394,10 +396,9 @@ using namespace rtfs::ssm;
 extern "C" {
 
 int rtfs_ssm_scan_bwd_parts(int B, int L, int H, int G) {
-    if (B <= 0 || L <= 0 || G <= 0 || H <= 0 || H % G) return RTFS_EINVAL;
+    if (!scan_sizes(B, L, H, 1, G, 1)) return RTFS_EINVAL;
     ScanArgs a{};
-    a.rows = B, a.L = L, a.H = H, a.G = G;
-    scan_cut(a);
+    a.rows = B, a.H = H, a.G = G, a.chunks = (L + kQ - 1) / kQ;
     int parts, heads;
     grad_parts(a, parts, heads);
     return parts;
@@ -409,7 +410,7 @@ int rtfs_ssm_scan_bwd(const void* x, long long x_row, long long x_tok, const voi
                       float* dD, float* dbias, float* dstate, float* starts, float* front, float* behind, float* parts, float* sums, int B, int L, int H, int P, int G,
                       int N, int type, void* stream) {
     if (!x || !dt || !A || !Bm || !C || !dy || !dx || !ddt || !dA || !dB || !dC || !front || !behind || !sums || !scan_sizes(B, L, H, P, G, N) || type < 0 ||
-        type > 1 || dt_type < 0 || dt_type > 1)
+        type > 1 || dt_type < 0 || dt_type > 1 || !scan_pitch(x_tok) || !scan_pitch(b_tok) || !scan_pitch(c_tok) || !scan_pitch((long long)H * P))
         return RTFS_EINVAL;
     hipStream_t st = (hipStream_t)stream;
     const Steps steps{dt, dt_row, dt_tok, dt_type, dt_bias, softplus};
@@ -432,8 +433,8 @@ int rtfs_ssm_scan_bwd(const void* x, long long x_row, long long x_tok, const voi
     if (rc != RTFS_OK) return rc;
     q.dy = dy, q.front = front, q.behind = behind, q.dx = dx, q.ddt = ddt, q.dB = dB, q.dC = dC, q.sums = sums;
     q.pB = parts, q.pC = parts ? parts + (long long)q.parts * B * L * G * N : nullptr;
-    q.fast_dy = back.fast_x;
-    auto grad = [&]() -> int { RTFS_SSM_DISPATCH(type, N, P, launch_grad, (q, st)); };
+    q.how_dy = back.how_x;
+    auto grad = [&]() -> int { RTFS_SSM_DISPATCH(type, N, 32, 128, P, launch_grad, (q, st)); };
     const int rg = grad();
     if (rg != RTFS_OK) return rg;
     hipLaunchKernelGGL(sum_heads_kernel, dim3(3 * H), dim3(256), 0, st, sums, (long long)B * q.a.chunks, H, dA, dD, dbias);

@@ -8,203 +8,262 @@
 namespace rtfs {
 namespace ssm {
 
-// Which segment of which row and head: heads are innermost (they share B and C), so an XCD's L2 sees one stretch of them.
-__device__ __forceinline__ void scan_place(const ScanArgs& a, int& b, int& seg, int& h) {
-    const unsigned i = xcd_block(blockIdx.x, gridDim.x);
-    h = (int)(i % a.H);
-    seg = (int)(i / a.H % a.segs);
-    b = (int)(i / a.H / a.segs);
+// One workgroup: four waves, each with one head's slice of P, all of one group of heads - they share the tiles of B and C in LDS.
+struct Place {
+    int b, seg, grp, head, p0;
+    bool works;  // waves past the group's last slice only help to load
+};
+__device__ __forceinline__ Place scan_place(const ScanArgs& a, int w) {
+    unsigned i = xcd_block(blockIdx.x, gridDim.x);
+    Place p;
+    const int quad = (int)(i % a.quads);
+    i /= a.quads;
+    p.grp = (int)(i % a.G);
+    i /= a.G;
+    p.seg = (int)(i % a.segs);
+    p.b = (int)(i / a.segs);
+    const int each = a.H / a.G, unit = quad * 4 + w;
+    p.works = unit < each * a.slices;
+    p.head = p.grp * each + (p.works ? unit / a.slices : 0);
+    p.p0 = p.works ? unit % a.slices * a.width : 0;
+    return p;
+}
+
+// S <- e^{s[63]} S + sum_j (weight[j] x[j]) B[j]^T, with the weights of a forward or a backward walk.  The weighted x, split, is one operand, tokens of B's
+// columns the other, each read once; the state's tiles lie rows n, columns p (S[n][p], the forward kernel's) or rows p, columns n (S[p][n], the walks').
+template <bool N_FIRST, typename T, int NP, int PW, int R, int C>
+__device__ __forceinline__ void advance(f32x4 (&S)[R][C], const Tile<T, kQ, PW>& X, const Tile<T, kQ, NP>& Bs, const Decays& e, bool backwards) {
+    constexpr int NT = NP / 16, PT = PW / 16;
+    const int g = (threadIdx.x & 63) >> 4;
+    const Lanes<T, NP> ln;
+    const Lanes<T, PW> lp;
+    const float whole = e.from[kQ - 1];
+    constexpr int kSome = PT < 2 ? PT : 2;  // tiles of P at a time: the split x of all four would take the registers of the loads in flight
+#pragma unroll
+    for (int p0 = 0; p0 < PT; p0 += kSome)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            Split<T> xs[kSome];
+            const int t = 32 * k + 4 * g;
+            f32x4 wa = *reinterpret_cast<const f32x4*>((backwards ? e.from : e.to) + t), wb = *reinterpret_cast<const f32x4*>((backwards ? e.from : e.to) + t + 16);
+            if (!backwards) wa *= *reinterpret_cast<const f32x4*>(e.step + t), wb *= *reinterpret_cast<const f32x4*>(e.step + t + 16);
+#pragma unroll
+            for (int pt = 0; pt < kSome; ++pt) {
+                f32x4 u, v;
+                widen(X.down(lp, 32 * k, 16 * (p0 + pt)), u, v);
+                split(u * wa, v * wb, xs[pt]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const Frag<T> bt = Bs.down(ln, 32 * k, 16 * nt);
+#pragma unroll
+                for (int term = Split<T>::kTerms - 1; term >= 0; --term)
+#pragma unroll
+                    for (int pt = 0; pt < kSome; ++pt) {
+                        f32x4& s = N_FIRST ? S[nt][p0 + pt] : S[p0 + pt][nt];
+                        if (k == 0 && term == Split<T>::kTerms - 1) s *= whole;
+                        s = N_FIRST ? mma(bt, xs[pt].part(term), s) : mma(xs[pt].part(term), bt, s);
+                    }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
 }
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------------------------------------
-// One workgroup walks one segment of one head.  Wave w owns 16 (P = 128: 32) of the P columns for all N and keeps their part of the state in its accumulators
-// from chunk to chunk: an accumulator tile is, as it lies, the operand of the product with C (the "pair" order), so the state never leaves registers.
-// C B^T is shared out by tiles of the lower triangle and meets the decays on its way to LDS; D joins its diagonal.
+// A wave walks one segment of its slice and keeps the state in its accumulators from chunk to chunk: an accumulator tile is, as it lies, the operand of the
+// product with C, so the state never leaves registers.  So do the scores: C B^T of a pair of token tiles, times decay and step (D joins the diagonal), is the
+// operand of the product with x.  LDS holds B and C once for four waves and each wave's x; two barriers per chunk.
 // Roundings (bf16): the scores times decay and step, and the state as it enters the product with C, once each to bf16 - y is rounded to that anyway; the
-// weighted inputs that build the state are kept as two bf16 (ssm.h), so the state that is handed on is good to 2^-17.
-template <typename T, int NP, int PP> struct ScanTiles {
-    static constexpr int kN = pitch<T>(NP), kP = pitch<T>(PP), kT = pitch<T>(kQ);
-    static constexpr int kBt = kTwice<T> ? NP * kT : 0, kX = kTwice<T> ? PP * kT : kQ * kP;
-    static constexpr int kBytes = (2 * kQ * kN + kBt + kX + kQ * kT) * (int)sizeof(T) + Waves<PP>::kWaves * (int)sizeof(Decays);
+// weighted inputs that build the state are split (ssm.h), so the state that is handed on has fp32's precision.
+template <typename T, int NP, int PW> struct ScanShare {
+    static constexpr int kBytes = 2 * Tile<T, kQ, NP>::kBytes + 4 * (Tile<T, kQ, PW>::kBytes + (int)sizeof(Decays));
     // waves per SIMD: two (256 registers each) where a CU's LDS holds as many workgroups, else one
     static constexpr int kWavesPerSimd = kBytes * 2 <= 160 * 1024 ? 2 : 1;
 };
 
-template <typename T, int NP, int PP>
-__global__ __launch_bounds__(Waves<PP>::kThreads, (ScanTiles<T, NP, PP>::kWavesPerSimd)) void scan_kernel(ScanArgs a, const float* __restrict__ starts,
-                                                                                                         T* __restrict__ y, float* __restrict__ last) {
-    typedef Waves<PP> W;
-    typedef ScanTiles<T, NP, PP> S_;
+template <typename T, int NP, int PW>
+__global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void scan_kernel(ScanArgs a, const float* __restrict__ starts, T* __restrict__ y,
+                                                                                          float* __restrict__ last) {
     typedef T T4 __attribute__((ext_vector_type(4)));
-    constexpr int kN = S_::kN, kP = S_::kP, kT = S_::kT;
-    __shared__ __attribute__((aligned(16))) T Bs[kQ * kN], Cs[kQ * kN], Bt[S_::kBt + 1], Xs[S_::kX], Ms[kQ * kT];
-    __shared__ __attribute__((aligned(16))) Decays decays[W::kWaves];
-    int b, seg, h;
-    scan_place(a, b, seg, h);
+    constexpr int NT = NP / 16, PT = PW / 16;
+    __shared__ __attribute__((aligned(16))) Tile<T, kQ, NP> Bs, Cs;
+    __shared__ __attribute__((aligned(16))) Tile<T, kQ, PW> Xs[4];
+    __shared__ __attribute__((aligned(16))) Decays decays[4];
     const int lane = threadIdx.x & 63, w = wave_index(), lc = lane & 15, g = lane >> 4;
-    const int len = row_length(a.lengths, b, a.L);
+    const Place at = scan_place(a, w);
+    const int b = at.b, h = at.head, len = row_length(a.lengths, b, a.L), cols = a.P - at.p0;
     const float A = a.A[h], D = a.D ? a.D[h] : 0.f;
-    const T* x = static_cast<const T*>(a.x) + b * a.x_row + (long long)h * a.P;
-    const T* Bg = static_cast<const T*>(a.B) + b * a.b_row + (long long)(h / (a.H / a.G)) * a.N;
-    const T* Cg = static_cast<const T*>(a.C) + b * a.c_row + (long long)(h / (a.H / a.G)) * a.N;
+    const T* x = static_cast<const T*>(a.x) + b * a.x_row + (long long)h * a.P + at.p0;
+    const T* Bg = static_cast<const T*>(a.B) + b * a.b_row + (long long)at.grp * a.N;
+    const T* Cg = static_cast<const T*>(a.C) + b * a.c_row + (long long)at.grp * a.N;
+    const long long state_at = ((long long)b * a.H + h) * a.P + at.p0;
+    Tile<T, kQ, PW>& X = Xs[w];
+    Decays& e = decays[w];
+    const Lanes<T, NP> ln;
+    const Lanes<T, PW> lp;
 
-    f32x4 S[NP / 16][W::kTiles];  // rows n, columns p
+    f32x4 S[NT][PT];  // rows n, columns p
+    const float* from = at.seg > 0 ? starts + (((long long)b * a.H + h) * a.segs + at.seg) * (padded(a.P) * NP) + at.p0 * NP : nullptr;
 #pragma unroll
-    for (int nt = 0; nt < NP / 16; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int pt = 0; pt < W::kTiles; ++pt) {
-            const int p = 16 * (w * W::kTiles + pt) + lc, n = 16 * nt + 4 * g;
+        for (int pt = 0; pt < PT; ++pt) {
+            const int p = 16 * pt + lc, n = 16 * nt + 4 * g;
             S[nt][pt] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (seg > 0) {
-                S[nt][pt] = *reinterpret_cast<const f32x4*>(starts + (((long long)b * a.H + h) * a.segs + seg) * PP * NP + p * NP + n);
-            } else if (a.state && p < a.P) {
+            if (from) {
+                S[nt][pt] = *reinterpret_cast<const f32x4*>(from + p * NP + n);
+            } else if (a.state && p < cols) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (n + i < a.N) S[nt][pt][i] = a.state[(((long long)b * a.H + h) * a.P + p) * a.N + n + i];
+                    if (n + i < a.N) S[nt][pt][i] = a.state[(state_at + p) * a.N + n + i];
             }
         }
-    for (int i = threadIdx.x; i < kQ * kT; i += W::kThreads) Ms[i] = (T)0.f;
 
-    const int c0 = seg * a.seg_chunks, c_all = c0 + a.seg_chunks < a.chunks ? c0 + a.seg_chunks : a.chunks;
+    const int c0 = at.seg * a.seg_chunks, c_all = c0 + a.seg_chunks < a.chunks ? c0 + a.seg_chunks : a.chunks;
     const int c_len = (len + kQ - 1) / kQ, c1 = c_all < c_len ? c_all : c_len;
-    Tile<T, NP, W::kThreads> tb, tc;
-    Tile<T, PP, W::kThreads> tx;
+    Load<T, NP, 256> lb, lcc;
+    Load<T, PW, 64> lx;
     float raw = 0.f;
     auto ask = [&](int c) {
         const long long t0 = (long long)c * kQ;
         const int rows = len - t0 < kQ ? (int)(len - t0) : kQ;
-        tb.load(threadIdx.x, Bg + t0 * a.b_tok, a.b_tok, rows, a.N, a.fast_b);
-        tc.load(threadIdx.x, Cg + t0 * a.c_tok, a.c_tok, rows, a.N, a.fast_c);
-        tx.load(threadIdx.x, x + t0 * a.x_tok, a.x_tok, rows, a.P, a.fast_x);
+        lb.ask(threadIdx.x, Bg + t0 * a.b_tok, a.b_tok, rows, a.N, a.how_b);
+        lcc.ask(threadIdx.x, Cg + t0 * a.c_tok, a.c_tok, rows, a.N, a.how_c);
+        lx.ask(lane, x + t0 * a.x_tok, a.x_tok, rows, cols, a.how_x);
+        raw = lane < rows ? a.dt.raw(b, t0 + lane, h) : 0.f;
     };
-    auto ask_step = [&](int c) {  // the steps of as many chunks as there are waves, one chunk per wave
-        const int t = (c + w) * kQ + lane;
-        raw = t < len ? a.dt.raw(b, t, h) : 0.f;
-    };
-    if (c0 < c1) ask(c0), ask_step(c0);
+    if (c0 < c1) ask(c0);
     for (int c = c0; c < c1; ++c) {
-        const int t0 = c * kQ, rows = len - t0 < kQ ? len - t0 : kQ, all = a.L - t0 < kQ ? a.L - t0 : kQ, which = (c - c0) % W::kWaves;
-        T* out = y + (((long long)b * a.L + t0) * a.H + h) * a.P;
+        const int t0 = c * kQ, rows = len - t0 < kQ ? len - t0 : kQ, all = a.L - t0 < kQ ? a.L - t0 : kQ;
+        T* out = y + (((long long)b * a.L + t0) * a.H + h) * a.P + at.p0;
         __syncthreads();  // the chunk before has been read
-        tb.rows(threadIdx.x, Bs), tc.rows(threadIdx.x, Cs);
-        if constexpr (kTwice<T>) tb.columns(threadIdx.x, Bt), tx.columns(threadIdx.x, Xs);
-        else tx.rows(threadIdx.x, Xs);
-        if (which == 0) {
-            put_decays(decays[w], raw, (c + w) * kQ + lane < len, a.dt.softplus, A);
-            if (c + W::kWaves < c1) ask_step(c + W::kWaves);
-        }
-        if (c + 1 < c1) ask(c + 1);
+        lb.put(threadIdx.x, Bs), lcc.put(threadIdx.x, Cs), lx.put(lane, X);
+        put_decays(e, raw, lane < rows, a.dt.softplus, A);
         __syncthreads();
-        const Decays& e = decays[which];
-        // scores of the tiles on and below the diagonal: lane l holds token t = its column, four tokens j = its rows
-        for (int i = w; i < 10; i += W::kWaves) {
-            const int tt = i < 1 ? 0 : i < 3 ? 1 : i < 6 ? 2 : 3, ss = i - tt * (tt + 1) / 2;
-            f32x4 m = {0.f, 0.f, 0.f, 0.f};
+        if (at.works) {
 #pragma unroll
-            for (int k = 0; k < NP / 32; ++k)
-                m = mma(frag(Bs + (16 * ss + lc) * kN + 32 * k + 8 * g), frag(Cs + (16 * tt + lc) * kN + 32 * k + 8 * g), m);
-            const int t = 16 * tt + lc, j = 16 * ss + 4 * g;
-            const float th = e.hi[t], tl = e.lo[t];
-            const f32x4 jh = *reinterpret_cast<const f32x4*>(e.hi + j), jl = *reinterpret_cast<const f32x4*>(e.lo + j), d = *reinterpret_cast<const f32x4*>(e.step + j);
-            T4 v;
+            for (int half = 0; half < 2; ++half) {  // token tiles 2 half and 2 half + 1
+                // read and convert again what both halves use: kept from the first half, it would take a hundred registers
+                asm volatile("" ::: "memory");
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float s = m[i] * exp2_fast((th - jh[i]) + (tl - jl[i])) * d[i];
-                v[i] = (T)(j + i < t ? s : j + i == t ? s + D : 0.f);
-            }
-            *reinterpret_cast<T4*>(Ms + t * kT + j) = v;
-        }
-        f32x4 acc[W::kTiles][4];  // rows p, columns t
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int pt = 0; pt < W::kTiles; ++pt)
+                    for (int pt = 0; pt < PT; ++pt) asm volatile("" : "+v"(S[nt][pt]));
+                Frag<T> q[2][NP / 32], m[2][2];
 #pragma unroll
-            for (int tt = 0; tt < 4; ++tt) acc[pt][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int k = 0; k < NP / 32; ++k) {
-            Frag<T> s[W::kTiles];
+                    for (int k = 0; k < NP / 32; ++k) q[r][k] = Cs.row(ln, 16 * (2 * half + r), 32 * k);
+                // scores: lane l holds token t = its column, four tokens j = its rows
 #pragma unroll
-            for (int pt = 0; pt < W::kTiles; ++pt) s[pt] = frag_of<T>(S[2 * k][pt], S[2 * k + 1][pt]);
+                for (int kk = 0; kk <= half; ++kk) {
+                    f32x4 s[2][2];
 #pragma unroll
-            for (int tt = 0; tt < 4; ++tt) {
-                const Frag<T> q = frag(Cs + (16 * tt + lc) * kN + 32 * k + 4 * g, Cs + (16 * tt + lc) * kN + 32 * k + 16 + 4 * g);
+                    for (int u = 0; u < 2; ++u) {
+                        const int ss = 2 * kk + u;
+                        s[0][u] = s[1][u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int pt = 0; pt < W::kTiles; ++pt) acc[pt][tt] = mma(s[pt], q, acc[pt][tt]);
-            }
-        }
+                        for (int k = 0; k < NP / 32; ++k) {
+                            const Frag<T> bj = Bs.row(ln, 16 * ss, 32 * k);
+                            if (ss <= 2 * half) s[0][u] = mma(bj, q[0][k], s[0][u]);
+                            s[1][u] = mma(bj, q[1][k], s[1][u]);
+                        }
+                        const int j = 16 * ss + 4 * g;
+                        const f32x4 jh = *reinterpret_cast<const f32x4*>(e.hi + j), jl = *reinterpret_cast<const f32x4*>(e.lo + j);
+                        const f32x4 d = *reinterpret_cast<const f32x4*>(e.step + j);
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
-            const float f = e.from[16 * tt + lc];
+                        for (int r = 0; r < 2; ++r) {
+                            const int tt = 2 * half + r, t = 16 * tt + lc;
+                            if (ss > tt) continue;
+                            const float th = e.hi[t], tl = e.lo[t];
 #pragma unroll
-            for (int pt = 0; pt < W::kTiles; ++pt) acc[pt][tt] *= f;
-        }
-        // the state, before the barrier that the scores wait for
-        const float whole = e.from[kQ - 1];
-#pragma unroll
-        for (int pt = 0; pt < W::kTiles; ++pt) {
-            Split<T> xs[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                f32x4 u, v;
-                widen(frag_down(Xs, kP, Xs, 16 * (w * W::kTiles + pt) + lc, 32 * k + 8 * g), u, v);
-                const float *to = e.to + 32 * k + 8 * g, *d = e.step + 32 * k + 8 * g;
-                u *= *reinterpret_cast<const f32x4*>(to) * *reinterpret_cast<const f32x4*>(d);
-                v *= *reinterpret_cast<const f32x4*>(to + 4) * *reinterpret_cast<const f32x4*>(d + 4);
-                split(u, v, xs[k]);
-            }
-#pragma unroll
-            for (int nt = 0; nt < NP / 16; ++nt) {
-                f32x4 s = S[nt][pt] * whole;
-#pragma unroll
-                for (int k = 0; k < 2; ++k) s = mma(frag_down(Bs, kN, Bt, 16 * nt + lc, 32 * k + 8 * g), xs[k], s);
-                S[nt][pt] = s;
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int pt = 0; pt < W::kTiles; ++pt) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const Frag<T> q = frag_down(Xs, kP, Xs, 16 * (w * W::kTiles + pt) + lc, 32 * k + 8 * g);
-#pragma unroll
-                for (int tt = 2 * k; tt < 4; ++tt) acc[pt][tt] = mma(q, frag(Ms + (16 * tt + lc) * kT + 32 * k + 8 * g), acc[pt][tt]);
-            }
-            const int p = 16 * (w * W::kTiles + pt) + 4 * g;
-#pragma unroll
-            for (int tt = 0; tt < 4; ++tt) {
-                const int t = 16 * tt + lc;
-                if (t < all && p < a.P) {
-                    T4 v;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = (T)(t < rows ? acc[pt][tt][i] : 0.f);
-                    T* o = out + (long long)t * a.H * a.P + p;
-                    if (a.P % 4 == 0) {
-                        *reinterpret_cast<T4*>(o) = v;
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (p + i < a.P) o[i] = v[i];
+                            for (int i = 0; i < 4; ++i) {
+                                s[r][u][i] *= exp2_fast((th - jh[i]) + (tl - jl[i])) * d[i];
+                                if (ss == tt) s[r][u][i] = j + i < t ? s[r][u][i] : j + i == t ? s[r][u][i] + D : 0.f;
+                            }
+                        }
                     }
+                    m[0][kk] = frag_of<T>(s[0][0], s[0][1]);
+                    m[1][kk] = frag_of<T>(s[1][0], s[1][1]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+                constexpr int kSome = PT < 2 ? PT : 2;
+#pragma unroll
+                for (int p0 = 0; p0 < PT; p0 += kSome) {
+                    f32x4 acc[2][kSome];  // rows p, columns t
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+#pragma unroll
+                        for (int pt = 0; pt < kSome; ++pt) acc[r][pt] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    // the state in front of the chunk
+#pragma unroll
+                    for (int k = 0; k < NP / 32; ++k)
+#pragma unroll
+                        for (int pt = 0; pt < kSome; ++pt) {
+                            const Frag<T> s = frag_of<T>(S[2 * k][p0 + pt], S[2 * k + 1][p0 + pt]);
+                            acc[0][pt] = mma(s, q[0][k], acc[0][pt]);
+                            acc[1][pt] = mma(s, q[1][k], acc[1][pt]);
+                        }
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float f = e.from[16 * (2 * half + r) + lc];
+#pragma unroll
+                        for (int pt = 0; pt < kSome; ++pt) acc[r][pt] *= f;
+                    }
+#pragma unroll
+                    for (int kk = 0; kk <= half; ++kk)
+#pragma unroll
+                        for (int pt = 0; pt < kSome; ++pt) {
+                            const Frag<T> xj = X.down(lp, 32 * kk, 16 * (p0 + pt));
+                            acc[0][pt] = mma(xj, m[0][kk], acc[0][pt]);
+                            acc[1][pt] = mma(xj, m[1][kk], acc[1][pt]);
+                        }
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const int t = 16 * (2 * half + r) + lc;
+                        T* o = out + (long long)t * a.H * a.P + 4 * g;
+#pragma unroll
+                        for (int pt = 0; pt < kSome; ++pt) {
+                            const int p = 16 * (p0 + pt) + 4 * g;
+                            if (t < all && p < cols) {
+                                T4 v;
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) v[i] = (T)(t < rows ? acc[r][pt][i] : 0.f);
+                                if (a.P % 4 == 0) {
+                                    *reinterpret_cast<T4*>(o + 16 * (p0 + pt)) = v;
+                                } else {
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i)
+                                        if (p + i < cols) o[16 * (p0 + pt) + i] = v[i];
+                                }
+                            }
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
+        if (c + 1 < c1) ask(c + 1);  // the registers of the products above are free again; the state's products hide the loads
+        if (at.works) advance<true>(S, X, Bs, e, false);
     }
+    if (!at.works) return;
     // chunks behind this row's end: nothing but zeros
     for (int c = c0 > c1 ? c0 : c1; c < c_all; ++c) {
-        const int t0 = c * kQ, all = a.L - t0 < kQ ? a.L - t0 : kQ;
-        T* out = y + (((long long)b * a.L + t0) * a.H + h) * a.P;
-        for (int i = threadIdx.x; i < all * a.P; i += W::kThreads) out[(long long)(i / a.P) * a.H * a.P + i % a.P] = (T)0.f;
+        const int t0 = c * kQ, all = a.L - t0 < kQ ? a.L - t0 : kQ, wide = cols < PW ? cols : PW;
+        T* out = y + (((long long)b * a.L + t0) * a.H + h) * a.P + at.p0;
+        for (int i = lane; i < all * wide; i += 64) out[(long long)(i / wide) * a.H * a.P + i % wide] = (T)0.f;
     }
-    if (last && seg == a.segs - 1) {
+    if (last && at.seg == a.segs - 1) {
 #pragma unroll
-        for (int nt = 0; nt < NP / 16; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int pt = 0; pt < W::kTiles; ++pt) {
-                const int p = 16 * (w * W::kTiles + pt) + lc, n = 16 * nt + 4 * g;
-                if (p < a.P) {
-                    float* o = last + (((long long)b * a.H + h) * a.P + p) * a.N + n;
+            for (int pt = 0; pt < PT; ++pt) {
+                const int p = 16 * pt + lc, n = 16 * nt + 4 * g;
+                if (p < cols) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (n + i < a.N) o[i] = S[nt][pt][i];
+                        if (n + i < a.N) last[(state_at + p) * a.N + n + i] = S[nt][pt][i];
                 }
             }
     }
@@ -215,127 +274,92 @@ __global__ __launch_bounds__(Waves<PP>::kThreads, (ScanTiles<T, NP, PP>::kWavesP
 // state, from the gradient of the next chunk's)  S <- e^{s[63]} S + sum_t e^{s[t]} dy[t] C[t]^T.  `x` and `B` of the arguments are dy and C then.
 // Two uses: a first pass over the segments of a row when rows and heads are too few to fill the chip (`ends`, `decays`: each segment's own state from zero,
 // which scan_join_kernel chains), and the states in front of every chunk for the gradients (`tiles`: accumulator tiles as they lie, 1 KB each).
-template <typename T, int NP, int PP> struct WalkTiles {
-    static constexpr int kN = pitch<T>(NP), kP = pitch<T>(PP), kT = pitch<T>(kQ);
-    static constexpr int kB = kTwice<T> ? NP * kT : kQ * kN, kX = kTwice<T> ? PP * kT : kQ * kP;
-};
-
-// two walks in one launch (blockIdx.y): the gradients need both directions at once
-template <typename T, int NP, int PP>
-__global__ __launch_bounds__(Waves<PP>::kThreads, 2) void scan_walk_kernel(ScanArgs a0, WalkOut o0, ScanArgs a1, WalkOut o1) {
-    typedef Waves<PP> W;
-    constexpr int kN = pitch<T>(NP), kP = pitch<T>(PP);
-    __shared__ __attribute__((aligned(16))) T Bs[WalkTiles<T, NP, PP>::kB], Xs[WalkTiles<T, NP, PP>::kX];
-    __shared__ __attribute__((aligned(16))) Decays decays[W::kWaves];
+// Two walks in one launch (blockIdx.y): the gradients need both directions at once.
+template <typename T, int NP, int PW>
+__global__ __launch_bounds__(256, 2) void scan_walk_kernel(ScanArgs a0, WalkOut o0, ScanArgs a1, WalkOut o1) {
+    constexpr int NT = NP / 16, PT = PW / 16;
+    __shared__ __attribute__((aligned(16))) Tile<T, kQ, NP> Bs;
+    __shared__ __attribute__((aligned(16))) Tile<T, kQ, PW> Xs[4];
+    __shared__ __attribute__((aligned(16))) Decays decays[4];
     ScanArgs a = a0;
     WalkOut o = o0;
     if (blockIdx.y) a = a1, o = o1;
-    int b, seg, h;
-    scan_place(a, b, seg, h);
     const int lane = threadIdx.x & 63, w = wave_index(), lc = lane & 15, g = lane >> 4;
-    const int len = row_length(a.lengths, b, a.L);
+    const Place at = scan_place(a, w);
+    const int b = at.b, h = at.head, len = row_length(a.lengths, b, a.L), cols = a.P - at.p0, PP = padded(a.P);
     const float A = a.A[h];
-    const T* x = static_cast<const T*>(a.x) + b * a.x_row + (long long)h * a.P;
-    const T* Bg = static_cast<const T*>(a.B) + b * a.b_row + (long long)(h / (a.H / a.G)) * a.N;
-    const bool chained = o.starts && seg > 0;
+    const T* x = static_cast<const T*>(a.x) + b * a.x_row + (long long)h * a.P + at.p0;
+    const T* Bg = static_cast<const T*>(a.B) + b * a.b_row + (long long)at.grp * a.N;
+    const long long head = (long long)b * a.H + h, state_at = head * a.P + at.p0;
+    const bool chained = o.starts && at.seg > 0;
+    Tile<T, kQ, PW>& X = Xs[w];
+    Decays& e = decays[w];
 
-    f32x4 S[W::kTiles][NP / 16];  // rows p, columns n
+    f32x4 S[PT][NT];  // rows p, columns n
 #pragma unroll
-    for (int pt = 0; pt < W::kTiles; ++pt)
+    for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
-        for (int nt = 0; nt < NP / 16; ++nt) {
-            const int p = 16 * (w * W::kTiles + pt) + 4 * g, n = 16 * nt + lc;
+        for (int nt = 0; nt < NT; ++nt) {
+            const int p = 16 * pt + 4 * g, n = 16 * nt + lc;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float v = 0.f;
-                if (chained) v = o.starts[(((long long)b * a.H + h) * a.segs + seg) * PP * NP + (p + i) * NP + n];
-                else if (!o.ends && a.state && p + i < a.P && n < a.N) v = a.state[(((long long)b * a.H + h) * a.P + p + i) * a.N + n];
+                if (chained) v = o.starts[(head * a.segs + at.seg) * PP * NP + (at.p0 + p + i) * NP + n];
+                else if (!o.ends && a.state && p + i < cols && n < a.N) v = a.state[(state_at + p + i) * a.N + n];
                 S[pt][nt][i] = v;
             }
         }
     // step k of the walk is chunk k, or the k-th from the back
-    const int k0 = seg * a.seg_chunks, k1 = k0 + a.seg_chunks < a.chunks ? k0 + a.seg_chunks : a.chunks;
+    const int k0 = at.seg * a.seg_chunks, k1 = k0 + a.seg_chunks < a.chunks ? k0 + a.seg_chunks : a.chunks;
     auto chunk = [&](int k) { return o.backwards ? a.chunks - 1 - k : k; };
-    Tile<T, NP, W::kThreads> tb;
-    Tile<T, PP, W::kThreads> tx;
+    Load<T, NP, 256> lb;
+    Load<T, PW, 64> lx;
     float raw = 0.f;
     double sum = 0.0;
     auto ask = [&](int k) {
         const long long t0 = (long long)chunk(k) * kQ;
         if (t0 >= len) return;
         const int rows = len - t0 < kQ ? (int)(len - t0) : kQ;
-        tb.load(threadIdx.x, Bg + t0 * a.b_tok, a.b_tok, rows, a.N, a.fast_b);
-        tx.load(threadIdx.x, x + t0 * a.x_tok, a.x_tok, rows, a.P, a.fast_x);
+        lb.ask(threadIdx.x, Bg + t0 * a.b_tok, a.b_tok, rows, a.N, a.how_b);
+        lx.ask(lane, x + t0 * a.x_tok, a.x_tok, rows, cols, a.how_x);
+        raw = lane < rows ? a.dt.raw(b, t0 + lane, h) : 0.f;
     };
-    auto ask_step = [&](int k) {
-        const long long t = (long long)chunk(k + w) * kQ + lane;
-        raw = k + w < k1 && t < len ? a.dt.raw(b, t, h) : 0.f;
-    };
-    ask(k0), ask_step(k0);
+    ask(k0);
     for (int k = k0; k < k1; ++k) {
-        const int c = chunk(k), t0 = c * kQ, which = (k - k0) % W::kWaves;
-        if (o.tiles) {
-            float* to_tile = o.tiles + (((long long)b * a.chunks + c) * a.H + h) * PP * NP;
+        const int c = chunk(k), t0 = c * kQ;
+        if (o.tiles && at.works) {
+            float* to = o.tiles + (((long long)b * a.chunks + c) * a.H + h) * PP * NP + at.p0 * NP + lane * 4;
 #pragma unroll
-            for (int pt = 0; pt < W::kTiles; ++pt)
+            for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
-                for (int nt = 0; nt < NP / 16; ++nt)
-                    *reinterpret_cast<f32x4*>(to_tile + ((w * W::kTiles + pt) * (NP / 16) + nt) * 256 + lane * 4) = S[pt][nt];
+                for (int nt = 0; nt < NT; ++nt) *reinterpret_cast<f32x4*>(to + (pt * NT + nt) * 256) = S[pt][nt];
         }
         __syncthreads();
         if (t0 < len) {
-            if constexpr (kTwice<T>) tb.columns(threadIdx.x, Bs), tx.columns(threadIdx.x, Xs);
-            else tb.rows(threadIdx.x, Bs), tx.rows(threadIdx.x, Xs);
-        }
-        if (which == 0) {
-            put_decays(decays[w], raw, k + w < k1 && (long long)chunk(k + w) * kQ + lane < len, a.dt.softplus, A);
-            if (k + W::kWaves < k1) ask_step(k + W::kWaves);
+            lb.put(threadIdx.x, Bs), lx.put(lane, X);
+            put_decays(e, raw, t0 + lane < len, a.dt.softplus, A);
         }
         if (k + 1 < k1) ask(k + 1);
         __syncthreads();
-        if (t0 >= len) continue;
-        const Decays& e = decays[which];
+        if (t0 >= len || !at.works) continue;
         sum += (double)e.hi[kQ - 1] + (double)e.lo[kQ - 1];
-        const float whole = e.from[kQ - 1];
-#pragma unroll
-        for (int pt = 0; pt < W::kTiles; ++pt) {
-            Split<T> xs[2];
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                f32x4 u, v;
-                widen(frag_down(Xs, kP, Xs, 16 * (w * W::kTiles + pt) + lc, 32 * q + 8 * g), u, v);
-                const int t = 32 * q + 8 * g;
-                if (o.backwards) {
-                    u *= *reinterpret_cast<const f32x4*>(e.from + t), v *= *reinterpret_cast<const f32x4*>(e.from + t + 4);
-                } else {
-                    u *= *reinterpret_cast<const f32x4*>(e.to + t) * *reinterpret_cast<const f32x4*>(e.step + t);
-                    v *= *reinterpret_cast<const f32x4*>(e.to + t + 4) * *reinterpret_cast<const f32x4*>(e.step + t + 4);
-                }
-                split(u, v, xs[q]);
-            }
-#pragma unroll
-            for (int nt = 0; nt < NP / 16; ++nt) {
-                f32x4 s = S[pt][nt] * whole;
-#pragma unroll
-                for (int q = 0; q < 2; ++q) s = mma(xs[q], frag_down(Bs, kN, Bs, 16 * nt + lc, 32 * q + 8 * g), s);
-                S[pt][nt] = s;
-            }
-        }
+        advance<false>(S, X, Bs, e, o.backwards);
     }
-    float* out = o.ends ? o.ends + (((long long)b * a.H + h) * a.segs + seg) * PP * NP : nullptr;
-    const bool final = o.last && seg == a.segs - 1;
+    if (!at.works) return;
+    float* out = o.ends ? o.ends + (head * a.segs + at.seg) * PP * NP + at.p0 * NP : nullptr;
+    const bool final = o.last && at.seg == a.segs - 1;
 #pragma unroll
-    for (int pt = 0; pt < W::kTiles; ++pt)
+    for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
-        for (int nt = 0; nt < NP / 16; ++nt) {
-            const int p = 16 * (w * W::kTiles + pt) + 4 * g, n = 16 * nt + lc;
+        for (int nt = 0; nt < NT; ++nt) {
+            const int p = 16 * pt + 4 * g, n = 16 * nt + lc;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (out) out[(p + i) * NP + n] = S[pt][nt][i];
-                if (final && p + i < a.P && n < a.N) o.last[(((long long)b * a.H + h) * a.P + p + i) * a.N + n] = S[pt][nt][i];
+                if (final && p + i < cols && n < a.N) o.last[(state_at + p + i) * a.N + n] = S[pt][nt][i];
             }
         }
-    if (o.decays && threadIdx.x == 0) o.decays[((long long)b * a.H + h) * a.segs + seg] = exp2_fast((float)sum);
+    if (o.decays && lane == 0 && at.p0 == 0) o.decays[head * a.segs + at.seg] = exp2_fast((float)sum);
 }
 
 // Chains the segments' own states: ends[i] becomes the state in front of segment i.  One thread per state element walks the segments.
@@ -413,29 +437,37 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const T* __restrict__ x,
     if ((threadIdx.x & 7) == 0) y[(b * H + h) * P + p] = (T)(acc + (Dv ? Dv[h] * xv : 0.f));
 }
 
-template <typename T, int NP, int PP>
+static unsigned scan_groups(const ScanArgs& a) { return (unsigned)a.rows * a.segs * a.G * a.quads; }
+
+template <typename T, int NP, int PW>
 static int launch_scan(const ScanArgs& a, const float* starts, void* y, float* last, hipStream_t st) {
-    hipLaunchKernelGGL((scan_kernel<T, NP, PP>), dim3((unsigned)a.rows * a.H * a.segs), dim3(Waves<PP>::kThreads), 0, st, a, starts, static_cast<T*>(y), last);
+    hipLaunchKernelGGL((scan_kernel<T, NP, PW>), dim3(scan_groups(a)), dim3(256), 0, st, a, starts, static_cast<T*>(y), last);
     RTFS_LAUNCH_CHECK();
     return RTFS_OK;
 }
-template <typename T, int NP, int PP>
+template <typename T, int NP, int PW>
 static int launch_walks(const ScanArgs& a0, const WalkOut& o0, const ScanArgs& a1, const WalkOut& o1, int both, hipStream_t st) {
-    hipLaunchKernelGGL((scan_walk_kernel<T, NP, PP>), dim3((unsigned)a0.rows * a0.H * a0.segs, both ? 2 : 1), dim3(Waves<PP>::kThreads), 0, st, a0, o0, a1, o1);
+    hipLaunchKernelGGL((scan_walk_kernel<T, NP, PW>), dim3(scan_groups(a0), both ? 2 : 1), dim3(256), 0, st, a0, o0, a1, o1);
     RTFS_LAUNCH_CHECK();
     return RTFS_OK;
 }
 
 int scan_walks(const ScanArgs& a0, const WalkOut& o0, const ScanArgs& a1, const WalkOut& o1, int both, int type, hipStream_t st) {
-    RTFS_SSM_DISPATCH(type, a0.N, a0.P, launch_walks, (a0, o0, a1, o1, both, st));
+    RTFS_SSM_DISPATCH(type, a0.N, 16, 32, a0.width, launch_walks, (a0, o0, a1, o1, both, st));
 }
 
-// Segments per row.  One workgroup per row and head walks its chunks in order; below two workgroups per CU rows are cut, as far as four chunks per segment, and
-// each segment's own state is walked first (B, x and dt read twice, half the products again).
+// A wave takes 64, 32 or 16 columns of P: the widest that leaves a group's heads four waves of work (the scores of a head are formed by each of its waves), and
+// whose state of N values each fits a wave's registers next to the loads in flight (64 columns of 128 spilled).
+// Rows are cut into segments, each walked by workgroups of its own, as far as it takes to give every CU two workgroups and no further than four chunks: a
+// segment's own state is walked first then (B, x and dt read twice, the state's products done twice).
 void scan_cut(ScanArgs& a) {
+    const int each = a.H / a.G;
+    for (a.width = a.P <= 16 ? 16 : a.P <= 32 || a.N > 64 ? 32 : 64; a.width > 16 && each * ((a.P + a.width - 1) / a.width) < 4; a.width /= 2) {}
+    a.slices = (a.P + a.width - 1) / a.width;
+    a.quads = (each * a.slices + 3) / 4;
     a.chunks = (a.L + kQ - 1) / kQ;
-    const long long work = (long long)a.rows * a.H;
-    const long long want = work >= 512 ? 1 : (1024 + work - 1) / work;
+    const long long groups = (long long)a.rows * a.G * a.quads;
+    const long long want = groups >= 512 ? 1 : (512 + groups - 1) / groups;
     const long long per = (a.chunks + want - 1) / want;
     a.seg_chunks = (int)(want == 1 ? a.chunks : per < 4 ? 4 : per);
     a.segs = (a.chunks + a.seg_chunks - 1) / a.seg_chunks;
@@ -474,10 +506,10 @@ using namespace rtfs::ssm;
 
 extern "C" {
 
-int rtfs_ssm_scan_segments(int B, int L, int H) {
-    if (B <= 0 || L <= 0 || H <= 0) return RTFS_EINVAL;
+int rtfs_ssm_scan_segments(int B, int L, int H, int P, int G, int N) {
+    if (!scan_sizes(B, L, H, P, G, N)) return RTFS_EINVAL;
     ScanArgs a{};
-    a.rows = B, a.L = L, a.H = H;
+    a.rows = B, a.L = L, a.H = H, a.P = P, a.G = G, a.N = N;
     scan_cut(a);
     return a.segs;
 }
@@ -488,7 +520,9 @@ int rtfs_ssm_scan_fwd(const void* x, long long x_row, long long x_tok, const voi
                       const void* Bm, long long b_row, long long b_tok, const void* C, long long c_row, long long c_tok, const float* D, const float* dt_bias,
                       int softplus, const float* state, const int* lengths, void* y, float* last, float* work, int B, int L, int H, int P, int G, int N, int type,
                       void* stream) {
-    if (!x || !dt || !A || !Bm || !C || !y || !scan_sizes(B, L, H, P, G, N) || type < 0 || type > 1 || dt_type < 0 || dt_type > 1) return RTFS_EINVAL;
+    if (!x || !dt || !A || !Bm || !C || !y || !scan_sizes(B, L, H, P, G, N) || type < 0 || type > 1 || dt_type < 0 || dt_type > 1 ||
+        !scan_pitch(x_tok) || !scan_pitch(b_tok) || !scan_pitch(c_tok))
+        return RTFS_EINVAL;
     ScanArgs a = scan_args(x, x_row, x_tok, Steps{dt, dt_row, dt_tok, dt_type, dt_bias, softplus}, A, Bm, b_row, b_tok, C, c_row, c_tok, D, state, lengths, B, L, H,
                            P, G, N, type);
     hipStream_t st = (hipStream_t)stream;
@@ -497,7 +531,7 @@ int rtfs_ssm_scan_fwd(const void* x, long long x_row, long long x_tok, const voi
         const int rc = scan_starts(a, a, nullptr, work, 0, type, st);
         if (rc != RTFS_OK) return rc;
     }
-    RTFS_SSM_DISPATCH(type, N, P, launch_scan, (a, work, y, last, st));
+    RTFS_SSM_DISPATCH(type, N, 16, 32, a.width, launch_scan, (a, work, y, last, st));
 }
 
 int rtfs_ssm_step(const void* x, long long x_row, const void* dt, long long dt_row, int dt_type, const float* A, const void* Bm, long long b_row, const void* C,

@@ -57,8 +57,11 @@ def _on_gpu(name, x):
 
 
 def _tokens(t, dims):
-    """t with its last `dims` dimensions contiguous, and its row and token pitches in elements (of [B, L, ...])"""
+    """t with its last `dims` dimensions contiguous, and its row and token pitches in elements (of [B, L, ...]); tokens further apart than the kernels' 32-bit
+    offsets allow are copied together"""
     size = 1
+    if t.stride(1) >= 1 << 23:
+        t = t.contiguous()
     for n, s in zip(t.shape[:-dims - 1:-1], t.stride()[:-dims - 1:-1]):
         if n != 1 and s != size:
             t = t.contiguous()
@@ -180,7 +183,7 @@ class _SelectiveScan(torch.autograd.Function):
         y = torch.empty(B, L, H, P, dtype=x.dtype, device=x.device)
         last = torch.empty(B, H, P, N, device=x.device) if want_state else None
         handle = lib.load()
-        segs = handle.rtfs_ssm_scan_segments(B, L, H)
+        segs = handle.rtfs_ssm_scan_segments(B, L, H, P, G, N)
         work = torch.empty(B * H * segs * (handle.rtfs_ssm_tile(P, N) + 1), device=x.device) if segs > 1 else None
         lib.call("rtfs_ssm_scan_fwd", _raw(x), xr, xt, _raw(dt), tr, tt, _TYPES[dt.dtype], A, _raw(Bm), br, bt, _raw(C), cr, ct, D, dt_bias, int(softplus), state,
                  lengths, y, last, work, B, L, H, P, G, N, _TYPES[x.dtype])
@@ -206,7 +209,7 @@ class _SelectiveScan(torch.autograd.Function):
         dA, dD, db = new(H), new(H) if D is not None else None, new(H) if dt_bias is not None else None
         ds = torch.empty_like(state) if state is not None else None
         handle = lib.load()
-        segs, tile, parts, chunks = handle.rtfs_ssm_scan_segments(B, L, H), handle.rtfs_ssm_tile(P, N), handle.rtfs_ssm_scan_bwd_parts(B, L, H, G), -(-L // 64)
+        segs, tile, parts, chunks = handle.rtfs_ssm_scan_segments(B, L, H, P, G, N), handle.rtfs_ssm_tile(P, N), handle.rtfs_ssm_scan_bwd_parts(B, L, H, G), -(-L // 64)
         starts = new(2 * B * H * segs * (tile + 1)) if segs > 1 else None
         wide = new(2 * parts * B * L * G * N) if parts > 1 else None
         lib.call("rtfs_ssm_scan_bwd", _raw(x), xr, xt, _raw(dt), tr, tt, _TYPES[dt.dtype], A, _raw(Bm), br, bt, _raw(C), cr, ct, D, dt_bias, int(ctx.softplus), state,
