@@ -18,8 +18,9 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 // ---- fragments ------------------------------------------------------------------------------------------------------------------------------------------
 // One fragment is a 16 x 32 operand of D[16x16] += A[16x32] B[32x16]: lane l holds 8 values of row (A) or column (B) l & 15; which 8 of the 32 products it
-// holds is free as long as A and B agree.  Here, with g = l >> 4: k = 4 g + j and 16 + 4 g + j (j < 4), which is how two accumulator tiles lie in registers
-// (lane l: column l & 15, rows 4 g + i) - an accumulator becomes an operand without leaving its lane.
+// holds is free as long as A and B agree.  With g = l >> 4, two accumulator tiles (lane l: column l & 15, rows 4 g + i) become an operand without leaving their
+// lane, of the products 4 g + j and 16 + 4 g + j (j < 4) of their 32 rows - or of 8 g + j and 8 g + 4 + j, if row 4 g + i of the pair's first tile stands for
+// value 8 g + i and that of its second for 8 g + 4 + i.  The latter is how tiles over N lie (swapped()), so that rows of B and C are read 16 bytes at a time.
 // fp32 goes through v_mfma_f32_16x16x4_f32 (exact products, one value per lane and step), bf16 through one v_mfma_f32_16x16x32_bf16.
 template <typename T> struct Frag;
 template <> struct Frag<float> { f32x4 a, b; };
@@ -72,98 +73,121 @@ __device__ __forceinline__ void widen(const Frag<__bf16>& f, f32x4& a, f32x4& b)
     for (int j = 0; j < 4; ++j) a[j] = (float)f.v[j], b[j] = (float)f.v[4 + j];
 }
 
+// the value of N that place i (0 .. 15) of tile t stands for
+__device__ __forceinline__ int swapped(int t, int i) { return 32 * (t >> 1) + 8 * (i >> 2) + 4 * (t & 1) + (i & 3); }
+
 // ---- tiles in LDS -----------------------------------------------------------------------------------------------------------------------------------------
-// ROWS x COLS values, read two ways as operands: 4 + 4 neighbours of a row (products over values: row()), and 4 + 4 rows of a column (products over tokens:
-// down()).  fp32 takes down() one value at a time, as many bytes per cycle; rows are 16 bytes apart from a multiple of all banks.  bf16 takes it with the
-// transposing read ds_read_b64_tr_b16 (16 lanes fetch four rows of 16 values, each lane gets one column of them), so no tile is stored twice.  Its rows have no
-// padding; instead the 8-byte granules of a row are permuted by an exclusive or with a code of the row that sends the 16 rows of a row() read and the four
-// rows x four granules of a down() read to 16 different pairs of banks (a tile of 16 columns is only read down(): it needs none).
+// ROWS x COLS values, read two ways as operands: 8 values of a row (products over values: row()), and 4 + 4 rows of a column (products over tokens: down()).
+// Three KINDs, by what their accumulator tiles are to be:
+//   kSwapped  B and C: row() gives values 8 g .. 8 g + 7; lane i of a down() tile gets column swapped(t, i)
+//   kInOrder  x and dy of the gradients, scores: row() gives values 4 g .. and 16 + 4 g ..; lane i of a down() tile gets column 16 t + i
+//   kDownOnly x of the scan, states: down() as kInOrder, no row()
+// fp32 takes down() one value at a time, as many bytes per cycle; rows are 16 bytes apart from a multiple of all banks.  bf16 takes it with the transposing
+// read ds_read_b64_tr_b16 (16 lanes fetch four rows of 16 values, each lane gets one column of them), so no tile is stored twice.  Its rows have no padding;
+// their 16-byte chunks are permuted by an exclusive or with a code of the row instead: the eight rows of a phase of row() and the four rows of down() meet
+// different banks (kSwapped's down(): twice each, it takes one half of every chunk).  kInOrder stores granules of four so that the 16 bytes row() reads are the
+// right ones.
+enum Kind { kSwapped, kInOrder, kDownOnly };
+
 template <typename T> struct Vec8;
 template <> struct Vec8<float> { f32x4 a, b; };
 template <> struct Vec8<__bf16> { bf16x8 v; };
+
 // Where a lane reads, in values from the start of a tile of COLS columns; formed once, all else is a constant added to it.
-template <typename T, int COLS> struct Lanes;
-template <int COLS> struct Lanes<float, COLS> {
+template <typename T, int COLS, Kind KIND> struct Lanes;
+template <int COLS, Kind KIND> struct Lanes<float, COLS, KIND> {
     static constexpr int kPitch = COLS + 4;
     int row, down;
     __device__ __forceinline__ Lanes() {
         const int lane = threadIdx.x & 63, lc = lane & 15, g = lane >> 4;
-        row = lc * kPitch + 4 * g, down = 4 * g * kPitch + lc;
+        row = lc * kPitch + (KIND == kSwapped ? 8 * g : 4 * g), down = 4 * g * kPitch + (KIND == kSwapped ? swapped(0, lc) : lc);
     }
 };
-template <int COLS> struct Lanes<__bf16, COLS> {
-    // Granules c / 4 of a row r lie at (c / 4) ^ code(r): 16 (COLS = 32: 8, 16: 4) of them permuted, the codes chosen so that ...
-    __device__ __forceinline__ static int code(int r) {
-        return COLS >= 64 ? (r & 3) << 2 | ((r >> 2) & 3) : COLS == 32 ? ((r >> 1) & 1) << 2 | ((r >> 2) & 3) : 0;
-    }
-    // ... a constant granule 4 v in front of a lane's own is an exclusive or with it: one offset per v, and the rest of the constant is added
-    static constexpr int kOffsets = COLS >= 64 ? 4 : COLS / 16;
-    int row[kOffsets], down[kOffsets];
+template <int COLS, Kind KIND> struct Lanes<__bf16, COLS, KIND> {
+    // chunk c of row r lies at c ^ code(r); 128 bytes of banks hold one row of 64 values, two of 32, four of 16
+    __device__ __forceinline__ static int code(int r) { return COLS >= 64 ? (r & 1) << 2 | (r & 2) | ((r >> 2) & 1) : COLS == 32 ? (r & 2) | ((r >> 2) & 1) : 0; }
+    // a constant chunk in front of a lane's own is an exclusive or with it where it is among the permuted ones: one offset each, the rest is added
+    static constexpr int kRow = COLS >= 64 ? 2 : 1, kDown = KIND != kDownOnly ? kRow : COLS >= 64 ? 4 : COLS / 16;
+    int row[kRow], down[kDown];
     __device__ __forceinline__ Lanes() {
-        const int lane = threadIdx.x & 63, lc = lane & 15, g = lane >> 4, r = 4 * g + (lc >> 2);
+        const int lane = threadIdx.x & 63, lc = lane & 15, g = lane >> 4, r = 4 * g + (lc >> 2), q = lc & 3;
 #pragma unroll
-        for (int v = 0; v < kOffsets; ++v) {
-            row[v] = lc * COLS + ((g ^ code(lc) ^ v << 2) << 2);
-            down[v] = r * COLS + (((lc & 3) ^ code(r) ^ v << 2) << 2);
-        }
+        for (int v = 0; v < kRow; ++v) row[v] = lc * COLS + ((g ^ code(lc) ^ v << 2) << 3);
+#pragma unroll
+        for (int v = 0; v < kDown; ++v)
+            down[v] = r * COLS + (KIND != kDownOnly ? (q ^ code(r) ^ v << 2) << 3 : ((q >> 1) ^ code(r) ^ v << 1) << 3 | (q & 1) << 2);
     }
 };
 
-template <typename T, int ROWS, int COLS> struct Tile;
+template <typename T, int ROWS, int COLS, Kind KIND> struct Tile;
 
-template <int ROWS, int COLS> struct Tile<float, ROWS, COLS> {
-    typedef Lanes<float, COLS> Lane;
+template <int ROWS, int COLS, Kind KIND> struct Tile<float, ROWS, COLS, KIND> {
+    typedef Lanes<float, COLS, KIND> Lane;
     static constexpr int kPitch = Lane::kPitch, kBytes = ROWS * kPitch * 4;
     float v[ROWS * kPitch];
-    __device__ __forceinline__ void put8(int r, int c, const Vec8<float>& x) {
-        *reinterpret_cast<f32x4*>(v + r * kPitch + c) = x.a;
-        *reinterpret_cast<f32x4*>(v + r * kPitch + c + 4) = x.b;
+    // where 8 neighbours of a row go; rows 8 apart are 8 * kPitch apart
+    struct Place {
+        int at;
+        __device__ __forceinline__ Place(int r, int c) : at(r * kPitch + c) {}
+    };
+    __device__ __forceinline__ void put8(const Place& p, int rows, const Vec8<float>& x) {
+        *reinterpret_cast<f32x4*>(v + p.at + rows * kPitch) = x.a;
+        *reinterpret_cast<f32x4*>(v + p.at + rows * kPitch + 4) = x.b;
     }
     __device__ __forceinline__ void put4(int r, int c, f32x4 x) { *reinterpret_cast<f32x4*>(v + r * kPitch + c) = x; }
     __device__ __forceinline__ void put(int r, int c, float x) { v[r * kPitch + c] = x; }
     __device__ __forceinline__ float get(int r, int c) const { return v[r * kPitch + c]; }
-    // r, c: multiples of 16.  Lane l: row r + (l & 15), values c + 4 g .. and c + 16 + 4 g ..
+    // lane l: row r + (l & 15), values from c (a multiple of 32) on
     __device__ __forceinline__ Frag<float> row(const Lane& l, int r, int c) const {
         const float* p = v + l.row + r * kPitch + c;
-        return {*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + 16)};
+        return {*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + (KIND == kSwapped ? 4 : 16))};
     }
-    __device__ __forceinline__ Frag<float> down_any(int r, int c) const { return down(Lane(), r, c); }
-    // lane l: column c + (l & 15), rows r + 4 g .. and r + 16 + 4 g ..
-    __device__ __forceinline__ Frag<float> down(const Lane& l, int r, int c) const {
-        const float* p = v + l.down + r * kPitch + c;
+    // lane l: place l & 15 of column tile t, rows r + 4 g .. and r + 16 + 4 g ..
+    __device__ __forceinline__ Frag<float> down(const Lane& l, int r, int t) const {
+        const float* p = v + l.down + r * kPitch + (KIND == kSwapped ? swapped(t, 0) : 16 * t);
         Frag<float> f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) f.a[j] = p[j * kPitch], f.b[j] = p[(16 + j) * kPitch];
         return f;
     }
+    __device__ __forceinline__ Frag<float> down_any(int r, int t) const { return down(Lane(), r, t); }  // t not known to the compiler
 };
 
-template <int ROWS, int COLS> struct Tile<__bf16, ROWS, COLS> {
-    typedef Lanes<__bf16, COLS> Lane;
+template <int ROWS, int COLS, Kind KIND> struct Tile<__bf16, ROWS, COLS, KIND> {
+    typedef Lanes<__bf16, COLS, KIND> Lane;
     static constexpr int kBytes = ROWS * COLS * 2;
     __bf16 v[ROWS * COLS];
     typedef short s16x4 __attribute__((ext_vector_type(4)));
-    __device__ __forceinline__ static int at(int r, int c) { return r * COLS + ((c >> 2 ^ Lane::code(r)) << 2 | (c & 3)); }
-    __device__ __forceinline__ void put8(int r, int c, const Vec8<__bf16>& x) {
-        *reinterpret_cast<bf16x4*>(v + at(r, c)) = __builtin_shufflevector(x.v, x.v, 0, 1, 2, 3);
-        *reinterpret_cast<bf16x4*>(v + at(r, c + 4)) = __builtin_shufflevector(x.v, x.v, 4, 5, 6, 7);
+    // four neighbours from column c (a multiple of 4) on; granule 4 h + g of eight is stored as 2 g + h where KIND is kInOrder
+    __device__ __forceinline__ static int at(int r, int c) {
+        const int q = c >> 2, s = KIND == kInOrder ? (q & ~7) | (q & 3) << 1 | ((q >> 2) & 1) : q;
+        return r * COLS + ((s >> 1 ^ Lane::code(r)) << 3 | (s & 1) << 2 | (c & 3));
+    }
+    struct Place {
+        int at0, at1;
+        __device__ __forceinline__ Place(int r, int c) : at0(at(r, c)), at1(KIND == kInOrder ? at(r, c + 4) : 0) {}
+    };
+    __device__ __forceinline__ void put8(const Place& p, int rows, const Vec8<__bf16>& x) {
+        if (KIND == kInOrder) {
+            *reinterpret_cast<bf16x4*>(v + p.at0 + rows * COLS) = __builtin_shufflevector(x.v, x.v, 0, 1, 2, 3);
+            *reinterpret_cast<bf16x4*>(v + p.at1 + rows * COLS) = __builtin_shufflevector(x.v, x.v, 4, 5, 6, 7);
+        } else {
+            *reinterpret_cast<bf16x8*>(v + p.at0 + rows * COLS) = x.v;
+        }
     }
     __device__ __forceinline__ void put4(int r, int c, f32x4 x) { *reinterpret_cast<bf16x4*>(v + at(r, c)) = __builtin_convertvector(x, bf16x4); }
     __device__ __forceinline__ void put(int r, int c, float x) { v[at(r, c)] = (__bf16)x; }
     __device__ __forceinline__ float get(int r, int c) const { return (float)v[at(r, c)]; }
     __device__ __forceinline__ Frag<__bf16> row(const Lane& l, int r, int c) const {
-        constexpr int m = Lane::kOffsets - 1;
-        const __bf16* p = v + r * COLS + (c >> 6 << 6);
-        const bf16x4 a = *reinterpret_cast<const bf16x4*>(p + l.row[c >> 4 & m]), b = *reinterpret_cast<const bf16x4*>(p + l.row[(c + 16) >> 4 & m]);
-        return {__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7)};
+        return {*reinterpret_cast<const bf16x8*>(v + r * COLS + (c >> 6 << 6) + l.row[c >> 5 & (Lane::kRow - 1)])};
     }
-    __device__ __forceinline__ Frag<__bf16> down(const Lane& l, int r, int c) const {
-        return down_from(v + r * COLS + (c >> 6 << 6) + l.down[c >> 4 & (Lane::kOffsets - 1)]);
+    __device__ __forceinline__ Frag<__bf16> down(const Lane& l, int r, int t) const {
+        if (KIND == kDownOnly) return down_from(v + r * COLS + (t >> 2 << 6) + l.down[t & (Lane::kDown - 1)]);
+        return down_from(v + r * COLS + (t >> 2 << 6) + 4 * (t & 1) + l.down[t >> 1 & (Lane::kDown - 1)]);
     }
-    // the same where c is not known to the compiler
-    __device__ __forceinline__ Frag<__bf16> down_any(int r, int c) const {
-        const int lane = threadIdx.x & 63;
-        return down_from(v + at(r + 4 * (lane >> 4) + (lane >> 2 & 3), c + 4 * (lane & 3)));
+    __device__ __forceinline__ Frag<__bf16> down_any(int r, int t) const {
+        const int lane = threadIdx.x & 63, m = r + 4 * (lane >> 4) + (lane >> 2 & 3), q = lane & 3;
+        return down_from(v + at(m, KIND == kSwapped ? swapped(t, 4 * q) : 16 * t + 4 * q));
     }
     __device__ __forceinline__ static Frag<__bf16> down_from(const __bf16* p) {
         typedef __attribute__((address_space(3))) s16x4* lds;
@@ -224,30 +248,32 @@ struct Load {
     Vec8<T> r[kPer];
 
     __device__ __forceinline__ void ask(unsigned thread, const T* src, long long pitch, int rows, int cols, int how) {
-        // formed anew at every call: hoisted out of the chunk loop, the addresses of the value-by-value path alone take a hundred registers
-        asm volatile("" : "+v"(thread));
         // without a token the bound is 0: nothing is read (below 0 it would be no bound at all)
         const int bytes = rows > 0 ? (int)(((rows - 1) * pitch + cols) * (long long)sizeof(T)) : 0;
         const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(src), 0, bytes, 0x00027000);
         const unsigned step = (unsigned)pitch * sizeof(T);
-        auto all = [&](auto load) {
+        auto all = [&](unsigned thread, auto load) {
+            const unsigned c = thread % kVecs * 8, at = thread / kVecs * step + c * (unsigned)sizeof(T);
 #pragma unroll
-            for (int k = 0; k < kPer; ++k) {
-                const unsigned u = thread + k * THREADS, c = u % kVecs * 8, at = u / kVecs * step + c * (unsigned)sizeof(T);
-                load(r[k], at, kUnits % THREADS == 0 || u < kUnits ? cols - (int)c : 0);
-            }
+            for (int k = 0; k < kPer; ++k)
+                load(r[k], at + k * (THREADS / kVecs) * step, kUnits % THREADS == 0 || thread + k * THREADS < kUnits ? cols - (int)c : 0);
         };
-        if (how == kAligned) all([&](Vec8<T>& v, unsigned at, int n) { load8(v, rsrc, at, n); });
-        else if (how == kAnywhere && cols * (int)sizeof(T) >= 16) all([&](Vec8<T>& v, unsigned at, int n) { load8_anywhere(v, rsrc, at, n); });
-        else all([&](Vec8<T>& v, unsigned at, int n) { load8_singly(v, rsrc, at, n); });
-    }
-    __device__ __forceinline__ void put(unsigned thread, Tile<T, kQ, COLS>& tile) const {
-        asm volatile("" : "+v"(thread));
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-            const unsigned u = thread + k * THREADS;
-            if (kUnits % THREADS == 0 || u < kUnits) tile.put8(u / kVecs, u % kVecs * 8, r[k]);
+        if (how == kAligned) {
+            all(thread, [&](Vec8<T>& v, unsigned at, int n) { load8(v, rsrc, at, n); });
+            return;
         }
+        // formed anew at every call: hoisted out of the chunk loop, these offsets and conditions would take a hundred registers
+        asm volatile("" : "+v"(thread));
+        if (how == kAnywhere && cols * (int)sizeof(T) >= 16) all(thread, [&](Vec8<T>& v, unsigned at, int n) { load8_anywhere(v, rsrc, at, n); });
+        else all(thread, [&](Vec8<T>& v, unsigned at, int n) { load8_singly(v, rsrc, at, n); });
+    }
+    template <Kind KIND>
+    __device__ __forceinline__ void put(unsigned thread, Tile<T, kQ, COLS, KIND>& tile) const {
+        const typename Tile<T, kQ, COLS, KIND>::Place place(thread / kVecs, thread % kVecs * 8);
+        static_assert(THREADS / kVecs % 8 == 0, "a thread's rows are a multiple of 8 apart");
+#pragma unroll
+        for (int k = 0; k < kPer; ++k)
+            if (kUnits % THREADS == 0 || thread + k * THREADS < kUnits) tile.put8(place, k * (THREADS / kVecs), r[k]);
     }
 };
 
@@ -279,6 +305,9 @@ struct Steps {
     }
 };
 
+// a lane's value in all lanes
+__device__ __forceinline__ float lane_value(float v, int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); }
+
 template <int CTRL, int ROWS>
 __device__ __forceinline__ double dpp_add(double v) {
     const long long bits = __builtin_bit_cast(long long, v);
@@ -309,13 +338,34 @@ struct Decays {
 __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
 
 // by one wave for one chunk; `raw`: this lane's dt (with bias), `alive`: whether its token is within the row
-__device__ __forceinline__ void put_decays(Decays& o, float raw, bool alive, bool plus, float A) {
+struct Decay {
+    float step, hi, lo;  // of this lane's token
+};
+__device__ __forceinline__ Decay put_decays(Decays& o, float raw, bool alive, bool plus, float A) {
     const int lane = threadIdx.x & 63;
-    const float d = !alive ? 0.f : plus ? softplus(raw) : raw;
-    float hi, lo;
-    chunk_decay(d, A, hi, lo);
-    const float eh = __shfl(hi, 63, 64), el = __shfl(lo, 63, 64);
-    o.hi[lane] = hi, o.lo[lane] = lo, o.step[lane] = d, o.from[lane] = exp2_fast(hi), o.to[lane] = exp2_fast((eh - hi) + (el - lo));
+    Decay e;
+    e.step = !alive ? 0.f : plus ? softplus(raw) : raw;
+    chunk_decay(e.step, A, e.hi, e.lo);
+    const float eh = lane_value(e.hi, 63), el = lane_value(e.lo, 63);
+    o.hi[lane] = e.hi, o.lo[lane] = e.lo, o.step[lane] = e.step, o.from[lane] = exp2_fast(e.hi), o.to[lane] = exp2_fast((eh - e.hi) + (el - e.lo));
+    return e;
+}
+
+// e^{s[t]-s[j]} of tokens in different tiles of 16 as a product of two factors, with the last token r in front of t's tile between them: both are at most 1 where
+// states decay.  near[t] = e^{s[t]-s[r]}; far[k][j] = e^{s[r]-s[j]} weight[j] for the tile k + 1 of t, j <= r.
+struct Factors {
+    float near[kQ], far[3][kQ];
+};
+__device__ __forceinline__ void put_factors(Factors& o, const Decay& e, float weight) {
+    const int lane = threadIdx.x & 63;
+    float nh = 0.f, nl = 0.f;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        const float rh = lane_value(e.hi, 16 * k + 15), rl = lane_value(e.lo, 16 * k + 15);
+        o.far[k][lane] = lane <= 16 * k + 15 ? exp2_fast((rh - e.hi) + (rl - e.lo)) * weight : 0.f;
+        if (lane >> 4 == k + 1) nh = rh, nl = rl;
+    }
+    o.near[lane] = exp2_fast((e.hi - nh) + (e.lo - nl));
 }
 
 // blocks that follow each other share inputs (heads of a group): hand each XCD a contiguous part of them (workgroup i runs on XCD i % 8)

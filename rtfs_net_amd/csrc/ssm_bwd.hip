@@ -41,10 +41,10 @@ template <typename T, int NP, int PP> struct GradTiles {
     static constexpr int kWaves = NP == 128 ? 8 : 4, kThreads = 64 * kWaves, kHalf = kWaves / 2, kAlt = kWaves / 4;
     static constexpr int kSlices = NP / 16 / kHalf;  // 16-wide slices of N per wave
     static constexpr int PB = PP < 64 ? PP : 64;
-    typedef Tile<T, kQ, NP> Wide;
-    typedef Tile<T, kQ, PB> Slim;
-    typedef Tile<T, NP, PB> States;
-    typedef Tile<T, kQ, kQ> Scores;
+    typedef Tile<T, kQ, NP, kSwapped> Wide;
+    typedef Tile<T, kQ, PB, kInOrder> Slim;
+    typedef Tile<T, NP, PB, kDownOnly> States;
+    typedef Tile<T, kQ, kQ, kInOrder> Scores;
     static constexpr int kMain = 2 * Slim::kBytes + States::kBytes, kPool = kMain > Scores::kBytes ? kMain : Scores::kBytes;
     static constexpr int kBytes = 2 * Wide::kBytes + kPool + kRing * (int)(sizeof(Decays) + sizeof(HeadSums));
     static constexpr int kWavesPerSimd = kWaves == 8 || kBytes * 2 <= 160 * 1024 ? 2 : 1;
@@ -60,7 +60,7 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
     __shared__ __attribute__((aligned(16))) Decays decays[kRing];
     __shared__ __attribute__((aligned(16))) HeadSums sums[kRing];
     typename S::Slim &Ys = *reinterpret_cast<typename S::Slim*>(pool), &Xs = *reinterpret_cast<typename S::Slim*>(pool + S::Slim::kBytes);
-    typename S::States& Gs = *reinterpret_cast<typename S::States*>(pool + 2 * S::Slim::kBytes);  // rows n
+    typename S::States& Gs = *reinterpret_cast<typename S::States*>(pool + 2 * S::Slim::kBytes);  // rows: places of n
     const ScanArgs& a = q.a;
     unsigned i0 = xcd_block(blockIdx.x, gridDim.x);
     const int part = (int)(i0 % q.parts);
@@ -100,6 +100,7 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     const typename S::Wide::Lane ln;
     const typename S::Slim::Lane lp;
+    const typename S::States::Lane lg;
     f32x4 cb[4], dcb[4], sum[4][NS];  // rows t, columns j; rows t, columns n
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) {
@@ -229,7 +230,7 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
                     for (int i = 0; i < 4; ++i) {
 #pragma unroll
                         for (int s = 0; s < NS; ++s) {
-                            r[i] = fmaf(Ks.get(t + i, 16 * (first + S::kHalf * s) + lc), R[tt][s][i], r[i]);
+                            r[i] = fmaf(Ks.get(t + i, swapped(first + S::kHalf * s, lc)), R[tt][s][i], r[i]);
                             sum[tt][s][i] = fmaf(f[i], R[tt][s][i], sum[tt][s][i]);
                         }
                         r[i] = row16_sum(r[i]);
@@ -250,11 +251,11 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
                 if (pt % S::kAlt != alt) continue;
                 f32x4 acc = zero;  // rows p, columns j
 #pragma unroll
-                for (int k = 0; k < NP / 32; ++k) acc = mma(Gs.down(lp, 32 * k, 16 * pt), Bs.row(ln, 16 * jt, 32 * k), acc);
+                for (int k = 0; k < NP / 32; ++k) acc = mma(Gs.down(lg, 32 * k, pt), Bs.row(ln, 16 * jt, 32 * k), acc);
                 acc *= end;
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
-                    if (2 * k + 1 >= jt) acc = mma(Ys.down(lp, 32 * k, 16 * pt), wgt[k], acc);
+                    if (2 * k + 1 >= jt) acc = mma(Ys.down(lp, 32 * k, pt), wgt[k], acc);
                 const int p = 16 * pt + 4 * g;
                 if (j < all && p0 + p < a.P) {
                     T4 v;
@@ -312,12 +313,12 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
     const typename S::Wide& Os = role_v ? Cs : Bs;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-        const int n = 16 * (first + S::kHalf * s) + lc;
+        const int n = swapped(first + S::kHalf * s, lc);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const Frag<T> o = Os.down_any(32 * k, 16 * (first + S::kHalf * s));
+            const Frag<T> o = Os.down_any(32 * k, first + S::kHalf * s);
 #pragma unroll
-            for (int tt = 0; tt < 4; ++tt) sum[tt][s] = mma(role_v ? Ms.down(lq, 32 * k, 16 * tt) : Ms.row(lq, 16 * tt, 32 * k), o, sum[tt][s]);
+            for (int tt = 0; tt < 4; ++tt) sum[tt][s] = mma(role_v ? Ms.down(lq, 32 * k, tt) : Ms.row(lq, 16 * tt, 32 * k), o, sum[tt][s]);
         }
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)

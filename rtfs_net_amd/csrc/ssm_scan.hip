@@ -30,13 +30,13 @@ __device__ __forceinline__ Place scan_place(const ScanArgs& a, int w) {
 }
 
 // S <- e^{s[63]} S + sum_j (weight[j] x[j]) B[j]^T, with the weights of a forward or a backward walk.  The weighted x, split, is one operand, tokens of B's
-// columns the other, each read once; the state's tiles lie rows n, columns p (S[n][p], the forward kernel's) or rows p, columns n (S[p][n], the walks').
+// columns the other, each read once; the state's tiles lie rows n (swapped()), columns p (S[n][p], the forward kernel's) or rows p, columns n (S[p][n], the walks').
 template <bool N_FIRST, typename T, int NP, int PW, int R, int C>
-__device__ __forceinline__ void advance(f32x4 (&S)[R][C], const Tile<T, kQ, PW>& X, const Tile<T, kQ, NP>& Bs, const Decays& e, bool backwards) {
+__device__ __forceinline__ void advance(f32x4 (&S)[R][C], const Tile<T, kQ, PW, kDownOnly>& X, const Tile<T, kQ, NP, kSwapped>& Bs, const Decays& e, bool backwards) {
     constexpr int NT = NP / 16, PT = PW / 16;
     const int g = (threadIdx.x & 63) >> 4;
-    const Lanes<T, NP> ln;
-    const Lanes<T, PW> lp;
+    const Lanes<T, NP, kSwapped> ln;
+    const Lanes<T, PW, kDownOnly> lp;
     const float whole = e.from[kQ - 1];
     constexpr int kSome = PT < 2 ? PT : 2;  // tiles of P at a time: the split x of all four would take the registers of the loads in flight
 #pragma unroll
@@ -50,12 +50,12 @@ __device__ __forceinline__ void advance(f32x4 (&S)[R][C], const Tile<T, kQ, PW>&
 #pragma unroll
             for (int pt = 0; pt < kSome; ++pt) {
                 f32x4 u, v;
-                widen(X.down(lp, 32 * k, 16 * (p0 + pt)), u, v);
+                widen(X.down(lp, 32 * k, p0 + pt), u, v);
                 split(u * wa, v * wb, xs[pt]);
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const Frag<T> bt = Bs.down(ln, 32 * k, 16 * nt);
+                const Frag<T> bt = Bs.down(ln, 32 * k, nt);
 #pragma unroll
                 for (int term = Split<T>::kTerms - 1; term >= 0; --term)
 #pragma unroll
@@ -76,7 +76,7 @@ __device__ __forceinline__ void advance(f32x4 (&S)[R][C], const Tile<T, kQ, PW>&
 // Roundings (bf16): the scores times decay and step, and the state as it enters the product with C, once each to bf16 - y is rounded to that anyway; the
 // weighted inputs that build the state are split (ssm.h), so the state that is handed on has fp32's precision.
 template <typename T, int NP, int PW> struct ScanShare {
-    static constexpr int kBytes = 2 * Tile<T, kQ, NP>::kBytes + 4 * (Tile<T, kQ, PW>::kBytes + (int)sizeof(Decays));
+    static constexpr int kBytes = 2 * Tile<T, kQ, NP, kSwapped>::kBytes + 4 * (Tile<T, kQ, PW, kDownOnly>::kBytes + (int)(sizeof(Decays) + sizeof(Factors)));
     // waves per SIMD: two (256 registers each) where a CU's LDS holds as many workgroups, else one
     static constexpr int kWavesPerSimd = kBytes * 2 <= 160 * 1024 ? 2 : 1;
 };
@@ -86,9 +86,10 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
                                                                                           float* __restrict__ last) {
     typedef T T4 __attribute__((ext_vector_type(4)));
     constexpr int NT = NP / 16, PT = PW / 16;
-    __shared__ __attribute__((aligned(16))) Tile<T, kQ, NP> Bs, Cs;
-    __shared__ __attribute__((aligned(16))) Tile<T, kQ, PW> Xs[4];
+    __shared__ __attribute__((aligned(16))) Tile<T, kQ, NP, kSwapped> Bs, Cs;
+    __shared__ __attribute__((aligned(16))) Tile<T, kQ, PW, kDownOnly> Xs[4];
     __shared__ __attribute__((aligned(16))) Decays decays[4];
+    __shared__ __attribute__((aligned(16))) Factors factors[4];
     const int lane = threadIdx.x & 63, w = wave_index(), lc = lane & 15, g = lane >> 4;
     const Place at = scan_place(a, w);
     const int b = at.b, h = at.head, len = row_length(a.lengths, b, a.L), cols = a.P - at.p0;
@@ -97,21 +98,22 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
     const T* Bg = static_cast<const T*>(a.B) + b * a.b_row + (long long)at.grp * a.N;
     const T* Cg = static_cast<const T*>(a.C) + b * a.c_row + (long long)at.grp * a.N;
     const long long state_at = ((long long)b * a.H + h) * a.P + at.p0;
-    Tile<T, kQ, PW>& X = Xs[w];
+    Tile<T, kQ, PW, kDownOnly>& X = Xs[w];
     Decays& e = decays[w];
-    const Lanes<T, NP> ln;
-    const Lanes<T, PW> lp;
+    Factors& f = factors[w];
+    const Lanes<T, NP, kSwapped> ln;
+    const Lanes<T, PW, kDownOnly> lp;
 
     f32x4 S[NT][PT];  // rows n, columns p
-    const float* from = at.seg > 0 ? starts + (((long long)b * a.H + h) * a.segs + at.seg) * (padded(a.P) * NP) + at.p0 * NP : nullptr;
+    const float* start = at.seg > 0 ? starts + (((long long)b * a.H + h) * a.segs + at.seg) * (padded(a.P) * NP) + at.p0 * NP : nullptr;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int pt = 0; pt < PT; ++pt) {
-            const int p = 16 * pt + lc, n = 16 * nt + 4 * g;
+            const int p = 16 * pt + lc, n = swapped(nt, 4 * g);
             S[nt][pt] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (from) {
-                S[nt][pt] = *reinterpret_cast<const f32x4*>(from + p * NP + n);
+            if (start) {
+                S[nt][pt] = *reinterpret_cast<const f32x4*>(start + p * NP + n);
             } else if (a.state && p < cols) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -138,7 +140,8 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
         T* out = y + (((long long)b * a.L + t0) * a.H + h) * a.P + at.p0;
         __syncthreads();  // the chunk before has been read
         lb.put(threadIdx.x, Bs), lcc.put(threadIdx.x, Cs), lx.put(lane, X);
-        put_decays(e, raw, lane < rows, a.dt.softplus, A);
+        const Decay d = put_decays(e, raw, lane < rows, a.dt.softplus, A);
+        put_factors(f, d, d.step);
         __syncthreads();
         if (at.works) {
 #pragma unroll
@@ -169,17 +172,20 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
                             s[1][u] = mma(bj, q[1][k], s[1][u]);
                         }
                         const int j = 16 * ss + 4 * g;
-                        const f32x4 jh = *reinterpret_cast<const f32x4*>(e.hi + j), jl = *reinterpret_cast<const f32x4*>(e.lo + j);
-                        const f32x4 d = *reinterpret_cast<const f32x4*>(e.step + j);
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
                             const int tt = 2 * half + r, t = 16 * tt + lc;
-                            if (ss > tt) continue;
-                            const float th = e.hi[t], tl = e.lo[t];
+                            if (ss < tt) {
+                                s[r][u] *= *reinterpret_cast<const f32x4*>(f.far[tt - 1] + j) * f.near[t];
+                            } else if (ss == tt) {
+                                const f32x4 jh = *reinterpret_cast<const f32x4*>(e.hi + j), jl = *reinterpret_cast<const f32x4*>(e.lo + j);
+                                const f32x4 d = *reinterpret_cast<const f32x4*>(e.step + j);
+                                const float th = e.hi[t], tl = e.lo[t];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                s[r][u][i] *= exp2_fast((th - jh[i]) + (tl - jl[i])) * d[i];
-                                if (ss == tt) s[r][u][i] = j + i < t ? s[r][u][i] : j + i == t ? s[r][u][i] + D : 0.f;
+                                for (int i = 0; i < 4; ++i) {
+                                    const float v = s[r][u][i] * exp2_fast((th - jh[i]) + (tl - jl[i])) * d[i];
+                                    s[r][u][i] = j + i < t ? v : j + i == t ? v + D : 0.f;
+                                }
                             }
                         }
                     }
@@ -206,15 +212,15 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
                         }
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const float f = e.from[16 * (2 * half + r) + lc];
+                        const float from = e.from[16 * (2 * half + r) + lc];
 #pragma unroll
-                        for (int pt = 0; pt < kSome; ++pt) acc[r][pt] *= f;
+                        for (int pt = 0; pt < kSome; ++pt) acc[r][pt] *= from;
                     }
 #pragma unroll
                     for (int kk = 0; kk <= half; ++kk)
 #pragma unroll
                         for (int pt = 0; pt < kSome; ++pt) {
-                            const Frag<T> xj = X.down(lp, 32 * kk, 16 * (p0 + pt));
+                            const Frag<T> xj = X.down(lp, 32 * kk, p0 + pt);
                             acc[0][pt] = mma(xj, m[0][kk], acc[0][pt]);
                             acc[1][pt] = mma(xj, m[1][kk], acc[1][pt]);
                         }
@@ -259,7 +265,7 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int pt = 0; pt < PT; ++pt) {
-                const int p = 16 * pt + lc, n = 16 * nt + 4 * g;
+                const int p = 16 * pt + lc, n = swapped(nt, 4 * g);
                 if (p < cols) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -278,8 +284,8 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
 template <typename T, int NP, int PW>
 __global__ __launch_bounds__(256, 2) void scan_walk_kernel(ScanArgs a0, WalkOut o0, ScanArgs a1, WalkOut o1) {
     constexpr int NT = NP / 16, PT = PW / 16;
-    __shared__ __attribute__((aligned(16))) Tile<T, kQ, NP> Bs;
-    __shared__ __attribute__((aligned(16))) Tile<T, kQ, PW> Xs[4];
+    __shared__ __attribute__((aligned(16))) Tile<T, kQ, NP, kSwapped> Bs;
+    __shared__ __attribute__((aligned(16))) Tile<T, kQ, PW, kDownOnly> Xs[4];
     __shared__ __attribute__((aligned(16))) Decays decays[4];
     ScanArgs a = a0;
     WalkOut o = o0;
@@ -292,7 +298,7 @@ __global__ __launch_bounds__(256, 2) void scan_walk_kernel(ScanArgs a0, WalkOut 
     const T* Bg = static_cast<const T*>(a.B) + b * a.b_row + (long long)at.grp * a.N;
     const long long head = (long long)b * a.H + h, state_at = head * a.P + at.p0;
     const bool chained = o.starts && at.seg > 0;
-    Tile<T, kQ, PW>& X = Xs[w];
+    Tile<T, kQ, PW, kDownOnly>& X = Xs[w];
     Decays& e = decays[w];
 
     f32x4 S[PT][NT];  // rows p, columns n
@@ -300,7 +306,7 @@ __global__ __launch_bounds__(256, 2) void scan_walk_kernel(ScanArgs a0, WalkOut 
     for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int p = 16 * pt + 4 * g, n = 16 * nt + lc;
+            const int p = 16 * pt + 4 * g, n = swapped(nt, lc);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float v = 0.f;
@@ -352,7 +358,7 @@ __global__ __launch_bounds__(256, 2) void scan_walk_kernel(ScanArgs a0, WalkOut 
     for (int pt = 0; pt < PT; ++pt)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int p = 16 * pt + 4 * g, n = 16 * nt + lc;
+            const int p = 16 * pt + 4 * g, n = swapped(nt, lc);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (out) out[(p + i) * NP + n] = S[pt][nt][i];
