@@ -64,8 +64,8 @@ __device__ __forceinline__ Frag<__bf16> take_upper(f32x4& a, f32x4& b) {
     return {__builtin_bit_cast(bf16x8, v)};
 }
 __device__ __forceinline__ void split(f32x4 a, f32x4 b, Split<__bf16>& s) { s.hi = take_upper(a, b), s.mid = take_upper(a, b), s.lo = take_upper(a, b); }
-__device__ __forceinline__ f32x4 mma(const Frag<float>& x, const Split<float>& y, f32x4 c) { return mma(x, y.hi, c); }
-__device__ __forceinline__ f32x4 mma(const Frag<__bf16>& x, const Split<__bf16>& y, f32x4 c) { return mma(x, y.hi, mma(x, y.mid, mma(x, y.lo, c))); }
+__device__ __forceinline__ f32x4 mma(const Split<float>& x, const Frag<float>& y, f32x4 c) { return mma(x.hi, y, c); }
+__device__ __forceinline__ f32x4 mma(const Split<__bf16>& x, const Frag<__bf16>& y, f32x4 c) { return mma(x.hi, y, mma(x.mid, y, mma(x.lo, y, c))); }
 
 __device__ __forceinline__ void widen(const Frag<float>& f, f32x4& a, f32x4& b) { a = f.a, b = f.b; }
 __device__ __forceinline__ void widen(const Frag<__bf16>& f, f32x4& a, f32x4& b) {
@@ -136,12 +136,12 @@ template <int ROWS, int COLS, Kind KIND> struct Tile<float, ROWS, COLS, KIND> {
     }
     __device__ __forceinline__ void put4(int r, int c, f32x4 x) { *reinterpret_cast<f32x4*>(v + r * kPitch + c) = x; }
     __device__ __forceinline__ void put(int r, int c, float x) { v[r * kPitch + c] = x; }
-    __device__ __forceinline__ float get(int r, int c) const { return v[r * kPitch + c]; }
     // lane l: row r + (l & 15), values from c (a multiple of 32) on
     __device__ __forceinline__ Frag<float> row(const Lane& l, int r, int c) const {
         const float* p = v + l.row + r * kPitch + c;
         return {*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + (KIND == kSwapped ? 4 : 16))};
     }
+    __device__ __forceinline__ Frag<float> row_any(const Lane& l, int r, int c) const { return row(l, r, c); }  // c not known to the compiler
     // lane l: place l & 15 of column tile t, rows r + 4 g .. and r + 16 + 4 g ..
     __device__ __forceinline__ Frag<float> down(const Lane& l, int r, int t) const {
         const float* p = v + l.down + r * kPitch + (KIND == kSwapped ? swapped(t, 0) : 16 * t);
@@ -150,7 +150,7 @@ template <int ROWS, int COLS, Kind KIND> struct Tile<float, ROWS, COLS, KIND> {
         for (int j = 0; j < 4; ++j) f.a[j] = p[j * kPitch], f.b[j] = p[(16 + j) * kPitch];
         return f;
     }
-    __device__ __forceinline__ Frag<float> down_any(int r, int t) const { return down(Lane(), r, t); }  // t not known to the compiler
+    __device__ __forceinline__ Frag<float> down_any(int r, int t) const { return down(Lane(), r, t); }
 };
 
 template <int ROWS, int COLS, Kind KIND> struct Tile<__bf16, ROWS, COLS, KIND> {
@@ -177,9 +177,11 @@ template <int ROWS, int COLS, Kind KIND> struct Tile<__bf16, ROWS, COLS, KIND> {
     }
     __device__ __forceinline__ void put4(int r, int c, f32x4 x) { *reinterpret_cast<bf16x4*>(v + at(r, c)) = __builtin_convertvector(x, bf16x4); }
     __device__ __forceinline__ void put(int r, int c, float x) { v[at(r, c)] = (__bf16)x; }
-    __device__ __forceinline__ float get(int r, int c) const { return (float)v[at(r, c)]; }
     __device__ __forceinline__ Frag<__bf16> row(const Lane& l, int r, int c) const {
         return {*reinterpret_cast<const bf16x8*>(v + r * COLS + (c >> 6 << 6) + l.row[c >> 5 & (Lane::kRow - 1)])};
+    }
+    __device__ __forceinline__ Frag<__bf16> row_any(const Lane& l, int r, int c) const {
+        return {*reinterpret_cast<const bf16x8*>(v + r * COLS + (c >> 6 << 6) + (c >> 5 & (Lane::kRow - 1) ? l.row[Lane::kRow - 1] : l.row[0]))};
     }
     __device__ __forceinline__ Frag<__bf16> down(const Lane& l, int r, int t) const {
         if (KIND == kDownOnly) return down_from(v + r * COLS + (t >> 2 << 6) + l.down[t & (Lane::kDown - 1)]);

@@ -33,32 +33,43 @@ struct GradArgs {
 // way into a product.
 constexpr int kRing = 4;  // heads per ring of decays and sums
 
-struct HeadSums {
-    float rowZ[4][kQ], dotU[4][kQ], dotV[4][kQ], colZ[2][kQ], diagZ[kQ], diagV[kQ], crossing[4];
+template <int HALF, int ALT> struct HeadSums {
+    float rowZ[4][kQ], dotU[HALF][kQ], dotV[HALF][kQ], colZ[ALT][kQ], diagZ[kQ], diagV[kQ], crossing[4];
 };
 
-template <typename T, int NP, int PP> struct GradTiles {
+template <typename T, int NP, int PP> struct GradShare {
     static constexpr int kWaves = NP == 128 ? 8 : 4, kThreads = 64 * kWaves, kHalf = kWaves / 2, kAlt = kWaves / 4;
-    static constexpr int kSlices = NP / 16 / kHalf;  // 16-wide slices of N per wave
+    static constexpr int kSlices = NP / 16 / kHalf;  // 16-wide tiles of N per wave, neighbours
+    static constexpr int kOwn = 4 / kAlt;            // row tiles of the scores per wave: tt = o kAlt + alt
     static constexpr int PB = PP < 64 ? PP : 64;
     typedef Tile<T, kQ, NP, kSwapped> Wide;
     typedef Tile<T, kQ, PB, kInOrder> Slim;
     typedef Tile<T, NP, PB, kDownOnly> States;
     typedef Tile<T, kQ, kQ, kInOrder> Scores;
+    typedef HeadSums<kHalf, kAlt> Sums;
     static constexpr int kMain = 2 * Slim::kBytes + States::kBytes, kPool = kMain > Scores::kBytes ? kMain : Scores::kBytes;
-    static constexpr int kBytes = 2 * Wide::kBytes + kPool + kRing * (int)(sizeof(Decays) + sizeof(HeadSums));
+    static constexpr int kBytes = 2 * Wide::kBytes + kPool + kRing * (int)(sizeof(Decays) + sizeof(Factors) + sizeof(Sums));
     static constexpr int kWavesPerSimd = kWaves == 8 || kBytes * 2 <= 160 * 1024 ? 2 : 1;
 };
 
+// values of four token tiles, summed over the four lane groups g: lane l gets the total of token l
+__device__ __forceinline__ float sum_groups(const float (&v)[4]) {
+    const int g = (threadIdx.x & 63) >> 4;
+    const bool upper = g & 2, odd = g & 1;
+    const float a0 = (upper ? v[2] : v[0]) + __shfl_xor(upper ? v[0] : v[2], 32, 64), a1 = (upper ? v[3] : v[1]) + __shfl_xor(upper ? v[1] : v[3], 32, 64);
+    return (odd ? a1 : a0) + __shfl_xor(odd ? a0 : a1, 16, 64);
+}
+
 template <typename T, int NP, int PP>
-__global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP, PP>::kWavesPerSimd)) void scan_grad_kernel(GradArgs q) {
-    typedef GradTiles<T, NP, PP> S;
+__global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP, PP>::kWavesPerSimd)) void scan_grad_kernel(GradArgs q) {
+    typedef GradShare<T, NP, PP> S;
     typedef T T4 __attribute__((ext_vector_type(4)));
-    constexpr int PB = S::PB, NS = S::kSlices;
+    constexpr int PB = S::PB, NS = S::kSlices, kOwn = S::kOwn;
     __shared__ __attribute__((aligned(16))) typename S::Wide Bs, Cs;
     __shared__ __attribute__((aligned(16))) char pool[S::kPool];
     __shared__ __attribute__((aligned(16))) Decays decays[kRing];
-    __shared__ __attribute__((aligned(16))) HeadSums sums[kRing];
+    __shared__ __attribute__((aligned(16))) Factors factors[kRing];
+    __shared__ __attribute__((aligned(16))) typename S::Sums sums[kRing];
     typename S::Slim &Ys = *reinterpret_cast<typename S::Slim*>(pool), &Xs = *reinterpret_cast<typename S::Slim*>(pool + S::Slim::kBytes);
     typename S::States& Gs = *reinterpret_cast<typename S::States*>(pool + 2 * S::Slim::kBytes);  // rows: places of n
     const ScanArgs& a = q.a;
@@ -74,18 +85,17 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
     const int blocks = (a.P + PB - 1) / PB;  // of P that hold anything
     const int jt = w & 3, alt = w >> 2, j = 16 * jt + lc;  // this lane's column of the score tiles
     const bool role_v = w >= S::kHalf;
-    const int first = role_v ? w - S::kHalf : w;
+    const int first = role_v ? w - S::kHalf : w, nt0 = first * NS;  // this wave's tiles of N: nt0 and its NS - 1 neighbours
     const typename S::Slim& Rs = role_v ? Xs : Ys;
-    const typename S::Wide& Ks = role_v ? Bs : Cs;
+    const typename S::Wide &Ks = role_v ? Bs : Cs, &Os = role_v ? Cs : Bs;
     const float *mine = role_v ? q.behind : q.front;
     {
         const T* Bg = static_cast<const T*>(a.B) + b * a.b_row + t0 * a.b_tok + (long long)grp * a.N;
         const T* Cg = static_cast<const T*>(a.C) + b * a.c_row + t0 * a.c_tok + (long long)grp * a.N;
-        Load<T, NP, S::kThreads> load;
-        load.ask(threadIdx.x, Bg, a.b_tok, rows, a.N, a.how_b);
-        load.put(threadIdx.x, Bs);
-        load.ask(threadIdx.x, Cg, a.c_tok, rows, a.N, a.how_c);
-        load.put(threadIdx.x, Cs);
+        Load<T, NP, S::kThreads> lb, lcc;
+        lb.ask(threadIdx.x, Bg, a.b_tok, rows, a.N, a.how_b);
+        lcc.ask(threadIdx.x, Cg, a.c_tok, rows, a.N, a.how_c);
+        lb.put(threadIdx.x, Bs), lcc.put(threadIdx.x, Cs);
     }
     Load<T, PB, 128> ahead;  // x by waves 0 and 1, dy by waves 2 and 3
     auto ask = [&](int h, int p0) {
@@ -101,10 +111,11 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
     const typename S::Wide::Lane ln;
     const typename S::Slim::Lane lp;
     const typename S::States::Lane lg;
-    f32x4 cb[4], dcb[4], sum[4][NS];  // rows t, columns j; rows t, columns n
+    f32x4 cb[4], dcb[kOwn], sum[4][NS];  // rows t, columns j; rows n, columns t
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) {
-        cb[tt] = dcb[tt] = zero;
+        cb[tt] = zero;
+        if (tt < kOwn) dcb[tt] = zero;
         if (tt >= jt)
 #pragma unroll
             for (int k = 0; k < NP / 32; ++k) cb[tt] = mma(Cs.row(ln, 16 * tt, 32 * k), Bs.row(ln, 16 * jt, 32 * k), cb[tt]);
@@ -114,15 +125,27 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
     for (int h = h0; h < h1; ++h) {
         const int ring = (h - h0) % kRing;
         const Decays& e = decays[ring];
-        HeadSums& hs = sums[ring];
+        const Factors& f = factors[ring];
+        typename S::Sums& hs = sums[ring];
         const float D = a.D ? a.D[h] : 0.f;
         const long long at = (((long long)b * a.L + t0) * a.H + h) * a.P, tiles = (((long long)b * a.chunks + c) * a.H + h) * PP * NP;
-        f32x4 dM[4], R[4][NS];
+        // E of row tile tt >= jt in this lane's column
+        auto decay_tile = [&](int tt) {
+            const int t = 16 * tt + 4 * g;
+            if (tt > jt) return *reinterpret_cast<const f32x4*>(f.near + t) * f.far[tt - 1][j];
+            const f32x4 th = *reinterpret_cast<const f32x4*>(e.hi + t), tl = *reinterpret_cast<const f32x4*>(e.lo + t);
+            const float jh = e.hi[j], jl = e.lo[j];
+            f32x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = 4 * g + i >= lc ? exp2_fast((th[i] - jh) + (tl[i] - jl)) : 0.f;
+            return v;
+        };
+        f32x4 dM[kOwn], R[4][NS];
         Frag<T> wgt[2];
         float gh = 0.f;
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
-            dM[tt] = zero;
+            if (tt < kOwn) dM[tt] = zero;
 #pragma unroll
             for (int s = 0; s < NS; ++s) R[tt][s] = zero;
         }
@@ -133,30 +156,31 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
             for (int s = 0; s < NS; ++s)
 #pragma unroll
                 for (int pt = 0; pt < PB / 16; ++pt)  // (the walks leave tiles behind P unwritten)
-                    tile[s][pt] = p0 + 16 * pt < a.P ? *reinterpret_cast<const f32x4*>(mine + tiles + ((p0 / 16 + pt) * (NP / 16) + first + S::kHalf * s) * 256 + lane * 4) : zero;
+                    tile[s][pt] = p0 + 16 * pt < a.P ? *reinterpret_cast<const f32x4*>(mine + tiles + ((p0 / 16 + pt) * (NP / 16) + nt0 + s) * 256 + lane * 4) : zero;
             __syncthreads();  // the block before has been read
-            if (w < 2) ahead.put(threadIdx.x, Xs);
-            else if (w < 4) ahead.put(threadIdx.x - 128, Ys);
+            if (w < 2) ahead.put(threadIdx.x & 127, Xs);
+            else if (w < 4) ahead.put(threadIdx.x & 127, Ys);
             if (pb == 0 && ring == 0) {
-                if (w < kRing && h + w < h1) put_decays(decays[w], raw, lane < rows, a.dt.softplus, a.A[h + w]);
+                if (w < kRing && h + w < h1) put_factors(factors[w], put_decays(decays[w], raw, lane < rows, a.dt.softplus, a.A[h + w]), 1.f);
                 ask_step(h + kRing);
             }
             const bool next = pb + 1 == blocks;  // head
             if (!next || h + 1 < h1) ask(next ? h + 1 : h, next ? 0 : p0 + PB);
             __syncthreads();
             if (pb == 0) {
-                const float jh = e.hi[j], jl = e.lo[j], d = e.step[j];
+                const float d = e.step[j];
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     f32x4 m[2];
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const int t = 16 * (2 * k + r) + 4 * g;
-                        const f32x4 th = *reinterpret_cast<const f32x4*>(e.hi + t), tl = *reinterpret_cast<const f32x4*>(e.lo + t);
+                        const int tt = 2 * k + r;
+                        m[r] = zero;
+                        if (tt >= jt) {
+                            m[r] = cb[tt] * decay_tile(tt) * d;
+                            if (tt == jt)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            m[r][i] = t + i >= j ? cb[2 * k + r][i] * exp2_fast((th[i] - jh) + (tl[i] - jl)) * d : 0.f;
-                            if (t + i == j) m[r][i] += D;
+                                for (int i = 0; i < 4; ++i) m[r][i] += 4 * g + i == lc ? D : 0.f;
                         }
                     }
                     wgt[k] = frag_of<T>(m[0], m[1]);
@@ -166,20 +190,19 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
             for (int k = 0; k < PB / 32; ++k) {
                 const Frag<T> xj = Xs.row(lp, 16 * jt, 32 * k);
 #pragma unroll
-                for (int tt = 0; tt < 4; ++tt)
-                    if (tt >= jt && tt % S::kAlt == alt) dM[tt] = mma(Ys.row(lp, 16 * tt, 32 * k), xj, dM[tt]);
-                __builtin_amdgcn_sched_barrier(0);
+                for (int o = 0; o < kOwn; ++o)
+                    if (o * S::kAlt + alt >= jt) dM[o] = mma(Ys.row(lp, 16 * (o * S::kAlt + alt), 32 * k), xj, dM[o]);
             }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
                 if (role_v) {
 #pragma unroll
                     for (int pt = 0; pt < PB / 16; ++pt) {
-                        const int nt = first + S::kHalf * s;
-                        const f32x4 other = p0 + 16 * pt < a.P ? *reinterpret_cast<const f32x4*>(q.front + tiles + ((p0 / 16 + pt) * (NP / 16) + nt) * 256 + lane * 4) : zero;
+                        const f32x4 other = p0 + 16 * pt < a.P ? *reinterpret_cast<const f32x4*>(q.front + tiles + ((p0 / 16 + pt) * (NP / 16) + nt0 + s) * 256 + lane * 4) : zero;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) gh = fmaf(other[i], tile[s][pt][i], gh);
-                        Gs.put4(16 * nt + lc, 16 * pt + 4 * g, tile[s][pt]);
+                        Gs.put4(16 * (nt0 + s) + lc, 16 * pt + 4 * g, tile[s][pt]);
                     }
                 }
 #pragma unroll
@@ -187,33 +210,36 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
                     Split<T> op;
                     split(tile[s][2 * k], tile[s][2 * k + 1], op);
 #pragma unroll
-                    for (int tt = 0; tt < 4; ++tt)
-                        R[tt][s] = mma(Rs.row(lp, 16 * tt, 32 * k), op, R[tt][s]);
+                    for (int tt = 0; tt < 4; ++tt) R[tt][s] = mma(op, Rs.row(lp, 16 * tt, 32 * k), R[tt][s]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
             if (next) {
                 // per-token sums: over j (16 lanes, and the waves) for the rows, over t (this wave's registers) for the columns
                 float col = 0.f, diag = 0.f, dv = 0.f;
-                const float jh = e.hi[j], jl = e.lo[j], dj = e.step[j];
+                const float dj = e.step[j];
 #pragma unroll
-                for (int tt = 0; tt < 4; ++tt) {
-                    if (tt % S::kAlt != alt) continue;
-                    const int t = 16 * tt + 4 * g;
+                for (int o = 0; o < kOwn; ++o) {
+                    const int tt = o * S::kAlt + alt;
                     f32x4 r = zero;
                     if (tt >= jt) {
-                        const f32x4 th = *reinterpret_cast<const f32x4*>(e.hi + t), tl = *reinterpret_cast<const f32x4*>(e.lo + t);
+                        const f32x4 m = dM[o] * decay_tile(tt), z = m * (S::kAlt == 1 ? cb[o] : alt ? cb[(2 * o + 1) & 3] : cb[2 * o & 3]);
+                        dcb[o] += m * dj;
+                        r = z * dj;
+                        if (tt > jt) {
+                            col += (z[0] + z[1]) + (z[2] + z[3]);
+                        } else {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float m = t + i >= j ? dM[tt][i] * exp2_fast((th[i] - jh) + (tl[i] - jl)) : 0.f, z = m * cb[tt][i];
-                            dcb[tt][i] = fmaf(m, dj, dcb[tt][i]);
-                            if (t + i == j) diag = z, dv = dM[tt][i];
-                            else col += z;
-                            r[i] = row16_sum(t + i == j ? 0.f : z * dj);
+                            for (int i = 0; i < 4; ++i) {
+                                const bool on = 4 * g + i == lc;
+                                col += on ? 0.f : z[i], diag += on ? z[i] : 0.f, dv += on ? dM[o][i] : 0.f;
+                                r[i] = on ? 0.f : r[i];
+                            }
                         }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) r[i] = row16_sum(r[i]);
                     }
-                    if (lc == 0) *reinterpret_cast<f32x4*>(hs.rowZ[jt] + t) = r;
+                    if (lc == 0) *reinterpret_cast<f32x4*>(hs.rowZ[jt] + 16 * tt + 4 * g) = r;
                 }
                 col += __shfl_xor(col, 16, 64), diag += __shfl_xor(diag, 16, 64), dv += __shfl_xor(dv, 16, 64);
                 col += __shfl_xor(col, 32, 64), diag += __shfl_xor(diag, 32, 64), dv += __shfl_xor(dv, 32, 64);
@@ -221,22 +247,22 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
                     hs.colZ[alt][j] = col;
                     if (jt % S::kAlt == alt) hs.diagZ[j] = diag, hs.diagV[j] = dv;
                 }
+                float dots[4];
 #pragma unroll
                 for (int tt = 0; tt < 4; ++tt) {
-                    const int t = 16 * tt + 4 * g;
-                    f32x4 f = *reinterpret_cast<const f32x4*>((role_v ? e.to : e.from) + t), r = zero;
-                    if (role_v) f *= *reinterpret_cast<const f32x4*>(e.step + t);
+                    const int t = 16 * tt + lc;
+                    const float by = role_v ? e.to[t] * e.step[t] : e.from[t];
+                    f32x4 k0, k1, v = zero;
+                    widen(Ks.row_any(ln, 16 * tt, 16 * nt0 & ~31), k0, k1);
+                    if (NS == 1) k0 = nt0 & 1 ? k1 : k0;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                        for (int s = 0; s < NS; ++s) {
-                            r[i] = fmaf(Ks.get(t + i, swapped(first + S::kHalf * s, lc)), R[tt][s][i], r[i]);
-                            sum[tt][s][i] = fmaf(f[i], R[tt][s][i], sum[tt][s][i]);
-                        }
-                        r[i] = row16_sum(r[i]);
+                    for (int s = 0; s < NS; ++s) {
+                        v += (s == 0 ? k0 : k1) * R[tt][s];
+                        sum[tt][s] += R[tt][s] * by;
                     }
-                    if (lc == 0) *reinterpret_cast<f32x4*>((role_v ? hs.dotV : hs.dotU)[first] + t) = r;
+                    dots[tt] = (v[0] + v[1]) + (v[2] + v[3]);
                 }
+                (role_v ? hs.dotV : hs.dotU)[first][lane] = sum_groups(dots);
                 if (role_v) {
                     gh = wave_sum(gh);
                     if (lane == 0) hs.crossing[first] = gh;
@@ -246,17 +272,16 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
             const float end = e.to[j] * e.step[j];
             T* dx = static_cast<T*>(q.dx) + at + (long long)j * a.H * a.P + p0;
 #pragma unroll
-            for (int pt = 0; pt < PB / 16; ++pt) {
-                __builtin_amdgcn_sched_barrier(0);
-                if (pt % S::kAlt != alt) continue;
+            for (int i = 0; i < PB / 16 / S::kAlt; ++i) {
+                const int pt = S::kAlt == 1 ? i : 2 * i;  // of two neighbours this wave's is known when it runs
                 f32x4 acc = zero;  // rows p, columns j
 #pragma unroll
-                for (int k = 0; k < NP / 32; ++k) acc = mma(Gs.down(lg, 32 * k, pt), Bs.row(ln, 16 * jt, 32 * k), acc);
+                for (int k = 0; k < NP / 32; ++k) acc = mma(alt ? Gs.down(lg, 32 * k, pt + S::kAlt - 1) : Gs.down(lg, 32 * k, pt), Bs.row(ln, 16 * jt, 32 * k), acc);
                 acc *= end;
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
-                    if (2 * k + 1 >= jt) acc = mma(Ys.down(lp, 32 * k, pt), wgt[k], acc);
-                const int p = 16 * pt + 4 * g;
+                    if (2 * k + 1 >= jt) acc = mma(alt ? Ys.down(lp, 32 * k, pt + S::kAlt - 1) : Ys.down(lp, 32 * k, pt), wgt[k], acc);
+                const int p = 16 * (pt + alt) + 4 * g;
                 if (j < all && p0 + p < a.P) {
                     T4 v;
 #pragma unroll
@@ -269,18 +294,21 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
                             if (p0 + p + i < a.P) dx[p + i] = v[i];
                     }
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         if ((ring == kRing - 1 || h + 1 == h1) && w <= ring) {  // a wave per head of the ring, one token per lane
             const int hw = h - ring + w;
             const Decays& d = decays[w];
-            const HeadSums& s = sums[w];
-            const float step = d.step[lane], A = a.A[hw], v_all = S::kHalf == 4 ? s.dotV[2][lane] + s.dotV[3][lane] : 0.f;
-            const float u_all = S::kHalf == 4 ? s.dotU[2][lane] + s.dotU[3][lane] : 0.f, g_all = S::kHalf == 4 ? s.crossing[2] + s.crossing[3] : 0.f;
-            const float r = s.rowZ[0][lane] + s.rowZ[1][lane] + s.rowZ[2][lane] + s.rowZ[3][lane];
-            const float u = d.from[lane] * (s.dotU[0][lane] + s.dotU[1][lane] + u_all), v = d.to[lane] * (s.dotV[0][lane] + s.dotV[1][lane] + v_all);
-            const float col = S::kAlt == 2 ? s.colZ[0][lane] + s.colZ[1][lane] : s.colZ[0][lane];
-            const float cross = d.from[kQ - 1] * (s.crossing[0] + s.crossing[1] + g_all);
+            const typename S::Sums& s = sums[w];
+            const float step = d.step[lane], A = a.A[hw];
+            float u = 0.f, v = 0.f, cross = 0.f, col = 0.f;
+#pragma unroll
+            for (int i = 0; i < S::kHalf; ++i) u += s.dotU[i][lane], v += s.dotV[i][lane], cross += s.crossing[i];
+#pragma unroll
+            for (int i = 0; i < S::kAlt; ++i) col += s.colZ[i][lane];
+            u *= d.from[lane], v *= d.to[lane], cross *= d.from[kQ - 1];
+            const float r = (s.rowZ[0][lane] + s.rowZ[1][lane]) + (s.rowZ[2][lane] + s.rowZ[3][lane]);
             const double in = running_sum((double)(step * v)), out = running_sum((double)u + ((double)r - (double)step * col));
             const double total = __shfl(out, 63, 64), before = __shfl_up(out, 1, 64), in_before = __shfl_up(in, 1, 64);
             const float over = (float)((double)cross + (lane ? in_before : 0.0) + (total - (lane ? before : 0.0)));
@@ -303,34 +331,42 @@ __global__ __launch_bounds__((GradTiles<T, NP, PP>::kThreads), (GradTiles<T, NP,
     typename S::Scores& Ms = *reinterpret_cast<typename S::Scores*>(pool);
     __syncthreads();
 #pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
-        if (tt % S::kAlt == alt)
+    for (int o = 0; o < kOwn; ++o)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) Ms.put(16 * tt + 4 * g + i, j, dcb[tt][i]);
+        for (int i = 0; i < 4; ++i) Ms.put(16 * (o * S::kAlt + alt) + 4 * g + i, j, dcb[o][i]);
     __syncthreads();
     T* grad = static_cast<T*>(role_v ? q.dB : q.dC);
     float* wide = role_v ? q.pB : q.pC;
-    const typename S::Wide& Os = role_v ? Cs : Bs;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-        const int n = swapped(first + S::kHalf * s, lc);
+        const int n = swapped(nt0 + s, 4 * g);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const Frag<T> o = Os.down_any(32 * k, first + S::kHalf * s);
+            const Frag<T> o = Os.down_any(32 * k, nt0 + s);
 #pragma unroll
-            for (int tt = 0; tt < 4; ++tt) sum[tt][s] = mma(role_v ? Ms.down(lq, 32 * k, tt) : Ms.row(lq, 16 * tt, 32 * k), o, sum[tt][s]);
+            for (int tt = 0; tt < 4; ++tt) sum[tt][s] = mma(o, role_v ? Ms.down(lq, 32 * k, tt) : Ms.row(lq, 16 * tt, 32 * k), sum[tt][s]);
         }
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt)
+        for (int tt = 0; tt < 4; ++tt) {
+            const int t = 16 * tt + lc;
+            if (t >= all || n >= a.N) continue;
+            const long long o = (((long long)b * a.L + t0 + t) * a.G + grp) * a.N + n;
+            const long long ow = (long long)part * a.rows * a.L * a.G * a.N + o;
+            T4 v;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = 16 * tt + 4 * g + i;
-                if (t < all && n < a.N) {
-                    const long long o = (((long long)b * a.L + t0 + t) * a.G + grp) * a.N + n;
-                    if (q.parts > 1) wide[(long long)part * a.rows * a.L * a.G * a.N + o] = sum[tt][s][i];
-                    else grad[o] = (T)sum[tt][s][i];
-                }
+            for (int i = 0; i < 4; ++i) v[i] = (T)sum[tt][s][i];
+            if (a.N % 4 == 0) {
+                if (q.parts > 1) *reinterpret_cast<f32x4*>(wide + ow) = sum[tt][s];
+                else *reinterpret_cast<T4*>(grad + o) = v;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (n + i < a.N) {
+                        if (q.parts > 1) wide[ow + i] = sum[tt][s][i];
+                        else grad[o + i] = v[i];
+                    }
             }
+        }
     }
 }
 
@@ -377,7 +413,7 @@ template <typename T, int NP, int PP>
 static int launch_grad(const GradArgs& q, hipStream_t st) {
     const long long blocks = (long long)q.a.rows * q.a.chunks * q.a.G * q.parts;
     if (blocks > 0x7fffffffll) return RTFS_EINVAL;
-    hipLaunchKernelGGL((scan_grad_kernel<T, NP, PP>), dim3((unsigned)blocks), dim3(GradTiles<T, NP, PP>::kThreads), 0, st, q);
+    hipLaunchKernelGGL((scan_grad_kernel<T, NP, PP>), dim3((unsigned)blocks), dim3(GradShare<T, NP, PP>::kThreads), 0, st, q);
     RTFS_LAUNCH_CHECK();
     if (q.parts > 1) {
         const long long n = (long long)q.a.rows * q.a.L * q.a.G * q.a.N, wg = (n + 255) / 256;
