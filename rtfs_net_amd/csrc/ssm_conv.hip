@@ -3,28 +3,35 @@
 // with the K - 1 inputs before token 0 taken from `state` [B][K-1][D] (zeros without one), a length per row of a padded batch, and the K - 1 inputs before
 // each row's end returned as the state that the next call or the single-token form takes.
 // Bound: HBM.  A thread owns V neighbouring channels (16 bytes where alignment allows) and walks a run of tokens with the window in registers, so every
-// input is loaded once per run plus K - 1 of the run before it.  All arithmetic is fp32; x, y, state and their gradients are rounded once, on the way out.
+// input is loaded once per run plus K - 1 of the run before it; four tokens are asked for at a time.  All arithmetic is fp32; x, y, state and their gradients are rounded once, on the way out.
 #include "common.h"
 
 namespace rtfs {
 
 typedef __bf16 bhalf8 __attribute__((ext_vector_type(8)));
 
-template <typename T, int V> struct ConvVec { float v[V]; };
+// V values as they are loaded (16 bytes, or one)
+template <typename T, int V> struct ConvRaw;
+template <> struct ConvRaw<float, 1> { float v; };
+template <> struct ConvRaw<__bf16, 1> { __bf16 v; };
+template <> struct ConvRaw<float, 4> { float4 v; };
+template <> struct ConvRaw<__bf16, 8> { bhalf8 v; };
 
 template <typename T, int V>
-__device__ __forceinline__ void conv_load(const T* p, float (&v)[V]) {
+__device__ __forceinline__ ConvRaw<T, V> conv_raw(const T* p) { return *reinterpret_cast<const ConvRaw<T, V>*>(p); }
+template <typename T, int V>
+__device__ __forceinline__ void conv_widen(const ConvRaw<T, V>& a, float (&v)[V]) {
     if constexpr (V == 1) {
-        v[0] = (float)*p;
+        v[0] = (float)a.v;
     } else if constexpr (sizeof(T) == 4) {
-        const float4 a = *reinterpret_cast<const float4*>(p);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+        v[0] = a.v.x, v[1] = a.v.y, v[2] = a.v.z, v[3] = a.v.w;
     } else {
-        const bhalf8 a = *reinterpret_cast<const bhalf8*>(p);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (float)a[e];
+        for (int e = 0; e < 8; ++e) v[e] = (float)a.v[e];
     }
 }
+template <typename T, int V>
+__device__ __forceinline__ void conv_load(const T* p, float (&v)[V]) { conv_widen<T, V>(conv_raw<T, V>(p), v); }
 template <typename T, int V>
 __device__ __forceinline__ void conv_store(T* p, const float (&v)[V]) {
     if constexpr (V == 1) {
@@ -77,6 +84,8 @@ __device__ __forceinline__ void conv_weights(const ConvArgs& a, int d, float (&w
     }
 }
 
+constexpr int kConvAhead = 4;  // tokens asked for at a time
+
 template <typename T, int K, int V>
 __global__ __launch_bounds__(256) void causal_conv_kernel(ConvArgs a, T* __restrict__ y, T* __restrict__ last) {
     const int tile = blockIdx.x % a.tiles, across = 1 << a.tile_log2;
@@ -93,25 +102,29 @@ __global__ __launch_bounds__(256) void causal_conv_kernel(ConvArgs a, T* __restr
         else conv_zero(win[k + 1]);
     }
     T* out = y + ((long long)b * a.L + t0) * a.D + d;
-#pragma unroll 4
-    for (int t = t0; t < t1; ++t, out += a.D) {
-        float o[V];
-        conv_zero(o);
-        if (t < len) {
+    const T* in = static_cast<const T*>(a.x) + b * a.x_row + d;
+    const int end = len > 0 ? len - 1 : 0;  // loads go no further: a token behind the row's end counts as zero whatever is read in its place
+    for (int tb = t0; tb < t1; tb += kConvAhead) {
+        ConvRaw<T, V> raw[kConvAhead];
+#pragma unroll
+        for (int i = 0; i < kConvAhead; ++i) raw[i] = conv_raw<T, V>(in + (long long)(tb + i < end ? tb + i : end) * a.x_tok);
+#pragma unroll
+        for (int i = 0; i < kConvAhead; ++i, out += a.D) {
+            float o[V];
 #pragma unroll
             for (int k = 0; k < K - 1; ++k)
 #pragma unroll
                 for (int e = 0; e < V; ++e) win[k][e] = win[k + 1][e];
-            conv_load<T, V>(static_cast<const T*>(a.x) + b * a.x_row + t * a.x_tok + d, win[K - 1]);
+            conv_widen<T, V>(raw[i], win[K - 1]);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 float s = bias[e];
 #pragma unroll
                 for (int k = 0; k < K; ++k) s = fmaf(w[k][e], win[k][e], s);
-                o[e] = a.silu ? s * sigmoidf_fast(s) : s;
+                o[e] = tb + i >= len ? 0.f : a.silu ? s * sigmoidf_fast(s) : s;
             }
+            if (tb + i < t1) conv_store<T, V>(out, o);
         }
-        conv_store<T, V>(out, o);
     }
     if (last && t0 == 0) {
 #pragma unroll
@@ -150,33 +163,42 @@ __global__ __launch_bounds__(256) void causal_conv_bwd_kernel(ConvArgs a, const 
             if (t0 - (K - 1) + k < len) conv_input<T, K, V>(a, b, t0 - (K - 1) + k, d, win[k + 1]);
             else conv_zero(win[k + 1]);
         }
-#pragma unroll 2
-        for (int t = t0; t < t1 + K - 1; ++t) {
+        const T* in = static_cast<const T*>(a.x) + b * a.x_row + d;
+        const T* din = dy + (long long)b * a.L * a.D + d;
+        const int end = len > 0 ? len - 1 : 0;
+        for (int tb = t0; tb < t1 + K - 1; tb += kConvAhead) {
+          ConvRaw<T, V> rx[kConvAhead], rg[kConvAhead];
+#pragma unroll
+          for (int i = 0; i < kConvAhead; ++i) {
+            const int t = tb + i < end ? tb + i : end;
+            rx[i] = conv_raw<T, V>(in + (long long)t * a.x_tok);
+            rg[i] = conv_raw<T, V>(din + (long long)t * a.D);
+          }
+#pragma unroll
+          for (int i = 0; i < kConvAhead; ++i) {
+            const int t = tb + i;
+            if (t >= t1 + K - 1) break;
 #pragma unroll
             for (int k = 0; k < K - 1; ++k)
 #pragma unroll
                 for (int e = 0; e < V; ++e) win[k][e] = win[k + 1][e], g[k][e] = g[k + 1][e];
-            conv_zero(g[K - 1]);
-            if (t < len) {
-                conv_load<T, V>(static_cast<const T*>(a.x) + b * a.x_row + t * a.x_tok + d, win[K - 1]);
-                conv_load<T, V>(dy + ((long long)b * a.L + t) * a.D + d, g[K - 1]);
+            conv_widen<T, V>(rx[i], win[K - 1]);
+            conv_widen<T, V>(rg[i], g[K - 1]);
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    if (a.silu) {
-                        float s = bias[e];
+            for (int e = 0; e < V; ++e) {
+                if (a.silu) {
+                    float s = bias[e];
 #pragma unroll
-                        for (int k = 0; k < K; ++k) s = fmaf(w[k][e], win[k][e], s);
-                        const float q = sigmoidf_fast(s);
-                        g[K - 1][e] *= q * fmaf(s, 1.f - q, 1.f);
-                    }
-                    if (t < t1) {
-#pragma unroll
-                        for (int k = 0; k < K; ++k) dw[k][e] = fmaf(g[K - 1][e], win[k][e], dw[k][e]);
-                        dw[K][e] += g[K - 1][e];
-                    }
+                    for (int k = 0; k < K; ++k) s = fmaf(w[k][e], win[k][e], s);
+                    const float q = sigmoidf_fast(s);
+                    g[K - 1][e] *= q * fmaf(s, 1.f - q, 1.f);
                 }
-            } else {
-                conv_zero(win[K - 1]);
+                g[K - 1][e] = t < len ? g[K - 1][e] : 0.f;
+                if (t < t1 && t < len) {
+#pragma unroll
+                    for (int k = 0; k < K; ++k) dw[k][e] = fmaf(g[K - 1][e], win[k][e], dw[k][e]);
+                    dw[K][e] += g[K - 1][e];
+                }
             }
             const int u = t - (K - 1);  // g[j] is dpre[u + j]
             if (u >= t0 || (t0 == 0 && dstate)) {
@@ -197,6 +219,7 @@ __global__ __launch_bounds__(256) void causal_conv_bwd_kernel(ConvArgs a, const 
                 if (u >= 0) conv_store<T, V>(dx + ((long long)b * a.L + u) * a.D + d, o);
                 else conv_store<T, V>(dstate + ((long long)b * (K - 1) + u + K - 1) * a.D + d, o);
             }
+          }
         }
     }
 #pragma unroll
@@ -216,20 +239,22 @@ __global__ __launch_bounds__(256) void causal_conv_bwd_kernel(ConvArgs a, const 
     }
 }
 
-// parts [groups][K+1][D] -> dw [D][K], dbias [D]; 64 neighbouring outputs per workgroup, a quarter of the partials per wave
+// parts [groups][K+1][D] -> dw [D][K], dbias [D]; 16 neighbouring outputs per workgroup, a sixteenth of the partials per group of 16 lanes
 __global__ __launch_bounds__(256) void conv_finish_kernel(const float* __restrict__ parts, int groups, int D, int K, float* __restrict__ dw,
                                                           float* __restrict__ dbias) {
     __shared__ float red[256];
-    const int i = blockIdx.x * 64 + (threadIdx.x & 63), n = (K + 1) * D;
+    const int i = blockIdx.x * 16 + (threadIdx.x & 15), n = (K + 1) * D;
     float s = 0.f;
     if (i < n) {
-#pragma unroll 8
-        for (int g = threadIdx.x >> 6; g < groups; g += 4) s += parts[(long long)g * n + i];
+#pragma unroll 16
+        for (int g = threadIdx.x >> 4; g < groups; g += 16) s += parts[(long long)g * n + i];
     }
     red[threadIdx.x] = s;
     __syncthreads();
-    if (threadIdx.x < 64 && i < n) {
-        s = red[threadIdx.x] + red[threadIdx.x + 64] + red[threadIdx.x + 128] + red[threadIdx.x + 192];
+    if (threadIdx.x < 16 && i < n) {
+        s = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s += red[threadIdx.x + 16 * r];
         const int k = i / D, d = i % D;
         if (k < K) dw[(long long)d * K + k] = s;
         else if (dbias) dbias[d] = s;
@@ -307,7 +332,7 @@ static int conv_bwd(ConvArgs a, const void* dy, const void* dlast, void* dx, voi
     hipLaunchKernelGGL((causal_conv_bwd_kernel<T, K, V>), dim3(groups * a.tiles), dim3(256), 0, st, a, static_cast<const T*>(dy), static_cast<const T*>(dlast),
                        static_cast<T*>(dx), static_cast<T*>(dstate), parts);
     RTFS_LAUNCH_CHECK();
-    hipLaunchKernelGGL(conv_finish_kernel, dim3(((K + 1) * a.D + 63) / 64), dim3(256), 0, st, parts, groups, a.D, K, dw, dbias);
+    hipLaunchKernelGGL(conv_finish_kernel, dim3(((K + 1) * a.D + 15) / 16), dim3(256), 0, st, parts, groups, a.D, K, dw, dbias);
     RTFS_LAUNCH_CHECK();
     return RTFS_OK;
 }

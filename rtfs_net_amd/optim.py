@@ -149,35 +149,28 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0):
         raise ValueError(f"clip_grad_norm_: norm_type 2 or inf, got {norm_type}")
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    grads, device, seen = [], None, set()
-    at, sizes, types = array.array("q"), array.array("q"), array.array("i")
-    for p in parameters:
-        g = p.grad
-        if g is None or id(g) in seen:
-            continue
-        kind = _CLIP_TYPES.get(g.dtype)
-        if kind is None or g.layout != torch.strided or not g.is_cuda:
-            raise ValueError(f"clip_grad_norm_: gradients must be dense fp32, bf16 or fp16 HIP tensors, got {g.dtype}, {g.layout}, {g.device}")
-        if device is None:
-            device = g.device
-        elif g.device != device:
-            raise ValueError(f"clip_grad_norm_: gradients on {device} and {g.device}")
-        if not g.is_contiguous() and not _fills_its_span(g):
-            raise ValueError("clip_grad_norm_: a gradient has gaps or overlaps in memory")
-        seen.add(id(g))
-        grads.append(g)
-        if g.numel():
-            at.append(g.data_ptr())
-            sizes.append(g.numel())
-            types.append(kind)
-    if device is None:
+    grads = [g for g in [p.grad for p in parameters] if g is not None]
+    if not grads:
         return torch.zeros(())
-    if not at:
+    if len(set(map(id, grads))) != len(grads):
+        grads = list({id(g): g for g in grads}.values())
+    # one pass per question over all tensors: a small model's hundreds of them are host time, not device time
+    kinds = [_CLIP_TYPES.get(g.dtype, -1) for g in grads]
+    devices = set(map(torch.Tensor.get_device, grads))
+    if -1 in kinds or -1 in devices or {g.layout for g in grads} != {torch.strided}:
+        raise ValueError("clip_grad_norm_: gradients must be dense fp32, bf16 or fp16 HIP tensors")
+    if len(devices) > 1:
+        raise ValueError(f"clip_grad_norm_: gradients on devices {sorted(devices)}")
+    if not all(g.is_contiguous() or _fills_its_span(g) for g in grads):
+        raise ValueError("clip_grad_norm_: a gradient has gaps or overlaps in memory")
+    device = grads[0].device
+    sizes = array.array("q", map(torch.Tensor.numel, grads))
+    if not any(sizes):
         return torch.zeros((), device=device)
+    at, types = array.array("q", map(torch.Tensor.data_ptr, grads)), array.array("i", kinds)
     norm = torch.empty((), device=device)
-    n = len(at) + sum(s >> 30 for s in sizes)  # a tensor of over 2^30 elements is listed in pieces
-    parts = torch.empty(2048 + n, dtype=torch.float64, device=device)
-    lib.call("rtfs_clip_grad_norm", at.buffer_info()[0], sizes.buffer_info()[0], types.buffer_info()[0], len(at), max_norm, 2 if norm_type == 2.0 else 0, parts,
+    parts = torch.empty(2048 + len(grads) + (sum(sizes) >> 30), dtype=torch.float64, device=device)  # a tensor of over 2^30 elements is listed in pieces
+    lib.call("rtfs_clip_grad_norm", at.buffer_info()[0], sizes.buffer_info()[0], types.buffer_info()[0], len(grads), max_norm, 2 if norm_type == 2.0 else 0, parts,
              parts.numel(), norm)
     torch.autograd.graph.increment_version(grads)  # written through their addresses
     return norm

@@ -32,7 +32,7 @@ def _raw(t):
 def _check(name, what, t, shape, dtypes, device):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: {what} must be a tensor, got {type(t).__name__}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name}: {what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.dtype not in dtypes:
         raise ValueError(f"{name}: {what} must be {' or '.join(str(d)[6:] for d in dtypes)}, got {str(t.dtype)[6:]}")
@@ -78,7 +78,7 @@ def _lengths(name, lengths, B, device):
 
 
 def _dense(t):
-    return None if t is None else t.detach().contiguous()
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 # ---- convolution ---------------------------------------------------------------------------------------------------------------------------------------
@@ -89,7 +89,7 @@ class _CausalConv(torch.autograd.Function):
     def forward(ctx, x, weight, bias, state, lengths, silu, want_state):
         B, L, D = x.shape
         K = weight.shape[1]
-        x, row, tok = _tokens(x.detach(), 1)
+        x, row, tok = _tokens(x, 1)
         weight, bias, state = _dense(weight), _dense(bias), _dense(state)
         y = torch.empty(B, L, D, dtype=x.dtype, device=x.device)
         last = torch.empty(B, K - 1, D, dtype=x.dtype, device=x.device) if want_state else None
@@ -177,7 +177,6 @@ class _SelectiveScan(torch.autograd.Function):
     def forward(ctx, x, dt, A, Bm, C, D, dt_bias, state, lengths, softplus, want_state):
         B, L, H, P = x.shape
         G, N = Bm.shape[2:]
-        x, dt, Bm, C = x.detach(), dt.detach(), Bm.detach(), C.detach()
         A, D, dt_bias, state = _dense(A), _dense(D), _dense(dt_bias), _dense(state)
         (x, xr, xt), (dt, tr, tt), (Bm, br, bt), (C, cr, ct) = _tokens(x, 2), _tokens(dt, 1), _tokens(Bm, 2), _tokens(C, 2)
         y = torch.empty(B, L, H, P, dtype=x.dtype, device=x.device)
