@@ -555,7 +555,7 @@ int rtfs_causal_conv_bwd(const void* x, long long x_row, long long x_tok, const 
 /* one token per row: x [B][D] (x_row), state [B][K-1][D] moves on in place */
 int rtfs_causal_conv_step(const void* x, long long x_row, void* state, const float* w, const float* bias, void* y, int B, int D, int K, int silu, int type,
                           void* stream);
-int rtfs_ssm_scan_segments(int B, int L, int H, int P, int G, int N);
+int rtfs_ssm_scan_segments(int B, int L, int H, int P, int G, int N, int directions /* forward 1, backward 2 */);
 int rtfs_ssm_tile(int P, int N);
 int rtfs_ssm_scan_fwd(const void* x, long long x_row, long long x_tok, const void* dt, long long dt_row, long long dt_tok, int dt_type, const float* A,
                       const void* Bm, long long b_row, long long b_tok, const void* C, long long c_row, long long c_tok, const float* D, const float* dt_bias,

@@ -415,20 +415,20 @@ inline bool scan_sizes(int B, int L, int H, int P, int G, int N) {
 // 64 tokens must lie within 2^31 bytes of each other: buffer offsets
 inline bool scan_pitch(long long tok) { return tok >= 0 && tok < (1ll << 23); }
 
-void scan_cut(ScanArgs& a);
+void scan_cut(ScanArgs& a, int directions);
 int scan_starts(const ScanArgs& a0, const ScanArgs& a1, const float* state1, float* ws, int both, int type, hipStream_t st);
 int scan_walks(const ScanArgs& a0, const WalkOut& o0, const ScanArgs& a1, const WalkOut& o1, int both, int type, hipStream_t st);
 
 inline ScanArgs scan_args(const void* x, long long x_row, long long x_tok, const Steps& dt, const float* A, const void* B, long long b_row, long long b_tok,
                           const void* C, long long c_row, long long c_tok, const float* D, const float* state, const int* lengths, int rows, int L, int H, int P,
-                          int G, int N, int type) {
+                          int G, int N, int type, int directions) {
     ScanArgs a{x, B, C, x_row, x_tok, b_row, b_tok, c_row, c_tok, dt, A, D, state, lengths, rows, L, H, P, G, N, 1, 0, 0, 0, 0, 0, 0, 0, 0};
     const int v = type == 0 ? 4 : 8;  // values in 16 bytes
     auto how = [&](const void* p, int width, long long row, long long tok) {
         return width % v == 0 && row % v == 0 && tok % v == 0 && on16(p) ? kAligned : width >= v ? kAnywhere : kShort;
     };
     a.how_x = how(x, P, x_row, x_tok), a.how_b = how(B, N, b_row, b_tok), a.how_c = how(C, N, c_row, c_tok);
-    scan_cut(a);
+    scan_cut(a, directions);
     return a;
 }
 

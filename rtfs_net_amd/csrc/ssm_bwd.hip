@@ -452,10 +452,10 @@ int rtfs_ssm_scan_bwd(const void* x, long long x_row, long long x_tok, const voi
     hipStream_t st = (hipStream_t)stream;
     const Steps steps{dt, dt_row, dt_tok, dt_type, dt_bias, softplus};
     GradArgs q{};
-    q.a = scan_args(x, x_row, x_tok, steps, A, Bm, b_row, b_tok, C, c_row, c_tok, D, state, lengths, B, L, H, P, G, N, type);
+    q.a = scan_args(x, x_row, x_tok, steps, A, Bm, b_row, b_tok, C, c_row, c_tok, D, state, lengths, B, L, H, P, G, N, type, 2);
     const long long d_tok = (long long)H * P;
     // the walk back: dy in the place of x, C in the place of B, the last state's gradient in the place of the state
-    const ScanArgs back = scan_args(dy, d_tok * L, d_tok, steps, A, C, c_row, c_tok, C, c_row, c_tok, D, dlast, lengths, B, L, H, P, G, N, type);
+    const ScanArgs back = scan_args(dy, d_tok * L, d_tok, steps, A, C, c_row, c_tok, C, c_row, c_tok, D, dlast, lengths, B, L, H, P, G, N, type, 2);
     grad_parts(q.a, q.parts, q.part_heads);
     if ((q.a.segs > 1 && !starts) || (q.parts > 1 && !parts)) return RTFS_EINVAL;
     const long long n = (long long)B * H * q.a.segs, tile = (long long)padded(P) * padded(N);

@@ -464,17 +464,20 @@ int scan_walks(const ScanArgs& a0, const WalkOut& o0, const ScanArgs& a1, const 
 
 // A wave takes 64, 32 or 16 columns of P: the widest that leaves a group's heads four waves of work (the scores of a head are formed by each of its waves), and
 // whose state of N values each fits a wave's registers next to the loads in flight (64 columns of 128 spilled).
-// Rows are cut into segments, each walked by workgroups of its own, as far as it takes to give every CU two workgroups, and into no more than 256: a segment's own
-// state is walked first then (B, x and dt read twice, the state's products done twice) and the segments' states are chained (about 0.1 us each).  Seven rows of
-// eight chunks (6 heads of 48, fp32): 94 us uncut, 75 us in segments of four chunks, 35 us in segments of one.
-void scan_cut(ScanArgs& a) {
+// Rows are cut into segments, each walked by workgroups of its own, and into no more than 256: a segment's own state is walked first then (B, x and dt read twice,
+// the state's products done twice) and the segments' states are chained (about 0.1 us each).  A prompt is cut until every CU has two workgroups (seven rows of
+// eight chunks, 6 heads of 48, fp32: 94 us uncut, 75 us in segments of four chunks, 35 us in segments of one).  The gradients' walks, both directions in one
+// launch, are cut until every CU has one: they write a tile per chunk and are bound by that, not by the products (8 rows of 2048 tokens, 32 heads of 64, N = 128:
+// 172 us uncut at one workgroup per CU; at two 167 us and 118 us more for the first walk and the chain).
+void scan_cut(ScanArgs& a, int directions) {
     const int each = a.H / a.G;
     for (a.width = a.P <= 16 ? 16 : a.P <= 32 || a.N > 64 ? 32 : 64; a.width > 16 && each * ((a.P + a.width - 1) / a.width) < 4; a.width /= 2) {}
     a.slices = (a.P + a.width - 1) / a.width;
     a.quads = (each * a.slices + 3) / 4;
     a.chunks = (a.L + kQ - 1) / kQ;
-    const long long groups = (long long)a.rows * a.G * a.quads;
-    const long long want = groups >= 512 ? 1 : (512 + groups - 1) / groups;
+    const long long groups = (long long)a.rows * a.G * a.quads * directions;
+    const long long target = directions == 2 ? 256 : 512;
+    const long long want = groups >= target ? 1 : (target + groups - 1) / groups;
     const long long per = (a.chunks + want - 1) / want;
     a.seg_chunks = (int)(want == 1 ? a.chunks : per < (a.chunks + 255) / 256 ? (a.chunks + 255) / 256 : per);
     a.segs = (a.chunks + a.seg_chunks - 1) / a.seg_chunks;
@@ -513,11 +516,11 @@ using namespace rtfs::ssm;
 
 extern "C" {
 
-int rtfs_ssm_scan_segments(int B, int L, int H, int P, int G, int N) {
-    if (!scan_sizes(B, L, H, P, G, N)) return RTFS_EINVAL;
+int rtfs_ssm_scan_segments(int B, int L, int H, int P, int G, int N, int directions) {
+    if (!scan_sizes(B, L, H, P, G, N) || directions < 1 || directions > 2) return RTFS_EINVAL;
     ScanArgs a{};
     a.rows = B, a.L = L, a.H = H, a.P = P, a.G = G, a.N = N;
-    scan_cut(a);
+    scan_cut(a, directions);
     return a.segs;
 }
 
@@ -531,7 +534,7 @@ int rtfs_ssm_scan_fwd(const void* x, long long x_row, long long x_tok, const voi
         !scan_pitch(x_tok) || !scan_pitch(b_tok) || !scan_pitch(c_tok))
         return RTFS_EINVAL;
     ScanArgs a = scan_args(x, x_row, x_tok, Steps{dt, dt_row, dt_tok, dt_type, dt_bias, softplus}, A, Bm, b_row, b_tok, C, c_row, c_tok, D, state, lengths, B, L, H,
-                           P, G, N, type);
+                           P, G, N, type, 1);
     hipStream_t st = (hipStream_t)stream;
     if (a.segs > 1) {
         if (!work) return RTFS_EINVAL;

@@ -166,7 +166,7 @@ SIGNATURES = {
     "rtfs_causal_conv_bwd_work_floats": [I, I, I],
     "rtfs_causal_conv_bwd": [P, LL, LL] + [P] * 11 + [I] * 6 + [P],
     "rtfs_causal_conv_step": [P, LL, P, P, P, P, I, I, I, I, I, P],
-    "rtfs_ssm_scan_segments": [I, I, I, I, I, I],
+    "rtfs_ssm_scan_segments": [I] * 7,
     "rtfs_ssm_tile": [I, I],
     "rtfs_ssm_scan_fwd": [P, LL, LL, P, LL, LL, I, P, P, LL, LL, P, LL, LL, P, P, I, P, P, P, P, P] + [I] * 7 + [P],
     "rtfs_ssm_scan_bwd_parts": [I, I, I, I],

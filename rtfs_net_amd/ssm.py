@@ -182,7 +182,7 @@ class _SelectiveScan(torch.autograd.Function):
         y = torch.empty(B, L, H, P, dtype=x.dtype, device=x.device)
         last = torch.empty(B, H, P, N, device=x.device) if want_state else None
         handle = lib.load()
-        segs = handle.rtfs_ssm_scan_segments(B, L, H, P, G, N)
+        segs = handle.rtfs_ssm_scan_segments(B, L, H, P, G, N, 1)
         work = torch.empty(B * H * segs * (handle.rtfs_ssm_tile(P, N) + 1), device=x.device) if segs > 1 else None
         lib.call("rtfs_ssm_scan_fwd", _raw(x), xr, xt, _raw(dt), tr, tt, _TYPES[dt.dtype], A, _raw(Bm), br, bt, _raw(C), cr, ct, D, dt_bias, int(softplus), state,
                  lengths, y, last, work, B, L, H, P, G, N, _TYPES[x.dtype])
@@ -208,7 +208,7 @@ class _SelectiveScan(torch.autograd.Function):
         dA, dD, db = new(H), new(H) if D is not None else None, new(H) if dt_bias is not None else None
         ds = torch.empty_like(state) if state is not None else None
         handle = lib.load()
-        segs, tile, parts, chunks = handle.rtfs_ssm_scan_segments(B, L, H, P, G, N), handle.rtfs_ssm_tile(P, N), handle.rtfs_ssm_scan_bwd_parts(B, L, H, G), -(-L // 64)
+        segs, tile, parts, chunks = handle.rtfs_ssm_scan_segments(B, L, H, P, G, N, 2), handle.rtfs_ssm_tile(P, N), handle.rtfs_ssm_scan_bwd_parts(B, L, H, G), -(-L // 64)
         starts = new(2 * B * H * segs * (tile + 1)) if segs > 1 else None
         wide = new(2 * parts * B * L * G * N) if parts > 1 else None
         lib.call("rtfs_ssm_scan_bwd", _raw(x), xr, xt, _raw(dt), tr, tt, _TYPES[dt.dtype], A, _raw(Bm), br, bt, _raw(C), cr, ct, D, dt_bias, int(ctx.softplus), state,
