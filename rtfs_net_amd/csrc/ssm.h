@@ -310,19 +310,35 @@ struct Steps {
 // a lane's value in all lanes
 __device__ __forceinline__ float lane_value(float v, int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); }
 
+__device__ __forceinline__ double lane_value(double v, int lane) {
+    const long long bits = __builtin_bit_cast(long long, v);
+    const int lo = __builtin_amdgcn_readlane((int)bits, lane), hi = __builtin_amdgcn_readlane((int)(bits >> 32), lane);
+    return __builtin_bit_cast(double, (long long)(unsigned)lo | (long long)hi << 32);
+}
+
 template <int CTRL, int ROWS>
 __device__ __forceinline__ double dpp_add(double v) {
     const long long bits = __builtin_bit_cast(long long, v);
     const int lo = __builtin_amdgcn_update_dpp(0, (int)bits, CTRL, ROWS, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, (int)(bits >> 32), CTRL, ROWS, 0xf, false);
     return v + __builtin_bit_cast(double, (long long)(unsigned)lo | (long long)hi << 32);
 }
-// Sums over the tokens up to and including this lane's, in fp64: the differences s[t] - s[j] are what counts, and behind a strong decay both are large.
-// Shifts inside the rows of 16 lanes, then the rows' last lanes handed on; lanes a step does not reach add 0.
-__device__ __forceinline__ double running_sum(double v) {
+// sums over the lanes of this lane's row of 16: up to and including it, or from it on
+__device__ __forceinline__ double row_sum_to(double v) {
     v = dpp_add<0x111, 0xf>(v);  // row_shr:1
     v = dpp_add<0x112, 0xf>(v);  // row_shr:2
     v = dpp_add<0x114, 0xf>(v);  // row_shr:4
-    v = dpp_add<0x118, 0xf>(v);  // row_shr:8
+    return dpp_add<0x118, 0xf>(v);  // row_shr:8
+}
+__device__ __forceinline__ double row_sum_from(double v) {
+    v = dpp_add<0x101, 0xf>(v);  // row_shl:1
+    v = dpp_add<0x102, 0xf>(v);  // row_shl:2
+    v = dpp_add<0x104, 0xf>(v);  // row_shl:4
+    return dpp_add<0x108, 0xf>(v);  // row_shl:8
+}
+// Sums over the tokens up to and including this lane's, in fp64: the differences s[t] - s[j] are what counts, and behind a strong decay both are large.
+// Shifts inside the rows of 16 lanes, then the rows' last lanes handed on; lanes a step does not reach add 0.
+__device__ __forceinline__ double running_sum(double v) {
+    v = row_sum_to(v);
     v = dpp_add<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
     return dpp_add<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
 }
@@ -349,14 +365,16 @@ __device__ __forceinline__ Decay put_decays(Decays& o, float raw, bool alive, bo
     e.step = !alive ? 0.f : plus ? softplus(raw) : raw;
     chunk_decay(e.step, A, e.hi, e.lo);
     const float eh = lane_value(e.hi, 63), el = lane_value(e.lo, 63);
-    o.hi[lane] = e.hi, o.lo[lane] = e.lo, o.step[lane] = e.step, o.from[lane] = exp2_fast(e.hi), o.to[lane] = exp2_fast((eh - e.hi) + (el - e.lo));
+    o.hi[lane] = e.hi, o.lo[lane] = e.lo, o.step[lane] = e.step, o.to[lane] = exp2_fast((eh - e.hi) + (el - e.lo));
+    o.from[lane] = exp2_fast(e.hi) * fmaf(e.lo, 0.693147181f, 1.f);  // every token behind this one has the error of this
     return e;
 }
 
 // e^{s[t]-s[j]} of tokens in different tiles of 16 as a product of two factors, with the last token r in front of t's tile between them: both are at most 1 where
-// states decay.  near[t] = e^{s[t]-s[r]}; far[k][j] = e^{s[r]-s[j]} weight[j] for the tile k + 1 of t, j <= r.
+// states decay.  near[t] = e^{s[t]-s[r]}; to(tile of t)[j] = e^{s[r]-s[j]} weight[j], j <= r.
 struct Factors {
-    float near[kQ], far[3][kQ];
+    float near[kQ], far[16 + 32 + 48];  // far of the tiles 1, 2, 3 one behind the other
+    __device__ __forceinline__ const float* to(int tile) const { return far + (tile == 1 ? 0 : tile == 2 ? 16 : 48); }
 };
 __device__ __forceinline__ void put_factors(Factors& o, const Decay& e, float weight) {
     const int lane = threadIdx.x & 63;
@@ -364,7 +382,7 @@ __device__ __forceinline__ void put_factors(Factors& o, const Decay& e, float we
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
         const float rh = lane_value(e.hi, 16 * k + 15), rl = lane_value(e.lo, 16 * k + 15);
-        o.far[k][lane] = lane <= 16 * k + 15 ? exp2_fast((rh - e.hi) + (rl - e.lo)) * weight : 0.f;
+        if (lane <= 16 * k + 15) o.far[(k == 0 ? 0 : k == 1 ? 16 : 48) + lane] = exp2_fast((rh - e.hi) + (rl - e.lo)) * weight;
         if (lane >> 4 == k + 1) nh = rh, nl = rl;
     }
     o.near[lane] = exp2_fast((e.hi - nh) + (e.lo - nl));
@@ -408,8 +426,9 @@ struct WalkOut {
 __host__ __device__ constexpr int padded(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : 128; }
 inline bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// B H < 2^22: no launch, the step's with four workgroups per head included, reaches 2^32 threads
 inline bool scan_sizes(int B, int L, int H, int P, int G, int N) {
-    return B > 0 && L > 0 && L <= (1 << 30) && H > 0 && P > 0 && P <= 128 && G > 0 && H % G == 0 && N > 0 && N <= 128 && (long long)B * H <= (1 << 24);
+    return B > 0 && L > 0 && L <= (1 << 30) && H > 0 && P > 0 && P <= 128 && G > 0 && H % G == 0 && N > 0 && N <= 128 && (long long)B * H < (1 << 22);
 }
 
 // 64 tokens must lie within 2^31 bytes of each other: buffer offsets

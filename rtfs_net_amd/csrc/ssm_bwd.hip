@@ -34,7 +34,8 @@ struct GradArgs {
 constexpr int kRing = 4;  // heads per ring of decays and sums
 
 template <int HALF, int ALT> struct HeadSums {
-    float rowZ[4][kQ], dotU[HALF][kQ], dotV[HALF][kQ], colZ[ALT][kQ], diagZ[kQ], diagV[kQ], crossing[4];
+    float rowZ[4][kQ], lowZ[ALT][kQ], inZ[kQ], diagZ[kQ];  // rows per column tile; columns below their own row tile, within it, on its diagonal
+    float dotU[HALF][kQ], dotV[HALF][kQ], diagV[kQ], crossing[4];
 };
 
 template <typename T, int NP, int PP> struct GradShare {
@@ -132,7 +133,7 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
         // E of row tile tt >= jt in this lane's column
         auto decay_tile = [&](int tt) {
             const int t = 16 * tt + 4 * g;
-            if (tt > jt) return *reinterpret_cast<const f32x4*>(f.near + t) * f.far[tt - 1][j];
+            if (tt > jt) return *reinterpret_cast<const f32x4*>(f.near + t) * f.to(tt)[j];
             const f32x4 th = *reinterpret_cast<const f32x4*>(e.hi + t), tl = *reinterpret_cast<const f32x4*>(e.lo + t);
             const float jh = e.hi[j], jl = e.lo[j];
             f32x4 v;
@@ -142,7 +143,7 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
         };
         f32x4 dM[kOwn], R[4][NS];
         Frag<T> wgt[2];
-        float gh = 0.f;
+        f32x4 gh = zero;  // four sums: an error of <G, H> is all the chunk's tokens'
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
             if (tt < kOwn) dM[tt] = zero;
@@ -200,8 +201,7 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
 #pragma unroll
                     for (int pt = 0; pt < PB / 16; ++pt) {
                         const f32x4 other = p0 + 16 * pt < a.P ? *reinterpret_cast<const f32x4*>(q.front + tiles + ((p0 / 16 + pt) * (NP / 16) + nt0 + s) * 256 + lane * 4) : zero;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) gh = fmaf(other[i], tile[s][pt][i], gh);
+                        gh += other * tile[s][pt];
                         Gs.put4(16 * (nt0 + s) + lc, 16 * pt + 4 * g, tile[s][pt]);
                     }
                 }
@@ -216,7 +216,7 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
             }
             if (next) {
                 // per-token sums: over j (16 lanes, and the waves) for the rows, over t (this wave's registers) for the columns
-                float col = 0.f, diag = 0.f, dv = 0.f;
+                float low = 0.f, in = 0.f, diag = 0.f, dv = 0.f;
                 const float dj = e.step[j];
 #pragma unroll
                 for (int o = 0; o < kOwn; ++o) {
@@ -227,12 +227,12 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
                         dcb[o] += m * dj;
                         r = z * dj;
                         if (tt > jt) {
-                            col += (z[0] + z[1]) + (z[2] + z[3]);
+                            low += (z[0] + z[1]) + (z[2] + z[3]);
                         } else {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const bool on = 4 * g + i == lc;
-                                col += on ? 0.f : z[i], diag += on ? z[i] : 0.f, dv += on ? dM[o][i] : 0.f;
+                                in += on ? 0.f : z[i], diag += on ? z[i] : 0.f, dv += on ? dM[o][i] : 0.f;
                                 r[i] = on ? 0.f : r[i];
                             }
                         }
@@ -241,11 +241,11 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
                     }
                     if (lc == 0) *reinterpret_cast<f32x4*>(hs.rowZ[jt] + 16 * tt + 4 * g) = r;
                 }
-                col += __shfl_xor(col, 16, 64), diag += __shfl_xor(diag, 16, 64), dv += __shfl_xor(dv, 16, 64);
-                col += __shfl_xor(col, 32, 64), diag += __shfl_xor(diag, 32, 64), dv += __shfl_xor(dv, 32, 64);
+                low += __shfl_xor(low, 16, 64), in += __shfl_xor(in, 16, 64), diag += __shfl_xor(diag, 16, 64), dv += __shfl_xor(dv, 16, 64);
+                low += __shfl_xor(low, 32, 64), in += __shfl_xor(in, 32, 64), diag += __shfl_xor(diag, 32, 64), dv += __shfl_xor(dv, 32, 64);
                 if (g == 0) {
-                    hs.colZ[alt][j] = col;
-                    if (jt % S::kAlt == alt) hs.diagZ[j] = diag, hs.diagV[j] = dv;
+                    hs.lowZ[alt][j] = low;
+                    if (jt % S::kAlt == alt) hs.inZ[j] = in, hs.diagZ[j] = diag, hs.diagV[j] = dv;
                 }
                 float dots[4];
 #pragma unroll
@@ -264,8 +264,8 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
                 }
                 (role_v ? hs.dotV : hs.dotU)[first][lane] = sum_groups(dots);
                 if (role_v) {
-                    gh = wave_sum(gh);
-                    if (lane == 0) hs.crossing[first] = gh;
+                    const float v = wave_sum((gh[0] + gh[1]) + (gh[2] + gh[3]));
+                    if (lane == 0) hs.crossing[first] = v;
                 }
             }
             __syncthreads();
@@ -302,16 +302,23 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
             const Decays& d = decays[w];
             const typename S::Sums& s = sums[w];
             const float step = d.step[lane], A = a.A[hw];
-            float u = 0.f, v = 0.f, cross = 0.f, col = 0.f;
+            float u = 0.f, v = 0.f, cross = 0.f, low = 0.f;
 #pragma unroll
             for (int i = 0; i < S::kHalf; ++i) u += s.dotU[i][lane], v += s.dotV[i][lane], cross += s.crossing[i];
 #pragma unroll
-            for (int i = 0; i < S::kAlt; ++i) col += s.colZ[i][lane];
+            for (int i = 0; i < S::kAlt; ++i) low += s.lowZ[i][lane];
             u *= d.from[lane], v *= d.to[lane], cross *= d.from[kQ - 1];
-            const float r = (s.rowZ[0][lane] + s.rowZ[1][lane]) + (s.rowZ[2][lane] + s.rowZ[3][lane]);
-            const double in = running_sum((double)(step * v)), out = running_sum((double)u + ((double)r - (double)step * col));
-            const double total = __shfl(out, 63, 64), before = __shfl_up(out, 1, 64), in_before = __shfl_up(in, 1, 64);
-            const float over = (float)((double)cross + (lane ? in_before : 0.0) + (total - (lane ? before : 0.0)));
+            // What crosses token t: sums over tokens in front of it (v) and from it on (u), and sum_{j < t <= t'} Z[t'][j] d[j].  The latter as the rows from t on less
+            // the columns from t on would be a small difference of sums whose roundings add up over the chunk, so that only holds within t's own tile; the
+            // tiles further away are added, rows of tiles in front of it or columns in front of t.
+            const int tile = lane >> 4;
+            const float z0 = s.rowZ[0][lane], z1 = s.rowZ[1][lane], z2 = s.rowZ[2][lane], z3 = s.rowZ[3][lane], in = s.inZ[lane];
+            const float own = tile == 0 ? z0 : tile == 1 ? z1 : tile == 2 ? z2 : z3, left = tile == 0 ? 0.f : tile == 1 ? z0 : tile == 2 ? z0 + z1 : z0 + z1 + z2;
+            const float past1 = wave_sum(tile > 1 ? z0 : 0.f), past2 = wave_sum(tile > 2 ? z0 + z1 : 0.f);  // rows behind tiles 1 and 2 of columns in front of them
+            const double near = row_sum_from((double)left + ((double)own - (double)step * in)), below = (double)step * low;
+            const double us = running_sum((double)u), vs = running_sum((double)step * v);
+            const double over64 = (double)cross + (vs - (double)step * v) + (lane_value(us, 63) - (us - (double)u)) + near + (row_sum_to(below) - below);
+            const float over = (float)(over64 + (double)(tile == 1 ? past1 : tile == 2 ? past2 : 0.f)), col = in + low;
             float dstep = lane < rows ? fmaf(A, over, col + s.diagZ[lane] + v) : 0.f;
             if (a.dt.softplus) dstep *= -expm1f(-step);  // softplus'(v) = 1 - e^{-softplus(v)}
             if (lane < all) {
@@ -412,7 +419,7 @@ static void grad_parts(const ScanArgs& a, int& parts, int& heads) {
 template <typename T, int NP, int PP>
 static int launch_grad(const GradArgs& q, hipStream_t st) {
     const long long blocks = (long long)q.a.rows * q.a.chunks * q.a.G * q.parts;
-    if (blocks > 0x7fffffffll) return RTFS_EINVAL;
+    if (blocks * GradShare<T, NP, PP>::kThreads > 0xffffffffll) return RTFS_EINVAL;  // threads of a launch
     hipLaunchKernelGGL((scan_grad_kernel<T, NP, PP>), dim3((unsigned)blocks), dim3(GradShare<T, NP, PP>::kThreads), 0, st, q);
     RTFS_LAUNCH_CHECK();
     if (q.parts > 1) {

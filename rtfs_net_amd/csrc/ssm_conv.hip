@@ -3,7 +3,8 @@
 // with the K - 1 inputs before token 0 taken from `state` [B][K-1][D] (zeros without one), a length per row of a padded batch, and the K - 1 inputs before
 // each row's end returned as the state that the next call or the single-token form takes.
 // Bound: HBM.  A thread owns V neighbouring channels (16 bytes where alignment allows) and walks a run of tokens with the window in registers, so every
-// input is loaded once per run plus K - 1 of the run before it; four tokens are asked for at a time.  All arithmetic is fp32; x, y, state and their gradients are rounded once, on the way out.
+// input is loaded once per run plus K - 1 of the run before it; four tokens are asked for at a time.  All arithmetic is fp32; x, y, state and their gradients
+// are rounded once, on the way out.
 #include "common.h"
 
 namespace rtfs {
@@ -167,59 +168,59 @@ __global__ __launch_bounds__(256) void causal_conv_bwd_kernel(ConvArgs a, const 
         const T* din = dy + (long long)b * a.L * a.D + d;
         const int end = len > 0 ? len - 1 : 0;
         for (int tb = t0; tb < t1 + K - 1; tb += kConvAhead) {
-          ConvRaw<T, V> rx[kConvAhead], rg[kConvAhead];
+            ConvRaw<T, V> rx[kConvAhead], rg[kConvAhead];
 #pragma unroll
-          for (int i = 0; i < kConvAhead; ++i) {
-            const int t = tb + i < end ? tb + i : end;
-            rx[i] = conv_raw<T, V>(in + (long long)t * a.x_tok);
-            rg[i] = conv_raw<T, V>(din + (long long)t * a.D);
-          }
-#pragma unroll
-          for (int i = 0; i < kConvAhead; ++i) {
-            const int t = tb + i;
-            if (t >= t1 + K - 1) break;
-#pragma unroll
-            for (int k = 0; k < K - 1; ++k)
-#pragma unroll
-                for (int e = 0; e < V; ++e) win[k][e] = win[k + 1][e], g[k][e] = g[k + 1][e];
-            conv_widen<T, V>(rx[i], win[K - 1]);
-            conv_widen<T, V>(rg[i], g[K - 1]);
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                if (a.silu) {
-                    float s = bias[e];
-#pragma unroll
-                    for (int k = 0; k < K; ++k) s = fmaf(w[k][e], win[k][e], s);
-                    const float q = sigmoidf_fast(s);
-                    g[K - 1][e] *= q * fmaf(s, 1.f - q, 1.f);
-                }
-                g[K - 1][e] = t < len ? g[K - 1][e] : 0.f;
-                if (t < t1 && t < len) {
-#pragma unroll
-                    for (int k = 0; k < K; ++k) dw[k][e] = fmaf(g[K - 1][e], win[k][e], dw[k][e]);
-                    dw[K][e] += g[K - 1][e];
-                }
+            for (int i = 0; i < kConvAhead; ++i) {
+                const int t = tb + i < end ? tb + i : end;
+                rx[i] = conv_raw<T, V>(in + (long long)t * a.x_tok);
+                rg[i] = conv_raw<T, V>(din + (long long)t * a.D);
             }
-            const int u = t - (K - 1);  // g[j] is dpre[u + j]
-            if (u >= t0 || (t0 == 0 && dstate)) {
-                float o[V];
+#pragma unroll
+            for (int i = 0; i < kConvAhead; ++i) {
+                const int t = tb + i;
+                if (t >= t1 + K - 1) break;
+#pragma unroll
+                for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) win[k][e] = win[k + 1][e], g[k][e] = g[k + 1][e];
+                conv_widen<T, V>(rx[i], win[K - 1]);
+                conv_widen<T, V>(rg[i], g[K - 1]);
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    o[e] = 0.f;
+                    if (a.silu) {
+                        float s = bias[e];
 #pragma unroll
-                    for (int k = 0; k < K; ++k) o[e] = fmaf(w[k][e], g[K - 1 - k][e], o[e]);
-                }
-                const int j = u + K - 1 - len;  // which of the returned state's inputs this one is
-                if (dlast && j >= 0 && u < len) {
-                    float v[V];
-                    conv_load<T, V>(dlast + ((long long)b * (K - 1) + j) * a.D + d, v);
+                        for (int k = 0; k < K; ++k) s = fmaf(w[k][e], win[k][e], s);
+                        const float q = sigmoidf_fast(s);
+                        g[K - 1][e] *= q * fmaf(s, 1.f - q, 1.f);
+                    }
+                    g[K - 1][e] = t < len ? g[K - 1][e] : 0.f;
+                    if (t < t1 && t < len) {
 #pragma unroll
-                    for (int e = 0; e < V; ++e) o[e] += v[e];
+                        for (int k = 0; k < K; ++k) dw[k][e] = fmaf(g[K - 1][e], win[k][e], dw[k][e]);
+                        dw[K][e] += g[K - 1][e];
+                    }
                 }
-                if (u >= 0) conv_store<T, V>(dx + ((long long)b * a.L + u) * a.D + d, o);
-                else conv_store<T, V>(dstate + ((long long)b * (K - 1) + u + K - 1) * a.D + d, o);
+                const int u = t - (K - 1);  // g[j] is dpre[u + j]
+                if (u >= t0 || (t0 == 0 && dstate)) {
+                    float o[V];
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        o[e] = 0.f;
+#pragma unroll
+                        for (int k = 0; k < K; ++k) o[e] = fmaf(w[k][e], g[K - 1 - k][e], o[e]);
+                    }
+                    const int j = u + K - 1 - len;  // which of the returned state's inputs this one is
+                    if (dlast && j >= 0 && u < len) {
+                        float v[V];
+                        conv_load<T, V>(dlast + ((long long)b * (K - 1) + j) * a.D + d, v);
+#pragma unroll
+                        for (int e = 0; e < V; ++e) o[e] += v[e];
+                    }
+                    if (u >= 0) conv_store<T, V>(dx + ((long long)b * a.L + u) * a.D + d, o);
+                    else conv_store<T, V>(dstate + ((long long)b * (K - 1) + u + K - 1) * a.D + d, o);
+                }
             }
-          }
         }
     }
 #pragma unroll
@@ -317,7 +318,7 @@ static int conv_fwd(ConvArgs a, void* y, void* last, hipStream_t st) {
     conv_tiles(a, vecs);
     conv_runs(a, vecs, 32);
     const long long rows = 256 >> a.tile_log2, blocks = ((long long)a.B * a.runs + rows - 1) / rows * a.tiles;
-    if (blocks > 0x7fffffffll) return RTFS_EINVAL;
+    if (blocks * 256 > 0xffffffffll) return RTFS_EINVAL;  // threads of a launch
     hipLaunchKernelGGL((causal_conv_kernel<T, K, V>), dim3((unsigned)blocks), dim3(256), 0, st, a, static_cast<T*>(y), static_cast<T*>(last));
     RTFS_LAUNCH_CHECK();
     return RTFS_OK;
@@ -339,7 +340,7 @@ static int conv_bwd(ConvArgs a, const void* dy, const void* dlast, void* dx, voi
 template <typename T, int K, int V>
 static int conv_step(ConvArgs a, const void* x, void* state, void* y, hipStream_t st) {
     const long long blocks = ((long long)a.B * (a.D / V) + 255) / 256;
-    if (blocks > 0x7fffffffll) return RTFS_EINVAL;
+    if (blocks * 256 > 0xffffffffll) return RTFS_EINVAL;  // threads of a launch
     hipLaunchKernelGGL((causal_conv_step_kernel<T, K, V>), dim3((unsigned)blocks), dim3(256), 0, st, static_cast<const T*>(x), a.x_row, static_cast<T*>(state), a,
                        static_cast<T*>(y));
     RTFS_LAUNCH_CHECK();

@@ -176,7 +176,7 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
                         for (int r = 0; r < 2; ++r) {
                             const int tt = 2 * half + r, t = 16 * tt + lc;
                             if (ss < tt) {
-                                s[r][u] *= *reinterpret_cast<const f32x4*>(f.far[tt - 1] + j) * f.near[t];
+                                s[r][u] *= *reinterpret_cast<const f32x4*>(f.to(tt) + j) * f.near[t];
                             } else if (ss == tt) {
                                 const f32x4 jh = *reinterpret_cast<const f32x4*>(e.hi + j), jl = *reinterpret_cast<const f32x4*>(e.lo + j);
                                 const f32x4 d = *reinterpret_cast<const f32x4*>(e.step + j);
@@ -501,7 +501,6 @@ static int launch_step(const void* x, long long x_row, const Steps& dt, const fl
                        const float* D, float* state, void* y, int rows, int H, int P, int G, int N, hipStream_t st) {
     const int blocks_p = (P + 31) / 32;
     const long long blocks = (long long)rows * H * blocks_p;
-    if (blocks > 0x7fffffffll) return RTFS_EINVAL;
     hipLaunchKernelGGL((scan_step_kernel<T, J>), dim3((unsigned)blocks), dim3(256), 0, st, static_cast<const T*>(x), x_row, dt, A, static_cast<const T*>(B), b_row,
                        static_cast<const T*>(C), c_row, D, state, static_cast<T*>(y), H, P, G, N, blocks_p);
     RTFS_LAUNCH_CHECK();
@@ -552,9 +551,15 @@ int rtfs_ssm_step(const void* x, long long x_row, const void* dt, long long dt_r
         return RTFS_EINVAL;
     const Steps s{dt, dt_row, 0, dt_type, dt_bias, softplus};
     hipStream_t st = (hipStream_t)stream;
-#define RTFS_SSM_STEP(T)                                                                                               do {                                                                                                                   if (N <= 32) return launch_step<T, 1>(x, x_row, s, A, Bm, b_row, C, c_row, D, state, y, B, H, P, G, N, st);         if (N <= 64) return launch_step<T, 2>(x, x_row, s, A, Bm, b_row, C, c_row, D, state, y, B, H, P, G, N, st);         return launch_step<T, 4>(x, x_row, s, A, Bm, b_row, C, c_row, D, state, y, B, H, P, G, N, st);                  } while (0)
-    if (type == 0) RTFS_SSM_STEP(float);
-    else RTFS_SSM_STEP(__bf16);
+#define RTFS_SSM_STEP(T, J) return launch_step<T, J>(x, x_row, s, A, Bm, b_row, C, c_row, D, state, y, B, H, P, G, N, st)
+    if (type == 0) {
+        if (N <= 32) RTFS_SSM_STEP(float, 1);
+        if (N <= 64) RTFS_SSM_STEP(float, 2);
+        RTFS_SSM_STEP(float, 4);
+    }
+    if (N <= 32) RTFS_SSM_STEP(__bf16, 1);
+    if (N <= 64) RTFS_SSM_STEP(__bf16, 2);
+    RTFS_SSM_STEP(__bf16, 4);
 #undef RTFS_SSM_STEP
 }
 

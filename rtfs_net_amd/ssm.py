@@ -120,6 +120,8 @@ class _CausalConv(torch.autograd.Function):
 def _conv_parameters(name, x, weight, bias, D):
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not 1 <= weight.shape[1] <= 8:
         raise ValueError(f"{name}: weight must be a [D, K] tensor with 1 <= K <= 8")
+    if D > 1 << 24:
+        raise ValueError(f"{name}: more than {1 << 24} channels")
     _check(name, "weight", weight, (D, weight.shape[1]), (torch.float32,), x.device)
     if bias is not None:
         _check(name, "bias", bias, (D,), (torch.float32,), x.device)
@@ -235,8 +237,10 @@ def _scan_parameters(name, x, dt, A, B, C, D, dt_bias, state, lead):
             _check(name, what, t, (H,), (torch.float32,), x.device)
     if state is not None:
         _check(name, "state", state, (lead[0], H, P, N), (torch.float32,), x.device)
-    if lead[0] * H > 1 << 24:
-        raise ValueError(f"{name}: more than {1 << 24} rows times heads")
+    if lead[0] * H >= 1 << 22:
+        raise ValueError(f"{name}: {1 << 22} rows times heads, or more")
+    if max(H * P, G * N) >= 1 << 23:
+        raise ValueError(f"{name}: a token of {1 << 23} values, or more")
     return G, N
 
 
@@ -245,7 +249,7 @@ def selective_scan(x, dt, A, B, C, D=None, *, dt_bias=None, softplus=False, stat
     y[t] = S[t] C[t] + D x[t].
 
     x [B, L, H, P], B and C [B, L, G, N], fp32 or bf16 (head h uses group h // (H // G)); dt [B, L, H] of x's type or fp32; A, D, dt_bias [H] fp32, the rates in A
-    negative for a state that decays; state [B, H, P, N] fp32 in front of token 0 (None: zeros); lengths int32 [B].  P, N <= 128.
+    negative for a state that decays; state [B, H, P, N] fp32 in front of token 0 (None: zeros); lengths int32 [B].  P, N <= 128, B H < 2^22, H P < 2^23.
     -> y [B, L, H, P], or (y, last) with `return_state`: last [B, H, P, N], the state behind each row's end.  Differentiable in every tensor but lengths."""
     _first("selective_scan", x, 4)
     rows, L, H, P = x.shape

@@ -101,6 +101,7 @@ def cuda(v, leaf=False):
 SHAPES = [  # B, L, H, G, P, N
     (1, 1, 1, 1, 1, 1), (2, 2, 4, 2, 32, 32), (3, 63, 2, 1, 17, 5), (2, 64, 4, 4, 64, 64), (1, 65, 2, 1, 128, 128), (2, 130, 6, 2, 48, 40),
     (5, 200, 3, 1, 33, 128), (1, 64 * 9 + 5, 2, 2, 64, 16), (2, 320, 4, 1, 20, 65), (1, 1030, 1, 1, 100, 33),
+    (2, 130, 5, 1, 66, 9), (1, 200, 8, 1, 64, 128), (1, 128, 12, 3, 24, 64), (1, 70, 16, 1, 128, 100), (4, 190, 7, 7, 96, 31),
 ]
 
 
@@ -428,6 +429,165 @@ def test_broadcast_inputs_get_summed_gradients():
     assert all(off(a, b) <= tol(torch.float32) for a, b in zip(got, want))
 
 
+@gpu
+def test_lengths_outside_the_batch_are_clamped():
+    from rtfs_net_amd.ssm import causal_conv
+
+    v = cuda(scan_inputs(3, 80, 2, 1, 16, 8, torch.float32, seed=11))
+    far, near = torch.tensor([-5, 300, 2 ** 31 - 1], dtype=torch.int32), torch.tensor([0, 80, 80], dtype=torch.int32)
+    assert all(torch.equal(a, b) for a, b in zip(gpu_scan(v, far), gpu_scan(v, near)))
+    x, w = v["x"].flatten(2), torch.randn(32, 4, device="cuda")
+    for a, b in zip(causal_conv(x, w, lengths=far.cuda(), return_state=True), causal_conv(x, w, lengths=near.cuda(), return_state=True)):
+        assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("tok,L", [(1 << 22, 1100), (1 << 23, 70)])
+def test_tokens_far_apart(tok, L):
+    """slices of a wide bf16 tensor whose offsets pass 2^32 elements (and tokens too far apart for the kernels, which are copied together): the bits of dense inputs"""
+    from rtfs_net_amd.ssm import causal_conv, selective_scan
+
+    wide = torch.empty(1, L, tok, dtype=torch.bfloat16, device="cuda")
+    wide[..., :132].normal_(generator=torch.Generator(device="cuda").manual_seed(0))
+    A, w = torch.tensor([-1.0, -4.0], device="cuda"), torch.randn(64, 4, device="cuda")
+
+    def run(u):
+        u = u.requires_grad_()
+        y = selective_scan(u[..., :64].unflatten(-1, (2, 32)), u[..., 128:130], A, u[..., 64:96].unflatten(-1, (1, 32)), u[..., 96:128].unflatten(-1, (1, 32)),
+                           softplus=True)
+        z = causal_conv(u[..., :64], w)
+        return [y.detach(), z.detach(), *torch.autograd.grad((y, z), u, (torch.ones_like(y), torch.ones_like(z)))]
+
+    dense = run(wide[..., :132].contiguous())
+    here = run(wide.detach()[..., :132])
+    assert all(torch.equal(a, b) for a, b in zip(dense, here))
+
+
+@gpu
+def test_more_than_2_31_elements():
+    """the last tokens of sequences whose tensors pass 2^31 elements are those of a call that starts in front of them"""
+    from rtfs_net_amd.ssm import causal_conv, selective_scan
+
+    r, kind = torch.Generator(device="cuda").manual_seed(0), torch.bfloat16
+    L, H, P, N = 70016, 512, 64, 16
+    cut = L - 64 * 20
+    x = torch.randn(1, L, H, P, dtype=kind, device="cuda", generator=r)
+    dt = torch.randn(1, L, H, device="cuda", generator=r) * 0.5 - 2
+    bc = torch.randn(2, 1, L, 1, N, dtype=kind, device="cuda", generator=r)
+    A = -1 - torch.rand(H, device="cuda", generator=r)
+    dy = torch.zeros(1, L, H, P, dtype=kind, device="cuda")
+    dy[:, cut:].normal_(generator=r)
+    with torch.no_grad():
+        _, state = selective_scan(x[:, :cut], dt[:, :cut], A, bc[0, :, :cut], bc[1, :, :cut], softplus=True, return_state=True)
+
+    def run(a, state):
+        leaves = [t.detach().requires_grad_() for t in (x[:, a:], dt[:, a:], bc[0, :, a:], bc[1, :, a:])]
+        y, s = selective_scan(leaves[0], leaves[1], A, leaves[2], leaves[3], softplus=True, state=state, return_state=True)
+        grads = torch.autograd.grad(y, leaves, dy[:, a:])
+        return [t[:, cut - a:].clone() for t in (y.detach(), *grads)] + [s]
+
+    for a, b, bound in zip(run(0, None), run(cut, state), (6 * U16, 6 * U16, tol(kind), 4 * U16, 4 * U16, tol(kind))):
+        assert off(a, b) <= 2 * bound
+    x = torch.randn(1, (1 << 21) + 70, 1024, dtype=kind, device="cuda", generator=r)
+    w = torch.randn(1024, 4, device="cuda", generator=r)
+    dy = torch.zeros_like(x)
+    dy[:, -200:].normal_(generator=r)
+    u, t = x.requires_grad_(), x.detach()[:, -200:].requires_grad_()
+    y, z = causal_conv(u, w), causal_conv(t, w, state=x.detach()[:, -203:-200])
+    du, dz = torch.autograd.grad(y, u, dy)[0], torch.autograd.grad(z, t, dy[:, -200:])[0]
+    assert torch.equal(y[:, -200:], z) and torch.equal(du[:, -200:], dz)
+
+
+@gpu
+def test_many_rows():
+    from rtfs_net_amd.ssm import causal_conv_step, selective_scan, selective_scan_step
+
+    B, P = (1 << 22) - 1, 100
+    x = torch.randn(B, 1, 1, P, device="cuda")
+    dt, A, bc, s = torch.rand(B, 1, 1, device="cuda"), torch.tensor([-1.0], device="cuda"), torch.randn(2, B, 1, 1, 1, device="cuda"), torch.ones(B, 1, P, 1, device="cuda")
+    y, last = selective_scan(x, dt, A, bc[0], bc[1], state=s, return_state=True)
+    one = selective_scan_step(x[:, 0], dt[:, 0], A, bc[0, :, 0], bc[1, :, 0], s)
+    d = dt[:, :, :, None].double()
+    want = torch.exp(-d) + d * x.double() * bc[0].double()
+    for got in (last, s):
+        assert float((got.view(B, 1, 1, P).double() - want).norm() / want.norm()) <= tol(torch.float32)
+    want *= bc[1].double()
+    for got in (y, one[:, None]):
+        assert float((got.double() - want).norm() / want.norm()) <= tol(torch.float32)
+    x = x.view(B, P)
+    state, w = torch.ones(B, 1, P, device="cuda"), torch.ones(P, 2, device="cuda")
+    assert torch.equal(causal_conv_step(x, state, w, silu=False), 1 + x) and torch.equal(state[:, 0], x)
+
+
+@gpu
+def test_serving_in_inference_mode():
+    from rtfs_net_amd.ssm import causal_conv_step, selective_scan, selective_scan_step
+
+    v = cuda(scan_inputs(2, 3, 2, 1, 16, 8, torch.bfloat16, seed=12))
+    with torch.inference_mode():
+        y, s = selective_scan(v["x"], v["dt"], v["A"], v["Bm"], v["C"], return_state=True)
+        held = torch.zeros(2, 2, 16, 8, device="cuda")
+        steps = [selective_scan_step(v["x"][:, t], v["dt"][:, t], v["A"], v["Bm"][:, t], v["C"][:, t], held) for t in range(3)]
+        conv = torch.zeros(2, 3, 32, dtype=torch.bfloat16, device="cuda")
+        causal_conv_step(v["x"][:, 0].flatten(1), conv, torch.ones(32, 4, device="cuda"))
+    assert off(torch.stack(steps, 1), y) <= 2 * tol(torch.bfloat16, 3) and off(held, s) <= 2 * tol(torch.bfloat16)
+    assert torch.equal(conv[:, 2], v["x"][:, 0].flatten(1))
+
+
+@gpu
+def test_calls_on_two_streams_at_once():
+    """each call's workspaces are its own: interleaved on two streams they give the bits of one after the other"""
+    v = [cuda(scan_inputs(1, 64 * 40, 2, 1, 64, 64, torch.float32, seed=s), leaf=True) for s in (0, 1)]
+    dy = torch.randn(1, 64 * 40, 2, 64, device="cuda")
+
+    def once(u):
+        y, s = gpu_scan(u)
+        return [y.detach(), s.detach(), *torch.autograd.grad((y, s), list(u.values()), (dy, torch.ones_like(s)))]
+
+    want = [once(u) for u in v]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for u, st in zip(v, streams):
+            with torch.cuda.stream(st):
+                got.append(once(u))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for p, q in zip(got, want) for a, b in zip(p, q))
+
+
+@gpu
+def test_captured_training_step_replays():
+    """convolution, scan and their gradients in one graph: each replay has the eager bits"""
+    from rtfs_net_amd.ssm import causal_conv
+
+    v = cuda(scan_inputs(2, 64 * 5 + 3, 4, 2, 32, 16, torch.bfloat16, seed=13), leaf=True)
+    w = torch.randn(128, 4, device="cuda", requires_grad=True)
+    dy = torch.randn(2, 64 * 5 + 3, 4, 32, device="cuda").bfloat16()
+    leaves = [*v.values(), w]
+
+    def step():
+        x = causal_conv(v["x"].flatten(2), w).unflatten(-1, (4, 32))
+        y, s = gpu_scan({**v, "x": x})
+        return [y.detach(), s.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(4):
+        with torch.no_grad():
+            for t in (v["x"], v["Bm"], v["C"], dy, w):
+                t.normal_()
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want)), i
+
+
 def test_refusals_of_the_convolution():
     from rtfs_net_amd.ssm import causal_conv, causal_conv_step
 
@@ -464,7 +624,8 @@ def test_refusals_of_the_scan():
                 lambda: selective_scan_step(x[:, 0], dt[:, 0], A, bc[:, 0], bc[:, 0], None), lambda: selective_scan_step(x[:, 0], dt[:, 0], A, bc[:, 0], bc[:, 0], s.bfloat16()),
                 lambda: selective_scan_step(x[:, 0], dt[:, 0], A, bc[:, 0], bc[:, 0], torch.zeros(2, 4, 3, 8).transpose(2, 3)),
                 lambda: selective_scan_step(x[:, 0], dt[:, 0], A, bc[:, 0], bc[:, 0], torch.zeros(193)[1:].view(2, 4, 8, 3)),
-                lambda: selective_scan(torch.zeros(1 << 23, 1, 4, 1), torch.zeros(1 << 23, 1, 4), A, torch.zeros(1 << 23, 1, 1, 1), torch.zeros(1 << 23, 1, 1, 1))):
+                lambda: selective_scan(torch.zeros(1 << 20, 1, 4, 1), torch.zeros(1 << 20, 1, 4), A, torch.zeros(1 << 20, 1, 1, 1), torch.zeros(1 << 20, 1, 1, 1)),
+                lambda: selective_scan(torch.zeros(1, 1, 1 << 17, 64), torch.zeros(1, 1, 1 << 17), torch.zeros(1 << 17), bc[:1, :1], bc[:1, :1])):
         with pytest.raises(ValueError):
             bad()
     with pytest.raises(TypeError):
