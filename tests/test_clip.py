@@ -103,6 +103,34 @@ def test_a_tensor_listed_twice_counts_once_and_versions_move():
     assert off(norm, g.norm()) < 1e-6 and off(p.grad, g / (norm + 1e-6)) < 1e-6 and p.grad._version > version
 
 
+@pytest.mark.gpu
+def test_gradients_at_the_same_address_are_refused():
+    from rtfs_net_amd.optim import clip_grad_norm_
+
+    p, q, r = params([(100,), (100,), (0,)], [torch.float32], "cuda")
+    empty = torch.nn.Parameter(torch.zeros(0, device="cuda"))
+    empty.grad = torch.zeros(0, device="cuda")
+    clip_grad_norm_([p, q, r, empty], 1.0)
+    q.grad = p.grad.view(100)
+    with pytest.raises(ValueError, match="same address"):
+        clip_grad_norm_([p, q, r], 1.0)
+
+
+@pytest.mark.gpu
+def test_more_than_2_31_elements():
+    """ones, but for the ends: the norm by counting"""
+    from rtfs_net_amd.optim import clip_grad_norm_
+
+    n = (1 << 31) + 5
+    p = torch.nn.Parameter(torch.empty(n, dtype=torch.bfloat16, device="cuda"))
+    p.grad = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    p.grad[0], p.grad[-1] = 2.0 ** 14, 2.0 ** 15
+    want = math.sqrt(n - 2 + 2.0 ** 28 + 2.0 ** 30)
+    norm = clip_grad_norm_(p, want / 4)
+    assert abs(float(norm) / want - 1) <= 2 * U[torch.float32]
+    assert float(p.grad[0]) == 2.0 ** 12 and float(p.grad[-1]) == 2.0 ** 13 and bool((p.grad[1:-1] == 0.25).all())
+
+
 def off(a, b):
     return float((a.double() - b.double()).norm() / b.double().norm())
 
