@@ -561,7 +561,7 @@ int rtfs_ssm_scan_fwd(const void* x, long long x_row, long long x_tok, const voi
                       const void* Bm, long long b_row, long long b_tok, const void* C, long long c_row, long long c_tok, const float* D, const float* dt_bias,
                       int softplus, const float* state, const int* lengths, void* y, float* last, float* work, int B, int L, int H, int P, int G, int N, int type,
                       void* stream);
-int rtfs_ssm_scan_bwd_parts(int B, int L, int H, int G);
+int rtfs_ssm_scan_bwd_parts(int B, int L, int H, int G, int N);
 /* dy [B][L][H][P], dlast (or NULL) -> dx, ddt (contiguous, dt's type), dA, dB, dC, dD / dbias / dstate (or NULL), all written */
 int rtfs_ssm_scan_bwd(const void* x, long long x_row, long long x_tok, const void* dt, long long dt_row, long long dt_tok, int dt_type, const float* A,
                       const void* Bm, long long b_row, long long b_tok, const void* C, long long c_row, long long c_tok, const float* D, const float* dt_bias,

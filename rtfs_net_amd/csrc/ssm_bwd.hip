@@ -407,11 +407,12 @@ __global__ __launch_bounds__(256) void sum_heads_kernel(const float* __restrict_
     if (threadIdx.x == 0) out[h] = (float)(red[0] + red[1] + red[2] + red[3]);
 }
 
-// Workgroups that share a group's heads: as few as give the chip two workgroups per CU
+// Workgroups that share a group's heads: as few as fill the chip - two workgroups of four waves per CU, or one of eight (N > 64).  More form C B^T more often and
+// leave partial gradients of B and C to be added (8 rows of 2048 tokens, 32 heads of 64, N = 128, one group: 324 us in one part, 328 + 12 us in two).
 static void grad_parts(const ScanArgs& a, int& parts, int& heads) {
     const int each = a.H / a.G;
     const long long blocks = (long long)a.rows * a.chunks * a.G;
-    const long long want = blocks >= 512 ? 1 : (512 + blocks - 1) / blocks;
+    const long long full = a.N > 64 ? 256 : 512, want = blocks >= full ? 1 : (full + blocks - 1) / blocks;
     heads = want >= each ? 1 : (int)((each + want - 1) / want);
     parts = (each + heads - 1) / heads;
 }
@@ -439,10 +440,10 @@ using namespace rtfs::ssm;
 
 extern "C" {
 
-int rtfs_ssm_scan_bwd_parts(int B, int L, int H, int G) {
-    if (!scan_sizes(B, L, H, 1, G, 1)) return RTFS_EINVAL;
+int rtfs_ssm_scan_bwd_parts(int B, int L, int H, int G, int N) {
+    if (!scan_sizes(B, L, H, 1, G, N)) return RTFS_EINVAL;
     ScanArgs a{};
-    a.rows = B, a.H = H, a.G = G, a.chunks = (L + kQ - 1) / kQ;
+    a.rows = B, a.H = H, a.G = G, a.N = N, a.chunks = (L + kQ - 1) / kQ;
     int parts, heads;
     grad_parts(a, parts, heads);
     return parts;

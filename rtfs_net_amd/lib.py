@@ -169,7 +169,7 @@ SIGNATURES = {
     "rtfs_ssm_scan_segments": [I] * 7,
     "rtfs_ssm_tile": [I, I],
     "rtfs_ssm_scan_fwd": [P, LL, LL, P, LL, LL, I, P, P, LL, LL, P, LL, LL, P, P, I, P, P, P, P, P] + [I] * 7 + [P],
-    "rtfs_ssm_scan_bwd_parts": [I, I, I, I],
+    "rtfs_ssm_scan_bwd_parts": [I] * 5,
     "rtfs_ssm_scan_bwd": [P, LL, LL, P, LL, LL, I, P, P, LL, LL, P, LL, LL, P, P, I] + [P] * 17 + [I] * 7 + [P],
     "rtfs_ssm_step": [P, LL, P, LL, I, P, P, LL, P, LL, P, P, I, P, P] + [I] * 6 + [P],
     "rtfs_clip_grad_norm": [P, P, P, I, D, I, P, I, P, P],

@@ -22,22 +22,24 @@ from . import lib
 __all__ = ["causal_conv", "causal_conv_step", "selective_scan", "selective_scan_step"]
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
+_FP32 = (torch.float32,)
 
 
 def _raw(t):
-    """address of a tensor that need not be contiguous (its pitches travel next to it)"""
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    """a tensor that need not be contiguous, for lib.call: its address (its pitches travel next to it)"""
+    return t if t is None or t.is_contiguous() else ctypes.c_void_p(t.data_ptr())
 
 
 def _check(name, what, t, shape, dtypes, device):
+    if isinstance(t, torch.Tensor) and t.shape == shape and t.dtype in dtypes and t.device == device:
+        return  # a single token's call is host time: one look when all is well
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: {what} must be a tensor, got {type(t).__name__}")
     if t.shape != shape:
         raise ValueError(f"{name}: {what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.dtype not in dtypes:
         raise ValueError(f"{name}: {what} must be {' or '.join(str(d)[6:] for d in dtypes)}, got {str(t.dtype)[6:]}")
-    if t.device != device:
-        raise ValueError(f"{name}: {what} is on {t.device}, x on {device}")
+    raise ValueError(f"{name}: {what} is on {t.device}, x on {device}")
 
 
 def _first(name, x, dims):
@@ -68,6 +70,11 @@ def _tokens(t, dims):
             break
         size *= n
     return t, t.stride(0), t.stride(1)
+
+
+def _rows(t):
+    """one token per row: t with the values of a row contiguous"""
+    return t if t.is_contiguous() or t[0].is_contiguous() else t.contiguous()
 
 
 def _lengths(name, lengths, B, device):
@@ -160,7 +167,7 @@ def causal_conv_step(x, state, weight, bias=None, *, silu=True):
     _on_gpu("causal_conv_step", x)
     y = torch.empty(B, D, dtype=x.dtype, device=x.device)
     if B and D:
-        x = x if x.stride(1) == 1 or D == 1 else x.contiguous()
+        x = _rows(x)
         lib.call("rtfs_causal_conv_step", _raw(x), x.stride(0), state, _dense(weight), _dense(bias), y, B, D, K, int(bool(silu)), _TYPES[x.dtype])
         torch.autograd.graph.increment_version(state)  # written through its address
     return y
@@ -210,7 +217,7 @@ class _SelectiveScan(torch.autograd.Function):
         dA, dD, db = new(H), new(H) if D is not None else None, new(H) if dt_bias is not None else None
         ds = torch.empty_like(state) if state is not None else None
         handle = lib.load()
-        segs, tile, parts, chunks = handle.rtfs_ssm_scan_segments(B, L, H, P, G, N, 2), handle.rtfs_ssm_tile(P, N), handle.rtfs_ssm_scan_bwd_parts(B, L, H, G), -(-L // 64)
+        segs, tile, parts, chunks = handle.rtfs_ssm_scan_segments(B, L, H, P, G, N, 2), handle.rtfs_ssm_tile(P, N), handle.rtfs_ssm_scan_bwd_parts(B, L, H, G, N), -(-L // 64)
         starts = new(2 * B * H * segs * (tile + 1)) if segs > 1 else None
         wide = new(2 * parts * B * L * G * N) if parts > 1 else None
         lib.call("rtfs_ssm_scan_bwd", _raw(x), xr, xt, _raw(dt), tr, tt, _TYPES[dt.dtype], A, _raw(Bm), br, bt, _raw(C), cr, ct, D, dt_bias, int(ctx.softplus), state,
@@ -229,14 +236,17 @@ def _scan_parameters(name, x, dt, A, B, C, D, dt_bias, state, lead):
         raise ValueError(f"{name}: at least one head, and 1 to 128 values per head and per state row (P = {P}, N = {N}, H = {H})")
     if G < 1 or H % G:
         raise ValueError(f"{name}: {H} heads do not divide over {G} groups of B and C")
-    _check(name, "dt", dt, (*lead, H), (x.dtype, torch.float32), x.device)
-    _check(name, "B", B, (*lead, G, N), (x.dtype,), x.device)
-    _check(name, "C", C, (*lead, G, N), (x.dtype,), x.device)
-    for what, t in (("A", A), ("D", D), ("dt_bias", dt_bias)):
-        if t is not None or what == "A":
-            _check(name, what, t, (H,), (torch.float32,), x.device)
+    device, kinds = x.device, (x.dtype,)
+    _check(name, "dt", dt, (*lead, H), (x.dtype, torch.float32), device)
+    _check(name, "B", B, (*lead, G, N), kinds, device)
+    _check(name, "C", C, (*lead, G, N), kinds, device)
+    _check(name, "A", A, (H,), _FP32, device)
+    if D is not None:
+        _check(name, "D", D, (H,), _FP32, device)
+    if dt_bias is not None:
+        _check(name, "dt_bias", dt_bias, (H,), _FP32, device)
     if state is not None:
-        _check(name, "state", state, (lead[0], H, P, N), (torch.float32,), x.device)
+        _check(name, "state", state, (lead[0], H, P, N), _FP32, device)
     if lead[0] * H >= 1 << 22:
         raise ValueError(f"{name}: {1 << 22} rows times heads, or more")
     if max(H * P, G * N) >= 1 << 23:
@@ -278,8 +288,7 @@ def selective_scan_step(x, dt, A, B, C, state, D=None, *, dt_bias=None, softplus
     _on_gpu("selective_scan_step", x)
     y = torch.empty(rows, H, P, dtype=x.dtype, device=x.device)
     if rows:
-        x, B, C = (t if t[0].is_contiguous() else t.contiguous() for t in (x, B, C))
-        dt = dt if dt.stride(1) == 1 or H == 1 else dt.contiguous()
+        x, dt, B, C = _rows(x), _rows(dt), _rows(B), _rows(C)
         lib.call("rtfs_ssm_step", _raw(x), x.stride(0), _raw(dt), dt.stride(0), _TYPES[dt.dtype], _dense(A), _raw(B), B.stride(0), _raw(C), C.stride(0), _dense(D),
                  _dense(dt_bias), int(bool(softplus)), state, y, rows, H, P, G, N, _TYPES[x.dtype])
         torch.autograd.graph.increment_version(state)  # written through its address

@@ -652,4 +652,4 @@ def test_the_library_refuses_what_its_kernels_cannot_take():
     for dims in ((0, 1, 1, 1, 1, 0), (1, 1, 1, 9, 1, 0), (1, 1, 1, 0, 1, 0), (1, 1, 1, 1, 1, 3)):
         assert conv(*dims) == -1
     assert h.rtfs_ssm_tile(129, 1) == -1 and h.rtfs_ssm_tile(33, 65) == 64 * 128 and h.rtfs_causal_conv_bwd_work_floats(0, 4, 0) == -1
-    assert h.rtfs_ssm_scan_segments(1, 64 * 100, 1, 16, 1, 16, 1) == 100 and h.rtfs_ssm_scan_segments(512, 64 * 100, 1, 16, 1, 16, 1) == 1 and h.rtfs_ssm_scan_bwd_parts(1, 64, 8, 3) == -1
+    assert h.rtfs_ssm_scan_segments(1, 64 * 100, 1, 16, 1, 16, 1) == 100 and h.rtfs_ssm_scan_segments(512, 64 * 100, 1, 16, 1, 16, 1) == 1 and h.rtfs_ssm_scan_bwd_parts(1, 64, 8, 3, 1) == -1
