@@ -90,14 +90,6 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
     const typename S::Slim& Rs = role_v ? Xs : Ys;
     const typename S::Wide &Ks = role_v ? Bs : Cs, &Os = role_v ? Cs : Bs;
     const float *mine = role_v ? q.behind : q.front;
-    {
-        const T* Bg = static_cast<const T*>(a.B) + b * a.b_row + t0 * a.b_tok + (long long)grp * a.N;
-        const T* Cg = static_cast<const T*>(a.C) + b * a.c_row + t0 * a.c_tok + (long long)grp * a.N;
-        Load<T, NP, S::kThreads> lb, lcc;
-        lb.ask(threadIdx.x, Bg, a.b_tok, rows, a.N, a.how_b);
-        lcc.ask(threadIdx.x, Cg, a.c_tok, rows, a.N, a.how_c);
-        lb.put(threadIdx.x, Bs), lcc.put(threadIdx.x, Cs);
-    }
     Load<T, PB, 128> ahead;  // x by waves 0 and 1, dy by waves 2 and 3
     auto ask = [&](int h, int p0) {
         const T* src = w < 2 ? static_cast<const T*>(a.x) + b * a.x_row + t0 * a.x_tok : static_cast<const T*>(q.dy) + ((long long)b * a.L + t0) * a.H * a.P;
@@ -106,7 +98,15 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
     };
     float raw = 0.f;
     auto ask_step = [&](int h) { raw = w < kRing && h + w < h1 && lane < rows ? a.dt.raw(b, t0 + lane, h + w) : 0.f; };
-    ask(h0, 0), ask_step(h0);
+    {
+        const T* Bg = static_cast<const T*>(a.B) + b * a.b_row + t0 * a.b_tok + (long long)grp * a.N;
+        const T* Cg = static_cast<const T*>(a.C) + b * a.c_row + t0 * a.c_tok + (long long)grp * a.N;
+        Load<T, NP, S::kThreads> lb, lcc;
+        lb.ask(threadIdx.x, Bg, a.b_tok, rows, a.N, a.how_b);
+        lcc.ask(threadIdx.x, Cg, a.c_tok, rows, a.N, a.how_c);
+        ask(h0, 0), ask_step(h0);
+        lb.put(threadIdx.x, Bs), lcc.put(threadIdx.x, Cs);
+    }
     __syncthreads();
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     const typename S::Wide::Lane ln;

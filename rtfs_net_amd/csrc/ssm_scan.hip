@@ -121,6 +121,7 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
             }
         }
 
+    const bool wanted = last && at.seg == a.segs - 1;
     const int c0 = at.seg * a.seg_chunks, c_all = c0 + a.seg_chunks < a.chunks ? c0 + a.seg_chunks : a.chunks;
     const int c_len = (len + kQ - 1) / kQ, c1 = c_all < c_len ? c_all : c_len;
     Load<T, NP, 256> lb, lcc;
@@ -251,7 +252,7 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
             }
         }
         if (c + 1 < c1) ask(c + 1);  // the registers of the products above are free again; the state's products hide the loads
-        if (at.works) advance<true>(S, X, Bs, e, false);
+        if (at.works && (c + 1 < c1 || wanted)) advance<true>(S, X, Bs, e, false);
     }
     if (!at.works) return;
     // chunks behind this row's end: nothing but zeros
@@ -260,7 +261,7 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
         T* out = y + (((long long)b * a.L + t0) * a.H + h) * a.P + at.p0;
         for (int i = lane; i < all * wide; i += 64) out[(long long)(i / wide) * a.H * a.P + i % wide] = (T)0.f;
     }
-    if (last && at.seg == a.segs - 1) {
+    if (wanted) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -330,7 +331,10 @@ __global__ __launch_bounds__(256, 2) void scan_walk_kernel(ScanArgs a0, WalkOut 
         lx.ask(lane, x + t0 * a.x_tok, a.x_tok, rows, cols, a.how_x);
         raw = lane < rows ? a.dt.raw(b, t0 + lane, h) : 0.f;
     };
-    ask(k0);
+    // the last chunk's own step is taken if what is behind the segment is asked for
+    const bool final = o.last && at.seg == a.segs - 1;
+    const int k2 = o.ends || final ? k1 : k1 - 1;
+    if (k0 < k2) ask(k0);
     for (int k = k0; k < k1; ++k) {
         const int c = chunk(k), t0 = c * kQ;
         if (o.tiles && at.works) {
@@ -340,12 +344,13 @@ __global__ __launch_bounds__(256, 2) void scan_walk_kernel(ScanArgs a0, WalkOut 
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) *reinterpret_cast<f32x4*>(to + (pt * NT + nt) * 256) = S[pt][nt];
         }
+        if (k == k2) break;
         __syncthreads();
         if (t0 < len) {
             lb.put(threadIdx.x, Bs), lx.put(lane, X);
             put_decays(e, raw, t0 + lane < len, a.dt.softplus, A);
         }
-        if (k + 1 < k1) ask(k + 1);
+        if (k + 1 < k2) ask(k + 1);
         __syncthreads();
         if (t0 >= len || !at.works) continue;
         sum += (double)e.hi[kQ - 1] + (double)e.lo[kQ - 1];
@@ -353,7 +358,6 @@ __global__ __launch_bounds__(256, 2) void scan_walk_kernel(ScanArgs a0, WalkOut 
     }
     if (!at.works) return;
     float* out = o.ends ? o.ends + (head * a.segs + at.seg) * PP * NP + at.p0 * NP : nullptr;
-    const bool final = o.last && at.seg == a.segs - 1;
 #pragma unroll
     for (int pt = 0; pt < PT; ++pt)
 #pragma unroll

@@ -117,6 +117,7 @@ def test_scan_matches_the_recurrence(shape, kind):
         y, s = gpu_scan(cuda(v), lengths)
         assert y.dtype == kind and s.dtype == torch.float32
         assert off(y, want) <= tol(kind, 3) and off(s, last) <= tol(kind), (pad, off(y, want), off(s, last))
+        assert torch.equal(gpu_scan(cuda(v), lengths, want_state=False), y)
 
 
 @gpu
@@ -310,6 +311,21 @@ def test_optional_arguments():
         for k, a, b in zip(leaves, got, want):
             assert off(a, torch.zeros(a.shape) if b is None else b) <= 8 * tol(torch.float32), (pick, k)
     assert torch.equal(selective_scan(*(t.detach() for t in here.values())), selective_scan(*here.values()).detach())
+
+
+@gpu
+def test_no_state_is_a_state_of_zeros():
+    """nothing of what a call does not ask for is needed by the rest of it, in rows of one segment and of many"""
+    for B, L in ((1, 64), (1, 1030), (300, 130)):
+        v = scan_inputs(B, L, 4, 2, 32, 24, torch.bfloat16, seed=14)
+        v["state"].zero_()
+        here = cuda(v, leaf=True)
+        names = [k for k in here if k != "state"]
+        y, s = gpu_scan(here)
+        want = torch.autograd.grad(y, [here[k] for k in names], torch.ones_like(y))
+        z = gpu_scan({**here, "state": None}, want_state=False)
+        got = torch.autograd.grad(z, [here[k] for k in names], torch.ones_like(z))
+        assert torch.equal(y, z) and all(torch.equal(a, b) for a, b in zip(want, got)), (B, L)
 
 
 @gpu
