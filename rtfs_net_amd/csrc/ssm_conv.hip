@@ -77,12 +77,28 @@ __device__ __forceinline__ void conv_input(const ConvArgs& a, int b, int t, int 
 }
 template <int K, int V>
 __device__ __forceinline__ void conv_weights(const ConvArgs& a, int d, float (&w)[K][V], float (&bias)[V]) {
+    float all[V][K];
+    const float* from = a.w + (long long)d * K;
+    if constexpr (V == 1) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
+        for (int k = 0; k < K; ++k) all[0][k] = from[k];
+        bias[0] = a.bias ? a.bias[d] : 0.f;
+    } else {  // the weights of V neighbouring channels are V K neighbouring values
 #pragma unroll
-        for (int k = 0; k < K; ++k) w[k][e] = a.w[(long long)(d + e) * K + k];
-        bias[e] = a.bias ? a.bias[d + e] : 0.f;
+        for (int i = 0; i < V * K; i += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(from + i);
+            all[i / K][i % K] = v.x, all[(i + 1) / K][(i + 1) % K] = v.y, all[(i + 2) / K][(i + 2) % K] = v.z, all[(i + 3) / K][(i + 3) % K] = v.w;
+        }
+#pragma unroll
+        for (int e = 0; e < V; e += 4) {
+            const float4 v = a.bias ? *reinterpret_cast<const float4*>(a.bias + d + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+            bias[e] = v.x, bias[e + 1] = v.y, bias[e + 2] = v.z, bias[e + 3] = v.w;
+        }
     }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[k][e] = all[e][k];
 }
 
 constexpr int kConvAhead = 4;  // tokens asked for at a time
@@ -292,7 +308,7 @@ static bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) =
 template <typename T>
 static int conv_vector(const ConvArgs& a, const void* p0, const void* p1, const void* p2, const void* p3) {
     constexpr int V = 16 / sizeof(T);
-    const bool ok = a.D % V == 0 && a.x_row % V == 0 && a.x_tok % V == 0 && on16(a.x) && on16(a.state) && on16(p0) && on16(p1) && on16(p2) && on16(p3);
+    const bool ok = a.D % V == 0 && a.x_row % V == 0 && a.x_tok % V == 0 && on16(a.x) && on16(a.w) && on16(a.bias) && on16(a.state) && on16(p0) && on16(p1) && on16(p2) && on16(p3);
     return ok ? V : 1;
 }
 // channel vectors per workgroup row: the widest of 64, 32, 16, 8 that leaves no more idle threads than a narrower one would

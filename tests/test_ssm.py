@@ -175,13 +175,14 @@ def test_scan_gradient_against_differences():
 
 @gpu
 @pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
-@pytest.mark.parametrize("B,H,G,P,N", [(1, 4, 1, 32, 32), (3, 6, 2, 48, 40), (2, 3, 3, 33, 7), (2, 2, 1, 128, 128), (1, 1, 1, 1, 1)])
-def test_prompt_in_pieces_then_single_tokens(kind, B, H, G, P, N):
+@pytest.mark.parametrize("B,H,G,P,N,pad", [(1, 4, 1, 32, 32, 0), (3, 6, 2, 48, 40, 0), (2, 3, 3, 33, 7, 0), (2, 2, 1, 128, 128, 0), (1, 1, 1, 1, 1, 0), (2, 4, 2, 20, 12, 3),
+                                           (3, 2, 1, 16, 100, 4)])
+def test_prompt_in_pieces_then_single_tokens(kind, B, H, G, P, N, pad):
     """a prompt cut anywhere, then one token at a time, is the whole sequence; the conv goes on the same way"""
     from rtfs_net_amd.ssm import causal_conv, causal_conv_step, selective_scan, selective_scan_step
 
     L = 150
-    v = scan_inputs(B, L, H, G, P, N, kind, seed=9)
+    v = scan_inputs(B, L, H, G, P, N, kind, seed=9, pad=pad)
     want, last = ref_scan(*(v[k].double() for k in ("x", "dt", "A", "Bm", "C", "D", "bias")), True, v["state"].double(), None)
     c = cuda(v)
     ys, state = [], c["state"]
@@ -230,6 +231,30 @@ def test_conv_and_its_gradients(kind, B, L, D, K, silu, pad):
             # w and b: fp32 sums over B L tokens whose magnitudes add up to at most sqrt(B L) of the result for random signs
             bound = tol(kind, 1) if k in ("x", "state") else 64 * U32 * max(1.0, (B * L) ** 0.5)
             assert off(g, torch.zeros_like(g, device="cpu") if q is None else q) <= bound, (k, ragged, off(g, q))
+
+
+@gpu
+def test_addresses_off_16_bytes():
+    """every tensor a few values into its storage: the bits of aligned ones"""
+    from rtfs_net_amd.ssm import causal_conv, causal_conv_step, selective_scan_step
+
+    def shifted(t):
+        return torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)
+
+    for kind in (torch.float32, torch.bfloat16):
+        x, w, b, s = torch.randn(2, 40, 64, device="cuda").to(kind), torch.randn(64, 4, device="cuda"), torch.randn(64, device="cuda"), torch.randn(2, 3, 64, device="cuda").to(kind)
+        for off_x, off_w in ((True, False), (False, True), (True, True)):
+            (p, u), (q, c, t) = (shifted(v) if off_x else v.clone() for v in (x, s)), (shifted(w) if off_w else w, shifted(b) if off_w else b, s.clone())
+            for p0, p1 in zip(causal_conv(x, w, b, state=s, return_state=True), causal_conv(p, q, c, state=u, return_state=True)):
+                assert torch.equal(p0, p1)
+            assert torch.equal(causal_conv_step(x[:, 0], t, w, b), causal_conv_step(p[:, 0], u, q, c)) and torch.equal(t, u)
+        v = cuda(scan_inputs(2, 100, 4, 2, 32, 32, kind, seed=15))
+        m = {k: shifted(t) for k, t in v.items()}
+        y, z = gpu_scan(v), gpu_scan(m)
+        assert torch.equal(y[0], z[0]) and torch.equal(y[1], z[1])
+        s0, s1 = v["state"].clone(), v["state"].clone()
+        names = [(u["x"][:, 0], u["dt"][:, 0], u["A"], u["Bm"][:, 0], u["C"][:, 0]) for u in (v, m)]
+        assert torch.equal(selective_scan_step(*names[0], s0), selective_scan_step(*names[1], s1)) and torch.equal(s0, s1)
 
 
 @gpu
