@@ -104,6 +104,7 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
     const Lanes<T, NP, kSwapped> ln;
     const Lanes<T, PW, kDownOnly> lp;
 
+    const bool by_four = a.N % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.state) | reinterpret_cast<uintptr_t>(last)) & 15) == 0;  // state rows lie on 16 bytes
     f32x4 S[NT][PT];  // rows n, columns p
     const float* start = at.seg > 0 ? starts + (((long long)b * a.H + h) * a.segs + at.seg) * (padded(a.P) * NP) + at.p0 * NP : nullptr;
 #pragma unroll
@@ -115,9 +116,14 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
             if (start) {
                 S[nt][pt] = *reinterpret_cast<const f32x4*>(start + p * NP + n);
             } else if (a.state && p < cols) {
+                const float* from = a.state + (state_at + p) * a.N + n;
+                if (by_four) {
+                    if (n < a.N) S[nt][pt] = *reinterpret_cast<const f32x4*>(from);
+                } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (n + i < a.N) S[nt][pt][i] = a.state[(state_at + p) * a.N + n + i];
+                    for (int i = 0; i < 4; ++i)
+                        if (n + i < a.N) S[nt][pt][i] = from[i];
+                }
             }
         }
 
@@ -268,9 +274,14 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
             for (int pt = 0; pt < PT; ++pt) {
                 const int p = 16 * pt + lc, n = swapped(nt, 4 * g);
                 if (p < cols) {
+                    float* to = last + (state_at + p) * a.N + n;
+                    if (by_four) {
+                        if (n < a.N) *reinterpret_cast<f32x4*>(to) = S[nt][pt];
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (n + i < a.N) last[(state_at + p) * a.N + n + i] = S[nt][pt][i];
+                        for (int i = 0; i < 4; ++i)
+                            if (n + i < a.N) to[i] = S[nt][pt][i];
+                    }
                 }
             }
     }
