@@ -41,6 +41,8 @@ template <> __device__ __forceinline__ Frag<float> frag_of<float>(f32x4 a, f32x4
 template <> __device__ __forceinline__ Frag<__bf16> frag_of<__bf16>(f32x4 a, f32x4 b) {
     return {__builtin_shufflevector(__builtin_convertvector(a, bf16x4), __builtin_convertvector(b, bf16x4), 0, 1, 2, 3, 4, 5, 6, 7)};
 }
+// what rounding to bf16 leaves of them
+__device__ __forceinline__ f32x4 rest_of(f32x4 a) { return a - __builtin_convertvector(__builtin_convertvector(a, bf16x4), f32x4); }
 // An fp32 operand as the sum of three bf16, 8 bits of its 24-bit mantissa each and so exact: states, what builds them, and the sums that the gradients of dt and A
 // are differences of keep fp32's precision for bf16 tensors too.  fp32 operands are themselves.
 template <typename T> struct Split {
@@ -135,6 +137,7 @@ template <int ROWS, int COLS, Kind KIND> struct Tile<float, ROWS, COLS, KIND> {
         *reinterpret_cast<f32x4*>(v + p.at + rows * kPitch + 4) = x.b;
     }
     __device__ __forceinline__ void put4(int r, int c, f32x4 x) { *reinterpret_cast<f32x4*>(v + r * kPitch + c) = x; }
+    __device__ __forceinline__ f32x4 get4(int r, int c) const { return *reinterpret_cast<const f32x4*>(v + r * kPitch + c); }
     __device__ __forceinline__ void put(int r, int c, float x) { v[r * kPitch + c] = x; }
     // lane l: row r + (l & 15), values from c (a multiple of 32) on
     __device__ __forceinline__ Frag<float> row(const Lane& l, int r, int c) const {
@@ -176,6 +179,7 @@ template <int ROWS, int COLS, Kind KIND> struct Tile<__bf16, ROWS, COLS, KIND> {
         }
     }
     __device__ __forceinline__ void put4(int r, int c, f32x4 x) { *reinterpret_cast<bf16x4*>(v + at(r, c)) = __builtin_convertvector(x, bf16x4); }
+    __device__ __forceinline__ f32x4 get4(int r, int c) const { return __builtin_convertvector(*reinterpret_cast<const bf16x4*>(v + at(r, c)), f32x4); }
     __device__ __forceinline__ void put(int r, int c, float x) { v[at(r, c)] = (__bf16)x; }
     __device__ __forceinline__ Frag<__bf16> row(const Lane& l, int r, int c) const {
         return {*reinterpret_cast<const bf16x8*>(v + r * COLS + (c >> 6 << 6) + l.row[c >> 5 & (Lane::kRow - 1)])};

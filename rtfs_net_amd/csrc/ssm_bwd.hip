@@ -177,12 +177,7 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
                     for (int r = 0; r < 2; ++r) {
                         const int tt = 2 * k + r;
                         m[r] = zero;
-                        if (tt >= jt) {
-                            m[r] = cb[tt] * decay_tile(tt) * d;
-                            if (tt == jt)
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) m[r][i] += 4 * g + i == lc ? D : 0.f;
-                        }
+                        if (tt >= jt) m[r] = cb[tt] * decay_tile(tt) * d;
                     }
                     wgt[k] = frag_of<T>(m[0], m[1]);
                 }
@@ -277,7 +272,7 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
                 f32x4 acc = zero;  // rows p, columns j
 #pragma unroll
                 for (int k = 0; k < NP / 32; ++k) acc = mma(alt ? Gs.down(lg, 32 * k, pt + S::kAlt - 1) : Gs.down(lg, 32 * k, pt), Bs.row(ln, 16 * jt, 32 * k), acc);
-                acc *= end;
+                acc = acc * end + Ys.get4(j, 16 * (pt + alt) + 4 * g) * D;  // (as a part of the weights D would be rounded with them)
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
                     if (2 * k + 1 >= jt) acc = mma(alt ? Ys.down(lp, 32 * k, pt + S::kAlt - 1) : Ys.down(lp, 32 * k, pt), wgt[k], acc);

@@ -73,8 +73,9 @@ __device__ __forceinline__ void advance(f32x4 (&S)[R][C], const Tile<T, kQ, PW, 
 // A wave walks one segment of its slice and keeps the state in its accumulators from chunk to chunk: an accumulator tile is, as it lies, the operand of the
 // product with C, so the state never leaves registers.  So do the scores: C B^T of a pair of token tiles, times decay and step (D joins the diagonal), is the
 // operand of the product with x.  LDS holds B and C once for four waves and each wave's x; two barriers per chunk.
-// Roundings (bf16): the scores times decay and step, and the state as it enters the product with C, once each to bf16 - y is rounded to that anyway; the
-// weighted inputs that build the state are split (ssm.h), so the state that is handed on has fp32's precision.
+// Roundings (bf16): the scores times decay and step, and the state as it enters the product with C, once each to bf16 - y is rounded to that anyway.  The token
+// tiles on the diagonal keep what the rounding leaves as a second operand: D = 1.01 alone would be off by 0.2 % in every token, more than y's own rounding.
+// The weighted inputs that build the state are split (ssm.h), so the state that is handed on has fp32's precision.
 template <typename T, int NP, int PW> struct ScanShare {
     static constexpr int kBytes = 2 * Tile<T, kQ, NP, kSwapped>::kBytes + 4 * (Tile<T, kQ, PW, kDownOnly>::kBytes + (int)(sizeof(Decays) + sizeof(Factors)));
     // waves per SIMD: two (256 registers each) where a CU's LDS holds as many workgroups, else one
@@ -86,6 +87,7 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
                                                                                           float* __restrict__ last) {
     typedef T T4 __attribute__((ext_vector_type(4)));
     constexpr int NT = NP / 16, PT = PW / 16;
+    constexpr bool kRest = sizeof(T) == 2;
     __shared__ __attribute__((aligned(16))) Tile<T, kQ, NP, kSwapped> Bs, Cs;
     __shared__ __attribute__((aligned(16))) Tile<T, kQ, PW, kDownOnly> Xs[4];
     __shared__ __attribute__((aligned(16))) Decays decays[4];
@@ -159,7 +161,7 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int pt = 0; pt < PT; ++pt) asm volatile("" : "+v"(S[nt][pt]));
-                Frag<T> q[2][NP / 32], m[2][2];
+                Frag<T> q[2][NP / 32], m[2][2], rest[2];
 #pragma unroll
                 for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -198,6 +200,7 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
                     }
                     m[0][kk] = frag_of<T>(s[0][0], s[0][1]);
                     m[1][kk] = frag_of<T>(s[1][0], s[1][1]);
+                    if (kRest && kk == half) rest[0] = frag_of<T>(rest_of(s[0][0]), f32x4{0.f, 0.f, 0.f, 0.f}), rest[1] = frag_of<T>(f32x4{0.f, 0.f, 0.f, 0.f}, rest_of(s[1][1]));
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 constexpr int kSome = PT < 2 ? PT : 2;
@@ -230,6 +233,7 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
                             const Frag<T> xj = X.down(lp, 32 * kk, p0 + pt);
                             acc[0][pt] = mma(xj, m[0][kk], acc[0][pt]);
                             acc[1][pt] = mma(xj, m[1][kk], acc[1][pt]);
+                            if (kRest && kk == half) acc[0][pt] = mma(xj, rest[0], acc[0][pt]), acc[1][pt] = mma(xj, rest[1], acc[1][pt]);
                         }
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
