@@ -29,8 +29,8 @@ struct GradArgs {
 //   states: the first half of the waves forms U = dy H, the other V = x G, each for its 16-wide slices of N; the tiles of H and G come from memory as operands.
 // P goes through in blocks of 64.  Steps and decays are made for four heads at a time, one per wave, and the per-token sums of four heads are finished at a
 // time likewise: on one wave they were a third of a head's time.  x and dy are asked for one block ahead.
-// What a and d(step) need is summed in fp32 from products of split operands (ssm.h); what only dx, dB and dC need is rounded to the tensors' type once on its
-// way into a product.
+// What a and d(step) need is summed in fp32 from products of split operands (ssm.h), and so is what dB and dC take from the states; the scores that dB and dC are
+// formed of keep what the rounding leaves as a second operand.  What only dx needs is rounded to the tensors' type once on its way into a product.
 constexpr int kRing = 4;  // heads per ring of decays and sums
 
 template <int HALF, int ALT> struct HeadSums {
@@ -48,7 +48,8 @@ template <typename T, int NP, int PP> struct GradShare {
     typedef Tile<T, NP, PB, kDownOnly> States;
     typedef Tile<T, kQ, kQ, kInOrder> Scores;
     typedef HeadSums<kHalf, kAlt> Sums;
-    static constexpr int kMain = 2 * Slim::kBytes + States::kBytes, kPool = kMain > Scores::kBytes ? kMain : Scores::kBytes;
+    static constexpr int kParts = sizeof(T) == 2 ? 2 : 1;  // bf16: the scores summed over the heads, and what rounding leaves of them
+    static constexpr int kMain = 2 * Slim::kBytes + States::kBytes, kLast = kParts * Scores::kBytes, kPool = kMain > kLast ? kMain : kLast;
     static constexpr int kBytes = 2 * Wide::kBytes + kPool + kRing * (int)(sizeof(Decays) + sizeof(Factors) + sizeof(Sums));
     static constexpr int kWavesPerSimd = kWaves == 8 || kBytes * 2 <= 160 * 1024 ? 2 : 1;
 };
@@ -330,12 +331,16 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
     }
     // dC += (V o E) d B, dB += (V o E)^T d C, summed over the heads before the product
     const typename S::Scores::Lane lq;
-    typename S::Scores& Ms = *reinterpret_cast<typename S::Scores*>(pool);
+    typename S::Scores* Ms = reinterpret_cast<typename S::Scores*>(pool);
     __syncthreads();
 #pragma unroll
     for (int o = 0; o < kOwn; ++o)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) Ms.put(16 * (o * S::kAlt + alt) + 4 * g + i, j, dcb[o][i]);
+        for (int i = 0; i < 4; ++i) {
+            const int t = 16 * (o * S::kAlt + alt) + 4 * g + i;
+            Ms[0].put(t, j, dcb[o][i]);
+            if (S::kParts == 2) Ms[1].put(t, j, dcb[o][i] - (float)(T)dcb[o][i]);
+        }
     __syncthreads();
     T* grad = static_cast<T*>(role_v ? q.dB : q.dC);
     float* wide = role_v ? q.pB : q.pC;
@@ -346,7 +351,9 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
         for (int k = 0; k < 2; ++k) {
             const Frag<T> o = Os.down_any(32 * k, nt0 + s);
 #pragma unroll
-            for (int tt = 0; tt < 4; ++tt) sum[tt][s] = mma(o, role_v ? Ms.down(lq, 32 * k, tt) : Ms.row(lq, 16 * tt, 32 * k), sum[tt][s]);
+            for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+                for (int m = S::kParts - 1; m >= 0; --m) sum[tt][s] = mma(o, role_v ? Ms[m].down(lq, 32 * k, tt) : Ms[m].row(lq, 16 * tt, 32 * k), sum[tt][s]);
         }
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
