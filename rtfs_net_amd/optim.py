@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import array
 import math
+import operator
 
 import torch
 
@@ -140,8 +141,9 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0):
     passed over) taken as one vector, and every gradient scaled in place by min(1, max_norm / (norm + 1e-6)).
 
     norm_type 2 or inf.  fp32, bf16 and fp16 gradients in any mix, dense in any order of their dimensions, without memory in common, on one device; the same
-    tensor listed twice counts once.  The norm's squares are summed in fp64 in a fixed order.  -> the norm before clipping, a 0-dim fp32 tensor on the gradients' device (nothing is copied
-    to the host; a norm that is not finite is not an error: a NaN goes through to every gradient).  Every gradient is written, also where the factor is 1."""
+    tensor listed twice counts once.  The norm's squares are summed in fp64 in a fixed order.  -> the norm before clipping, a 0-dim fp32 tensor on the gradients'
+    device (nothing is copied to the host; a norm that is not finite is not an error: a NaN goes through to every gradient).  Every gradient is written, also where
+    the factor is 1."""
     max_norm, norm_type = float(max_norm), float(norm_type)
     if not max_norm >= 0.0:
         raise ValueError("clip_grad_norm_: max_norm must not be negative")
@@ -152,24 +154,26 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0):
     grads = [g for g in [p.grad for p in parameters] if g is not None]
     if not grads:
         return torch.zeros(())
-    if len(set(map(id, grads))) != len(grads):
-        grads = list({id(g): g for g in grads}.values())
     # one pass per question over all tensors: a small model's hundreds of them are host time, not device time
-    kinds = [_CLIP_TYPES.get(g.dtype, -1) for g in grads]
-    devices = set(map(torch.Tensor.get_device, grads))
-    if -1 in kinds or -1 in devices or {g.layout for g in grads} != {torch.strided}:
+    kinds, devices = set(map(operator.attrgetter("dtype"), grads)), set(map(torch.Tensor.get_device, grads))
+    if not kinds <= _CLIP_TYPES.keys() or -1 in devices or set(map(operator.attrgetter("layout"), grads)) != {torch.strided}:
         raise ValueError("clip_grad_norm_: gradients must be dense fp32, bf16 or fp16 HIP tensors")
     if len(devices) > 1:
         raise ValueError(f"clip_grad_norm_: gradients on devices {sorted(devices)}")
-    if not all(g.is_contiguous() or _fills_its_span(g) for g in grads):
+    if not all(map(torch.Tensor.is_contiguous, grads)) and not all(g.is_contiguous() or _fills_its_span(g) for g in grads):
         raise ValueError("clip_grad_norm_: a gradient has gaps or overlaps in memory")
     device = grads[0].device
+    at = array.array("q", map(torch.Tensor.data_ptr, grads))
+    if len(set(at)) != len(at):  # the same tensor more than once, or empty ones
+        grads = [g for g in {id(g): g for g in grads}.values() if g.numel()]
+        at = array.array("q", map(torch.Tensor.data_ptr, grads))
+        if len(set(at)) != len(at):
+            raise ValueError("clip_grad_norm_: two gradients start at the same address")
     sizes = array.array("q", map(torch.Tensor.numel, grads))
     if not any(sizes):
         return torch.zeros((), device=device)
-    at, types = array.array("q", map(torch.Tensor.data_ptr, grads)), array.array("i", kinds)
-    if len(set(at)) != len(at) and len({a for a, n in zip(at, sizes) if n}) != sum(1 for n in sizes if n):
-        raise ValueError("clip_grad_norm_: two gradients start at the same address")
+    types = [_CLIP_TYPES[g.dtype] for g in grads] if len(kinds) > 1 else [_CLIP_TYPES[grads[0].dtype]] * len(grads)
+    types = array.array("i", types)
     norm = torch.empty((), device=device)
     parts = torch.empty(2048 + len(grads) + (sum(sizes) >> 30), dtype=torch.float64, device=device)  # a tensor of over 2^30 elements is listed in pieces
     lib.call("rtfs_clip_grad_norm", at.buffer_info()[0], sizes.buffer_info()[0], types.buffer_info()[0], len(grads), max_norm, 2 if norm_type == 2.0 else 0, parts,

@@ -111,6 +111,11 @@ def test_gradients_at_the_same_address_are_refused():
     empty = torch.nn.Parameter(torch.zeros(0, device="cuda"))
     empty.grad = torch.zeros(0, device="cuda")
     clip_grad_norm_([p, q, r, empty], 1.0)
+    odd = torch.nn.Parameter(torch.zeros(5, 0, device="cuda"))
+    turned = torch.nn.Parameter(torch.zeros(4, 6, device="cuda").t())
+    odd.grad, turned.grad = torch.zeros(5, 0, device="cuda"), torch.randn(4, 6, device="cuda").t()
+    want = torch.cat([p.grad.flatten(), turned.grad.flatten()]).double().norm()
+    assert off(clip_grad_norm_([p, odd, turned, r, p, empty], 0.5), want) < 1e-6
     q.grad = p.grad.view(100)
     with pytest.raises(ValueError, match="same address"):
         clip_grad_norm_([p, q, r], 1.0)
