@@ -208,7 +208,8 @@ def test_prompt_in_pieces_then_single_tokens(kind, B, H, G, P, N, pad):
 @gpu
 @pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("B,L,D,K,silu,pad", [(1, 1, 1, 1, True, 0), (2, 3, 5, 8, True, 0), (3, 70, 64, 4, True, 0), (2, 33, 40, 3, False, 8), (1, 300, 24, 4, True, 3),
-                                              (4, 129, 512, 2, True, 0), (2, 2, 16, 5, True, 0), (7, 37, 192, 6, False, 0), (1, 40, 700, 7, True, 0)])
+                                              (4, 129, 512, 2, True, 0), (2, 2, 16, 5, True, 0), (7, 37, 192, 6, False, 0), (1, 40, 700, 7, True, 0), (2, 45, 64, 1, True, 0),
+                                              (2, 45, 64, 8, True, 0), (1, 9, 8, 5, True, 0)])
 def test_conv_and_its_gradients(kind, B, L, D, K, silu, pad):
     from rtfs_net_amd.ssm import causal_conv
 
@@ -537,6 +538,20 @@ def test_more_than_2_31_elements():
     y, z = causal_conv(u, w), causal_conv(t, w, state=x.detach()[:, -203:-200])
     du, dz = torch.autograd.grad(y, u, dy)[0], torch.autograd.grad(z, t, dy[:, -200:])[0]
     assert torch.equal(y[:, -200:], z) and torch.equal(du[:, -200:], dz)
+
+
+@gpu
+@pytest.mark.parametrize("K", range(1, 9))
+def test_single_tokens_of_every_width(K):
+    """prompt and single tokens give the same bits, and the same state, for each number of taps"""
+    from rtfs_net_amd.ssm import causal_conv, causal_conv_step
+
+    for kind, D in ((torch.float32, 64), (torch.bfloat16, 64), (torch.float32, 33), (torch.bfloat16, 33)):
+        x, w = torch.randn(3, 12, D, device="cuda").to(kind), torch.randn(D, K, device="cuda")
+        want, last = causal_conv(x, w, return_state=True)
+        state = torch.zeros(3, K - 1, D, dtype=kind, device="cuda")
+        got = torch.stack([causal_conv_step(x[:, t], state, w) for t in range(12)], 1)
+        assert torch.equal(got, want) and torch.equal(state, last)
 
 
 @gpu
