@@ -78,6 +78,9 @@ __device__ __forceinline__ void advance(f32x4 (&S)[R][C], const Tile<T, kQ, PW, 
 // Roundings (bf16): the scores times decay and step, and the state as it enters the product with C, once each to bf16 - y is rounded to that anyway.  The token
 // tiles on the diagonal keep what the rounding leaves as a second operand: D = 1.01 alone would be off by 0.2 % in every token, more than y's own rounding.
 // The weighted inputs that build the state are split (ssm.h), so the state that is handed on has fp32's precision.
+// Up to kChain segments a row are chained by the kernel itself, from the own states of the segments in front: that reads each of them half kChain times on average,
+// where a launch that chains them reads and writes each and has it read once more (8 rows of four segments, 32 heads of 64 x 128: 16 us).
+constexpr int kChain = 8;
 template <typename T, int NP, int PW> struct ScanShare {
     static constexpr int kBytes = 2 * Tile<T, kQ, NP, kSwapped>::kBytes + 4 * (Tile<T, kQ, PW, kDownOnly>::kBytes + (int)(sizeof(Decays) + sizeof(Factors)));
     // waves per SIMD: two (256 registers each) where a CU's LDS holds as many workgroups, else one
@@ -85,7 +88,8 @@ template <typename T, int NP, int PW> struct ScanShare {
 };
 
 template <typename T, int NP, int PW>
-__global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void scan_kernel(ScanArgs a, const float* __restrict__ starts, T* __restrict__ y,
+__global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void scan_kernel(ScanArgs a, const float* __restrict__ starts,
+                                                                                          const float* __restrict__ segment_decays, T* __restrict__ y,
                                                                                           float* __restrict__ last) {
     typedef T T4 __attribute__((ext_vector_type(4)));
     constexpr int NT = NP / 16, PT = PW / 16;
@@ -110,7 +114,10 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
 
     const bool by_four = a.N % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.state) | reinterpret_cast<uintptr_t>(last)) & 15) == 0;  // state rows lie on 16 bytes
     f32x4 S[NT][PT];  // rows n, columns p
-    const float* start = at.seg > 0 ? starts + (((long long)b * a.H + h) * a.segs + at.seg) * (padded(a.P) * NP) + at.p0 * NP : nullptr;
+    const int tile = padded(a.P) * NP;
+    const bool chain = a.segs <= kChain;
+    const float* ends = a.segs > 1 ? starts + ((long long)b * a.H + h) * a.segs * tile + at.p0 * NP + lc * NP + swapped(0, 4 * g) : nullptr;
+    const float* start = at.seg > 0 && !chain ? ends + (long long)at.seg * tile : nullptr;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -118,7 +125,7 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
             const int p = 16 * pt + lc, n = swapped(nt, 4 * g);
             S[nt][pt] = f32x4{0.f, 0.f, 0.f, 0.f};
             if (start) {
-                S[nt][pt] = *reinterpret_cast<const f32x4*>(start + p * NP + n);
+                S[nt][pt] = *reinterpret_cast<const f32x4*>(start + 16 * pt * NP + swapped(nt, 0));
             } else if (a.state && p < cols) {
                 const float* from = a.state + (state_at + p) * a.N + n;
                 if (by_four) {
@@ -131,6 +138,17 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
             }
         }
 
+    if (chain) {
+#pragma unroll 2
+        for (int i = 0; i < at.seg; ++i) {
+            const float decay = segment_decays[((long long)b * a.H + h) * a.segs + i];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int pt = 0; pt < PT; ++pt)
+                    S[nt][pt] = S[nt][pt] * decay + *reinterpret_cast<const f32x4*>(ends + (long long)i * tile + 16 * pt * NP + swapped(nt, 0));
+        }
+    }
     const bool wanted = last && at.seg == a.segs - 1;
     const int c0 = at.seg * a.seg_chunks, c_all = c0 + a.seg_chunks < a.chunks ? c0 + a.seg_chunks : a.chunks;
     const int c_len = (len + kQ - 1) / kQ, c1 = c_all < c_len ? c_all : c_len;
@@ -477,7 +495,8 @@ static unsigned scan_groups(const ScanArgs& a) { return (unsigned)a.rows * a.seg
 
 template <typename T, int NP, int PW>
 static int launch_scan(const ScanArgs& a, const float* starts, void* y, float* last, hipStream_t st) {
-    hipLaunchKernelGGL((scan_kernel<T, NP, PW>), dim3(scan_groups(a)), dim3(256), 0, st, a, starts, static_cast<T*>(y), last);
+    hipLaunchKernelGGL((scan_kernel<T, NP, PW>), dim3(scan_groups(a)), dim3(256), 0, st, a, starts,
+                       starts ? starts + (long long)a.rows * a.H * a.segs * (padded(a.P) * NP) : nullptr, static_cast<T*>(y), last);
     RTFS_LAUNCH_CHECK();
     return RTFS_OK;
 }
@@ -519,7 +538,7 @@ int scan_starts(const ScanArgs& a0, const ScanArgs& a1, const float* state1, flo
     float *e0 = ws, *d0 = ws + n * tile, *e1 = d0 + n, *d1 = e1 + n * tile;
     const WalkOut o0{nullptr, e0, d0, nullptr, nullptr, 0}, o1{nullptr, e1, d1, nullptr, nullptr, 1};
     const int rc = scan_walks(a0, o0, a1, o1, both, type, st);
-    if (rc != RTFS_OK) return rc;
+    if (rc != RTFS_OK || (!both && a0.segs <= kChain)) return rc;  // (the forward kernel chains them itself)
     hipLaunchKernelGGL(scan_join_kernel, dim3(a0.rows * a0.H, (unsigned)(tile / 256), both ? 2 : 1), dim3(256), 0, st, e0, d0, a0.state, e1, d1, state1, a0.segs,
                        a0.P, a0.N, padded(a0.N));
     RTFS_LAUNCH_CHECK();
