@@ -7,7 +7,7 @@
 // Squares are summed in fp64 from the first add on: the sum can neither overflow nor depend on the order beyond fp64's rounding, and a workgroup leaves
 // ONE partial at a fixed place (no atomics), so the norm has the same bits on every run.  The scaling kernel sums the <= 2048 + launches partials again in
 // every workgroup (16 KB out of L2, ~1 us) instead of waiting for one more launch.
-// 300 M bf16 values in 291 tensors (1.8 GB read and written): 430 us, 4.2 TB/s.  RTFS-Net's 403 tensors: 25 us on the device, 175 us on the host that lists them.
+// 300 M bf16 values in 291 tensors (1.8 GB read and written): 427 us, 4.2 TB/s.  RTFS-Net's 403 tensors: 25 us on the device, 175 us on the host that lists them.
 #include "common.h"
 
 namespace rtfs {

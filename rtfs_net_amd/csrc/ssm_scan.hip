@@ -73,7 +73,7 @@ __device__ __forceinline__ void advance(f32x4 (&S)[R][C], const Tile<T, kQ, PW, 
 // A wave walks one segment of its slice and keeps the state in its accumulators from chunk to chunk: an accumulator tile is, as it lies, the operand of the
 // product with C, so the state never leaves registers.  So do the scores: C B^T of a pair of token tiles, times decay and step (D joins the diagonal), is the
 // operand of the product with x.  LDS holds B and C once for four waves and each wave's x; two barriers per chunk.
-// 32768 tokens, 32 heads of 64, N = 128, bf16: 165 us (and 82 + 13 us for the segments' starts); 2048 rows of 125 tokens, 4 heads of 32, N = 32, fp32: 149 us, 40 % of
+// 32768 tokens, 32 heads of 64, N = 128, bf16: 167 us (and 82 + 13 us for the segments' starts); 2048 rows of 125 tokens, 4 heads of 32, N = 32, fp32: 149 us, 40 % of
 // it fp32 matrix instructions.  Per wave, vector instructions take as long as the matrix ones, and the LDS holds no third wave per SIMD to run under them.
 // Roundings (bf16): the scores times decay and step, and the state as it enters the product with C, once each to bf16 - y is rounded to that anyway.  The token
 // tiles on the diagonal keep what the rounding leaves as a second operand: D = 1.01 alone would be off by 0.2 % in every token, more than y's own rounding.
@@ -515,7 +515,7 @@ int scan_walks(const ScanArgs& a0, const WalkOut& o0, const ScanArgs& a1, const 
 // whose state of N values each fits a wave's registers next to the loads in flight (64 columns of 128 spilled).
 // Rows are cut into segments, each walked by workgroups of its own, and into no more than 256: a segment's own state is walked first then (B, x and dt read twice,
 // the state's products done twice) and the segments' states are chained (about 0.1 us each).  A prompt is cut until every CU has two workgroups (seven rows of
-// eight chunks, 6 heads of 48, fp32: 94 us uncut, 75 us in segments of four chunks, 35 us in segments of one).  The gradients' walks, both directions in one
+// eight chunks, 6 heads of 48, fp32: 94 us uncut, 75 us in segments of four chunks, 34 us in segments of one).  The gradients' walks, both directions in one
 // launch, are cut until every CU has one: they write a tile per chunk and are bound by that, not by the products (8 rows of 2048 tokens, 32 heads of 64, N = 128:
 // 172 us uncut at one workgroup per CU; at two 167 us and 118 us more for the first walk and the chain).
 void scan_cut(ScanArgs& a, int directions) {
