@@ -266,12 +266,12 @@ struct Load {
             for (int k = 0; k < kPer; ++k)
                 load(r[k], at + k * (THREADS / kVecs) * step, kUnits % THREADS == 0 || thread + k * THREADS < kUnits ? cols - (int)c : 0);
         };
+        // formed anew at every call: hoisted out of the chunk loop, these offsets and conditions would take a hundred registers
+        asm volatile("" : "+v"(thread));
         if (how == kAligned) {
             all(thread, [&](Vec8<T>& v, unsigned at, int n) { load8(v, rsrc, at, n); });
             return;
         }
-        // formed anew at every call: hoisted out of the chunk loop, these offsets and conditions would take a hundred registers
-        asm volatile("" : "+v"(thread));
         if (how == kAnywhere && cols * (int)sizeof(T) >= 16) all(thread, [&](Vec8<T>& v, unsigned at, int n) { load8_anywhere(v, rsrc, at, n); });
         else all(thread, [&](Vec8<T>& v, unsigned at, int n) { load8_singly(v, rsrc, at, n); });
     }

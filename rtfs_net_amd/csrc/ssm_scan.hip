@@ -75,9 +75,10 @@ __device__ __forceinline__ void advance(f32x4 (&S)[R][C], const Tile<T, kQ, PW, 
 // operand of the product with x.  LDS holds B and C once for four waves and each wave's x; two barriers per chunk.
 // 32768 tokens, 32 heads of 64, N = 128, bf16: 167 us (and 82 + 13 us for the segments' starts); 2048 rows of 125 tokens, 4 heads of 32, N = 32, fp32: 149 us, 40 % of
 // it fp32 matrix instructions.  Per wave, vector instructions take as long as the matrix ones, and the LDS holds no third wave per SIMD to run under them.
-// Roundings (bf16): the scores times decay and step, and the state as it enters the product with C, once each to bf16 - y is rounded to that anyway.  The token
-// tiles on the diagonal keep what the rounding leaves as a second operand: D = 1.01 alone would be off by 0.2 % in every token, more than y's own rounding.
-// The weighted inputs that build the state are split (ssm.h), so the state that is handed on has fp32's precision.
+// Roundings (bf16): y's own alone counts. The scores times decay and step (with D on the diagonal) and the state as it enters the product with C are operands of
+// two bf16 each, the second what rounding to the first leaves: they lose 2^-17 of a factor where y is rounded by 2^-9. As single bf16 they cost y 1.04 times its
+// rounding's error, and 33 us less of 273 on the prompt above. The weighted inputs that build the state are split in three (ssm.h), so the state that is handed on
+// has fp32's precision.
 // Up to kChain segments a row are chained by the kernel itself, from the own states of the segments in front: that reads each of them half kChain times on average,
 // where a launch that chains them reads and writes each and has it read once more (8 rows of four segments, 32 heads of 64 x 128: 16 us).
 constexpr int kChain = 8;
@@ -181,7 +182,7 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int pt = 0; pt < PT; ++pt) asm volatile("" : "+v"(S[nt][pt]));
-                Frag<T> q[2][NP / 32], m[2][2], rest[2];
+                Frag<T> q[2][NP / 32], m[2][2], rest[2][2];
 #pragma unroll
                 for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -220,7 +221,7 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
                     }
                     m[0][kk] = frag_of<T>(s[0][0], s[0][1]);
                     m[1][kk] = frag_of<T>(s[1][0], s[1][1]);
-                    if (kRest && kk == half) rest[0] = frag_of<T>(rest_of(s[0][0]), f32x4{0.f, 0.f, 0.f, 0.f}), rest[1] = frag_of<T>(f32x4{0.f, 0.f, 0.f, 0.f}, rest_of(s[1][1]));
+                    if (kRest) rest[0][kk] = frag_of<T>(rest_of(s[0][0]), rest_of(s[0][1])), rest[1][kk] = frag_of<T>(rest_of(s[1][0]), rest_of(s[1][1]));
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 constexpr int kSome = PT < 2 ? PT : 2;
@@ -236,7 +237,13 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
                     for (int k = 0; k < NP / 32; ++k)
 #pragma unroll
                         for (int pt = 0; pt < kSome; ++pt) {
-                            const Frag<T> s = frag_of<T>(S[2 * k][p0 + pt], S[2 * k + 1][p0 + pt]);
+                            const f32x4 upper = S[2 * k][p0 + pt], lower = S[2 * k + 1][p0 + pt];
+                            if (kRest) {
+                                const Frag<T> s = frag_of<T>(rest_of(upper), rest_of(lower));
+                                acc[0][pt] = mma(s, q[0][k], acc[0][pt]);
+                                acc[1][pt] = mma(s, q[1][k], acc[1][pt]);
+                            }
+                            const Frag<T> s = frag_of<T>(upper, lower);
                             acc[0][pt] = mma(s, q[0][k], acc[0][pt]);
                             acc[1][pt] = mma(s, q[1][k], acc[1][pt]);
                         }
@@ -253,7 +260,7 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
                             const Frag<T> xj = X.down(lp, 32 * kk, p0 + pt);
                             acc[0][pt] = mma(xj, m[0][kk], acc[0][pt]);
                             acc[1][pt] = mma(xj, m[1][kk], acc[1][pt]);
-                            if (kRest && kk == half) acc[0][pt] = mma(xj, rest[0], acc[0][pt]), acc[1][pt] = mma(xj, rest[1], acc[1][pt]);
+                            if (kRest) acc[0][pt] = mma(xj, rest[0][kk], acc[0][pt]), acc[1][pt] = mma(xj, rest[1][kk], acc[1][pt]);
                         }
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {

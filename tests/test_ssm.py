@@ -709,3 +709,18 @@ def test_the_library_refuses_what_its_kernels_cannot_take():
         assert conv(*dims) == -1
     assert h.rtfs_ssm_tile(129, 1) == -1 and h.rtfs_ssm_tile(33, 65) == 64 * 128 and h.rtfs_causal_conv_bwd_work_floats(0, 4, 0) == -1
     assert h.rtfs_ssm_scan_segments(1, 64 * 100, 1, 16, 1, 16, 1) == 100 and h.rtfs_ssm_scan_segments(512, 64 * 100, 1, 16, 1, 16, 1) == 1 and h.rtfs_ssm_scan_bwd_parts(1, 64, 8, 3, 1) == -1
+
+
+# A result that is off by d before it is rounded differs from the definition's rounded value only where a border lies between them: with probability |d| / step, by a
+# step (2 U16 of the value at most), so its square adds up to sum |d| step <= |d| |step|.
+BORDERS = (2 * U16 * tol(torch.bfloat16)) ** 0.5
+
+
+@gpu
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_bf16_outputs_are_the_definition_rounded_once(shape):
+    """nothing inside a prompt is rounded to bf16 alone: y is the definition's rounded value but next to the borders between two"""
+    v = scan_inputs(*shape, torch.bfloat16, seed=shape[1] + 1, fp32_dt=shape[1] % 2 == 0)
+    want, _ = ref_scan(*(v[k].double() for k in ("x", "dt", "A", "Bm", "C", "D", "bias")), True, v["state"].double(), None)
+    y, _ = gpu_scan(cuda(v))
+    assert off(y, want.bfloat16()) <= BORDERS
