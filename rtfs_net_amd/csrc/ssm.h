@@ -250,7 +250,8 @@ __device__ __forceinline__ void load8_singly(Vec8<float>& v, __amdgpu_buffer_rsr
 // zero and never read (a padded batch may hold anything there).  Buffer loads throughout: their bounds check supplies the zeros without a branch, and code
 // without branches lets the loads stay in flight until put() - a tile is asked for ahead of the work on the one before.  `how` the rows lie:
 enum { kAligned = 0, kAnywhere = 1, kShort = 2 };  // on 16 bytes, `cols` a multiple of them; rows of at least 16 bytes; shorter ones (and what a slice leaves of one), value by value
-template <typename T, int COLS, int THREADS>
+// ANEW: offsets of aligned rows are formed at every call too, a dozen registers fewer over the chunk loop (bf16 prompts, which spill otherwise: 290 us, 274 with it).
+template <typename T, int COLS, int THREADS, bool ANEW = false>
 struct Load {
     static constexpr int kVecs = COLS / 8, kUnits = kQ * kVecs, kPer = (kUnits + THREADS - 1) / THREADS;
     Vec8<T> r[kPer];
@@ -266,12 +267,13 @@ struct Load {
             for (int k = 0; k < kPer; ++k)
                 load(r[k], at + k * (THREADS / kVecs) * step, kUnits % THREADS == 0 || thread + k * THREADS < kUnits ? cols - (int)c : 0);
         };
-        // formed anew at every call: hoisted out of the chunk loop, these offsets and conditions would take a hundred registers
-        asm volatile("" : "+v"(thread));
         if (how == kAligned) {
+            if (ANEW) asm volatile("" : "+v"(thread));
             all(thread, [&](Vec8<T>& v, unsigned at, int n) { load8(v, rsrc, at, n); });
             return;
         }
+        // formed anew at every call: hoisted out of the chunk loop, these offsets and conditions would take a hundred registers
+        asm volatile("" : "+v"(thread));
         if (how == kAnywhere && cols * (int)sizeof(T) >= 16) all(thread, [&](Vec8<T>& v, unsigned at, int n) { load8_anywhere(v, rsrc, at, n); });
         else all(thread, [&](Vec8<T>& v, unsigned at, int n) { load8_singly(v, rsrc, at, n); });
     }

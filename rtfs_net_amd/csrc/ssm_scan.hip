@@ -153,8 +153,8 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
     const bool wanted = last && at.seg == a.segs - 1;
     const int c0 = at.seg * a.seg_chunks, c_all = c0 + a.seg_chunks < a.chunks ? c0 + a.seg_chunks : a.chunks;
     const int c_len = (len + kQ - 1) / kQ, c1 = c_all < c_len ? c_all : c_len;
-    Load<T, NP, 256> lb, lcc;
-    Load<T, PW, 64> lx;
+    Load<T, NP, 256, kRest> lb, lcc;
+    Load<T, PW, 64, kRest> lx;
     float raw = 0.f;
     auto ask = [&](int c) {
         const long long t0 = (long long)c * kQ;
