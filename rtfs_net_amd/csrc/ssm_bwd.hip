@@ -32,8 +32,9 @@ struct GradArgs {
 // 8 rows of 2048 tokens, 32 heads of 64, N = 128, bf16: 320 us; 2048 rows of 125 tokens, 4 heads of 32, N = 32, fp32: 325 us.  About 1100 vector instructions per head
 // and wave, spread evenly (the products with H and G a tenth, the per-token sums 13 %, the stores of dx 5 %), are what bounds it, with the matrix instructions
 // a third of the time; smaller rings for a third wave per SIMD were slower.
-// What a and d(step) need is summed in fp32 from products of split operands (ssm.h), and so is what dB and dC take from the states; the scores that dB and dC are
-// formed of keep what the rounding leaves as a second operand.  What only dx needs is rounded to the tensors' type once on its way into a product.
+// What a and d(step) need is summed in fp32 from products of split operands (ssm.h), and so is what dB and dC take from the states. The scores that dB and dC are
+// formed of, the weights of dx and G in its product are two bf16 each, the second what rounding to the first leaves: 2^-17 of a factor is lost, next to the results'
+// own 2^-9 (dx's as single bf16: 1.12 times its rounding's error; 18 us less of 662 at 8 x 2048 tokens).
 constexpr int kRing = 4;  // heads per ring of decays and sums
 
 template <int HALF, int ALT> struct HeadSums {
@@ -51,8 +52,11 @@ template <typename T, int NP, int PP> struct GradShare {
     typedef Tile<T, NP, PB, kDownOnly> States;
     typedef Tile<T, kQ, kQ, kInOrder> Scores;
     typedef HeadSums<kHalf, kAlt> Sums;
-    static constexpr int kParts = sizeof(T) == 2 ? 2 : 1;  // bf16: the scores summed over the heads, and what rounding leaves of them
-    static constexpr int kMain = 2 * Slim::kBytes + States::kBytes, kLast = kParts * Scores::kBytes, kPool = kMain > kLast ? kMain : kLast;
+    static constexpr int kParts = sizeof(T) == 2 ? 2 : 1;  // bf16: operands that were fp32 (G, scores), and what rounding leaves of them
+    // The weights of dx are formed with the first block of P where their registers are to spare, else anew where they are used (2048 rows of 125 tokens, 4 heads of
+    // 32, N = 32, fp32: 556 us, 560 formed late; 4 rows of 1024 tokens, 16 heads of 64, N = 128, fp32: 261 us, 272 formed early and spilled).
+    static constexpr bool kEarly = NP == 32;
+    static constexpr int kMain = 2 * Slim::kBytes + kParts * States::kBytes, kLast = kParts * Scores::kBytes, kPool = kMain > kLast ? kMain : kLast;
     static constexpr int kBytes = 2 * Wide::kBytes + kPool + kRing * (int)(sizeof(Decays) + sizeof(Factors) + sizeof(Sums));
     static constexpr int kWavesPerSimd = kWaves == 8 || kBytes * 2 <= 160 * 1024 ? 2 : 1;
 };
@@ -76,7 +80,7 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
     __shared__ __attribute__((aligned(16))) Factors factors[kRing];
     __shared__ __attribute__((aligned(16))) typename S::Sums sums[kRing];
     typename S::Slim &Ys = *reinterpret_cast<typename S::Slim*>(pool), &Xs = *reinterpret_cast<typename S::Slim*>(pool + S::Slim::kBytes);
-    typename S::States& Gs = *reinterpret_cast<typename S::States*>(pool + 2 * S::Slim::kBytes);  // rows: places of n
+    typename S::States* Gs = reinterpret_cast<typename S::States*>(pool + 2 * S::Slim::kBytes);  // rows: places of n
     const ScanArgs& a = q.a;
     unsigned i0 = xcd_block(blockIdx.x, gridDim.x);
     const int part = (int)(i0 % q.parts);
@@ -146,7 +150,22 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
             return v;
         };
         f32x4 dM[kOwn], R[4][NS];
-        Frag<T> wgt[2];
+        Frag<T> wgt[2][S::kParts];
+        auto weigh = [&] {
+            const float d = e.step[j];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                f32x4 m[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int tt = 2 * k + r;
+                    m[r] = zero;
+                    if (tt >= jt) m[r] = cb[tt] * decay_tile(tt) * d;
+                }
+                wgt[k][0] = frag_of<T>(m[0], m[1]);
+                if (S::kParts == 2) wgt[k][1] = frag_of<T>(rest_of(m[0]), rest_of(m[1]));
+            }
+        };
         f32x4 gh = zero;  // four sums: an error of <G, H> is all the chunk's tokens'
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
@@ -172,20 +191,7 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
             const bool next = pb + 1 == blocks;  // head
             if (!next || h + 1 < h1) ask(next ? h + 1 : h, next ? 0 : p0 + PB);
             __syncthreads();
-            if (pb == 0) {
-                const float d = e.step[j];
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    f32x4 m[2];
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const int tt = 2 * k + r;
-                        m[r] = zero;
-                        if (tt >= jt) m[r] = cb[tt] * decay_tile(tt) * d;
-                    }
-                    wgt[k] = frag_of<T>(m[0], m[1]);
-                }
-            }
+            if (S::kEarly && pb == 0) weigh();
 #pragma unroll
             for (int k = 0; k < PB / 32; ++k) {
                 const Frag<T> xj = Xs.row(lp, 16 * jt, 32 * k);
@@ -201,7 +207,8 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
                     for (int pt = 0; pt < PB / 16; ++pt) {
                         const f32x4 other = p0 + 16 * pt < a.P ? *reinterpret_cast<const f32x4*>(q.front + tiles + ((p0 / 16 + pt) * (NP / 16) + nt0 + s) * 256 + lane * 4) : zero;
                         gh += other * tile[s][pt];
-                        Gs.put4(16 * (nt0 + s) + lc, 16 * pt + 4 * g, tile[s][pt]);
+                        Gs[0].put4(16 * (nt0 + s) + lc, 16 * pt + 4 * g, tile[s][pt]);
+                        if (S::kParts == 2) Gs[1].put4(16 * (nt0 + s) + lc, 16 * pt + 4 * g, rest_of(tile[s][pt]));
                     }
                 }
 #pragma unroll
@@ -269,17 +276,23 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
             }
             __syncthreads();
             const float end = e.to[j] * e.step[j];
+            if (!S::kEarly) weigh();
             T* dx = static_cast<T*>(q.dx) + at + (long long)j * a.H * a.P + p0;
 #pragma unroll
             for (int i = 0; i < PB / 16 / S::kAlt; ++i) {
                 const int pt = S::kAlt == 1 ? i : 2 * i;  // of two neighbours this wave's is known when it runs
                 f32x4 acc = zero;  // rows p, columns j
 #pragma unroll
-                for (int k = 0; k < NP / 32; ++k) acc = mma(alt ? Gs.down(lg, 32 * k, pt + S::kAlt - 1) : Gs.down(lg, 32 * k, pt), Bs.row(ln, 16 * jt, 32 * k), acc);
+                for (int k = 0; k < NP / 32; ++k)
+#pragma unroll
+                    for (int m = S::kParts - 1; m >= 0; --m)
+                        acc = mma(alt ? Gs[m].down(lg, 32 * k, pt + S::kAlt - 1) : Gs[m].down(lg, 32 * k, pt), Bs.row(ln, 16 * jt, 32 * k), acc);
                 acc = acc * end + Ys.get4(j, 16 * (pt + alt) + 4 * g) * D;  // (as a part of the weights D would be rounded with them)
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
-                    if (2 * k + 1 >= jt) acc = mma(alt ? Ys.down(lp, 32 * k, pt + S::kAlt - 1) : Ys.down(lp, 32 * k, pt), wgt[k], acc);
+                    if (2 * k + 1 >= jt)
+#pragma unroll
+                        for (int m = S::kParts - 1; m >= 0; --m) acc = mma(alt ? Ys.down(lp, 32 * k, pt + S::kAlt - 1) : Ys.down(lp, 32 * k, pt), wgt[k][m], acc);
                 const int p = 16 * (pt + alt) + 4 * g;
                 if (j < all && p0 + p < a.P) {
                     T4 v;

@@ -724,3 +724,19 @@ def test_bf16_outputs_are_the_definition_rounded_once(shape):
     want, _ = ref_scan(*(v[k].double() for k in ("x", "dt", "A", "Bm", "C", "D", "bias")), True, v["state"].double(), None)
     y, _ = gpu_scan(cuda(v))
     assert off(y, want.bfloat16()) <= BORDERS
+
+
+@gpu
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_bf16_gradients_are_the_definition_rounded_once(shape):
+    B, L, H, G, P, N = shape
+    v = scan_inputs(*shape, torch.bfloat16, seed=L + 1)
+    r = torch.Generator().manual_seed(2)
+    dy, ds = torch.randn(B, L, H, P, generator=r).bfloat16(), torch.randn(B, H, P, N, generator=r)
+    leaves = {k: t.double().requires_grad_() for k, t in v.items()}
+    y, s = ref_scan(*(leaves[k] for k in ("x", "dt", "A", "Bm", "C", "D", "bias")), True, leaves["state"], None)
+    want = dict(zip(leaves, torch.autograd.grad((y, s), list(leaves.values()), (dy.double(), ds.double()))))
+    here = cuda(v, leaf=True)
+    got = dict(zip(here, torch.autograd.grad(gpu_scan(here), list(here.values()), (dy.cuda(), ds.cuda()))))
+    far = {k: off(got[k], want[k].bfloat16()) for k in ("x", "dt", "Bm", "C")}
+    assert max(far.values()) <= BORDERS, far
