@@ -14,6 +14,7 @@ CUDA tensors only: no CPU fallback."""
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -61,16 +62,16 @@ def _on_gpu(name, x):
 
 def _tokens(t, dims):
     """t with its last `dims` dimensions contiguous, and its row and token pitches in elements (of [B, L, ...]); tokens further apart than the kernels' 32-bit
-    offsets allow are copied together"""
-    size = 1
-    if t.stride(1) >= 1 << 23:
+    offsets allow are copied together.  One token has no pitch: whatever stride torch keeps for it (a time-first tensor's is the whole batch), a dense one's is given."""
+    size, one = 1, t.shape[1] == 1
+    if t.stride(1) >= 1 << 23 and not one:
         t = t.contiguous()
     for n, s in zip(t.shape[:-dims - 1:-1], t.stride()[:-dims - 1:-1]):
         if n != 1 and s != size:
             t = t.contiguous()
             break
         size *= n
-    return t, t.stride(0), t.stride(1)
+    return t, t.stride(0), math.prod(t.shape[-dims:]) if one else t.stride(1)
 
 
 def _rows(t):

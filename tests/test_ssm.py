@@ -740,3 +740,33 @@ def test_bf16_gradients_are_the_definition_rounded_once(shape):
     got = dict(zip(here, torch.autograd.grad(gpu_scan(here), list(here.values()), (dy.cuda(), ds.cuda()))))
     far = {k: off(got[k], want[k].bfloat16()) for k in ("x", "dt", "Bm", "C")}
     assert max(far.values()) <= BORDERS, far
+
+
+def test_one_token_has_no_pitch():
+    """torch calls a time-first token contiguous and keeps the stride of the whole batch for it"""
+    from rtfs_net_amd.ssm import _tokens
+
+    x = torch.empty(1, 2048, 4, 1024).transpose(0, 1)
+    assert x.is_contiguous() and x.stride(1) == 1 << 23
+    t, row, tok = _tokens(x, 2)
+    assert t is x and (row, tok) == (4096, 4096)
+
+
+@gpu
+def test_one_token_of_a_time_first_batch():
+    from rtfs_net_amd.ssm import causal_conv, selective_scan
+
+    r = torch.Generator(device="cuda").manual_seed(0)
+    x, dt, bc = (torch.randn(1, 2048, *s, device="cuda", generator=r).transpose(0, 1) for s in ((32, 128), (32,), (1, 8)))
+    A, w = -torch.rand(32, device="cuda", generator=r), torch.randn(4096, 2, device="cuda", generator=r)
+    assert x.stride(1) >= 1 << 23
+
+    def run(*leaves):
+        leaves = [t.detach().requires_grad_() for t in leaves]
+        y = selective_scan(*leaves[:2], A, leaves[2], leaves[2], softplus=True)
+        z = causal_conv(leaves[0].flatten(2), w)
+        return [y.detach(), z.detach(), *torch.autograd.grad((y, z), leaves, (torch.ones_like(y), torch.ones_like(z)))]
+
+    dense = [torch.empty(t.shape, device="cuda").copy_(t) for t in (x, dt, bc)]
+    assert dense[0].stride(1) < 1 << 23
+    assert all(torch.equal(a, b) for a, b in zip(run(x, dt, bc), run(*dense)))
