@@ -90,6 +90,11 @@ def _dense(t):
     return t if t is None or t.is_contiguous() else t.contiguous()
 
 
+def _through(t, shape, dtype, device):
+    """what comes out of a call without tokens where `t` went in (None: zeros)"""
+    return t.clone() if t is not None else torch.zeros(shape, dtype=dtype, device=device)
+
+
 # ---- convolution ---------------------------------------------------------------------------------------------------------------------------------------
 
 
@@ -101,8 +106,11 @@ class _CausalConv(torch.autograd.Function):
         x, row, tok = _tokens(x, 1)
         weight, bias, state = _dense(weight), _dense(bias), _dense(state)
         y = torch.empty(B, L, D, dtype=x.dtype, device=x.device)
-        last = torch.empty(B, K - 1, D, dtype=x.dtype, device=x.device) if want_state else None
-        lib.call("rtfs_causal_conv_fwd", _raw(x), row, tok, weight, bias, state, lengths, y, last, B, L, D, K, int(silu), _TYPES[x.dtype])
+        if y.numel():
+            last = torch.empty(B, K - 1, D, dtype=x.dtype, device=x.device) if want_state else None
+            lib.call("rtfs_causal_conv_fwd", _raw(x), row, tok, weight, bias, state, lengths, y, last, B, L, D, K, int(silu), _TYPES[x.dtype])
+        else:  # no token: nothing to launch, the state goes through
+            last = _through(state, (B, K - 1, D), x.dtype, x.device) if want_state else None
         ctx.save_for_backward(x, weight, bias, state, lengths)
         ctx.silu = silu
         ctx.set_materialize_grads(False)
@@ -120,6 +128,9 @@ class _CausalConv(torch.autograd.Function):
         dw = torch.empty_like(weight)
         db = torch.empty_like(bias) if bias is not None else None
         ds = torch.empty_like(state) if state is not None else None
+        if not x.numel():
+            ds = _through(dlast, ds.shape, x.dtype, x.device) if state is not None else None
+            return dx, dw.zero_(), db.zero_() if db is not None else None, ds, None, None, None
         kind = _TYPES[x.dtype]
         work = torch.empty(lib.load().rtfs_causal_conv_bwd_work_floats(D, K, kind), device=x.device)
         lib.call("rtfs_causal_conv_bwd", _raw(x), row, tok, weight, bias, state, lengths, dy, _dense(dlast), dx, ds, dw, db, work, B, L, D, K, int(ctx.silu), kind)
@@ -149,11 +160,7 @@ def causal_conv(x, weight, bias=None, *, silu=True, state=None, lengths=None, re
         _check("causal_conv", "state", state, (B, K - 1, D), (x.dtype,), x.device)
     lengths = _lengths("causal_conv", lengths, B, x.device)
     _on_gpu("causal_conv", x)
-    if 0 in (B, L, D):  # no token: nothing to launch, the state goes through
-        y = x * 1
-        last = state.clone() if state is not None else x.new_zeros(B, K - 1, D)
-    else:
-        y, last = _CausalConv.apply(x, weight, bias, state, lengths, bool(silu), bool(return_state))
+    y, last = _CausalConv.apply(x, weight, bias, state, lengths, bool(silu), bool(return_state))
     return (y, last) if return_state else y
 
 
@@ -191,12 +198,15 @@ class _SelectiveScan(torch.autograd.Function):
         A, D, dt_bias, state = _dense(A), _dense(D), _dense(dt_bias), _dense(state)
         (x, xr, xt), (dt, tr, tt), (Bm, br, bt), (C, cr, ct) = _tokens(x, 2), _tokens(dt, 1), _tokens(Bm, 2), _tokens(C, 2)
         y = torch.empty(B, L, H, P, dtype=x.dtype, device=x.device)
-        last = torch.empty(B, H, P, N, device=x.device) if want_state else None
-        handle = lib.load()
-        segs = handle.rtfs_ssm_scan_segments(B, L, H, P, G, N, 1)
-        work = torch.empty(B * H * segs * (handle.rtfs_ssm_tile(P, N) + 1), device=x.device) if segs > 1 else None
-        lib.call("rtfs_ssm_scan_fwd", _raw(x), xr, xt, _raw(dt), tr, tt, _TYPES[dt.dtype], A, _raw(Bm), br, bt, _raw(C), cr, ct, D, dt_bias, int(softplus), state,
-                 lengths, y, last, work, B, L, H, P, G, N, _TYPES[x.dtype])
+        if y.numel():
+            last = torch.empty(B, H, P, N, device=x.device) if want_state else None
+            handle = lib.load()
+            segs = handle.rtfs_ssm_scan_segments(B, L, H, P, G, N, 1)
+            work = torch.empty(B * H * segs * (handle.rtfs_ssm_tile(P, N) + 1), device=x.device) if segs > 1 else None
+            lib.call("rtfs_ssm_scan_fwd", _raw(x), xr, xt, _raw(dt), tr, tt, _TYPES[dt.dtype], A, _raw(Bm), br, bt, _raw(C), cr, ct, D, dt_bias, int(softplus), state,
+                     lengths, y, last, work, B, L, H, P, G, N, _TYPES[x.dtype])
+        else:
+            last = _through(state, (B, H, P, N), torch.float32, x.device) if want_state else None
         ctx.save_for_backward(x, dt, A, Bm, C, D, dt_bias, state, lengths)
         ctx.softplus = softplus
         ctx.set_materialize_grads(False)
@@ -218,6 +228,9 @@ class _SelectiveScan(torch.autograd.Function):
         dB, dC = new(B, L, G, N, dtype=x.dtype), new(B, L, G, N, dtype=x.dtype)
         dA, dD, db = new(H), new(H) if D is not None else None, new(H) if dt_bias is not None else None
         ds = torch.empty_like(state) if state is not None else None
+        if not x.numel():
+            ds = _through(dlast, ds.shape, torch.float32, x.device) if state is not None else None
+            return dx, ddt, dA.zero_(), dB, dC, dD.zero_() if dD is not None else None, db.zero_() if db is not None else None, ds, None, None, None
         handle = lib.load()
         segs, tile, parts, chunks = handle.rtfs_ssm_scan_segments(B, L, H, P, G, N, 2), handle.rtfs_ssm_tile(P, N), handle.rtfs_ssm_scan_bwd_parts(B, L, H, G, N), -(-L // 64)
         starts = new(2 * B * H * segs * (tile + 1)) if segs > 1 else None
@@ -268,11 +281,7 @@ def selective_scan(x, dt, A, B, C, D=None, *, dt_bias=None, softplus=False, stat
     G, N = _scan_parameters("selective_scan", x, dt, A, B, C, D, dt_bias, state, (rows, L))
     lengths = _lengths("selective_scan", lengths, rows, x.device)
     _on_gpu("selective_scan", x)
-    if 0 in (rows, L):
-        y = x * 1
-        last = state.clone() if state is not None else torch.zeros(rows, H, P, N, device=x.device)
-    else:
-        y, last = _SelectiveScan.apply(x, dt, A, B, C, D, dt_bias, state, lengths, bool(softplus), bool(return_state))
+    y, last = _SelectiveScan.apply(x, dt, A, B, C, D, dt_bias, state, lengths, bool(softplus), bool(return_state))
     return (y, last) if return_state else y
 
 
