@@ -8,6 +8,9 @@
 // ONE partial at a fixed place (no atomics), so the norm has the same bits on every run.  The scaling kernel sums the <= 2048 + launches partials again in
 // every workgroup (16 KB out of L2, ~1 us) instead of waiting for one more launch.
 // 300 M bf16 values in 291 tensors (1.8 GB read and written): 427 us, 4.2 TB/s.  RTFS-Net's 403 tensors: 25 us on the device, 175 us on the host that lists them.
+#include <algorithm>
+#include <new>
+
 #include "common.h"
 
 namespace rtfs {
@@ -149,6 +152,33 @@ static void clip_lists(const long long* grads, const long long* sizes, const int
     if (k) f(list, k, units);
 }
 
+// Whether two tensors have memory in common: their workgroups would scale it at once, in whatever order they run.  Lists in the order of their addresses, as
+// views of one buffer come, are seen in one pass; others are sorted.  -> 0, 1, or -1 without memory to sort them in
+static int clip_overlaps(const long long* grads, const long long* sizes, const int* types, int n) {
+    struct Span {
+        unsigned long long from, to;
+        bool operator<(const Span& o) const { return from < o.from; }
+    };
+    auto span = [&](int i) { return Span{(unsigned long long)grads[i], (unsigned long long)grads[i] + (unsigned long long)sizes[i] * (types[i] == 0 ? 4 : 2)}; };
+    unsigned long long end = 0;
+    bool ordered = true;
+    for (int i = 0; i < n && ordered; ++i) {
+        if (!sizes[i]) continue;
+        const Span s = span(i);
+        ordered = s.from >= end, end = s.to;
+    }
+    if (ordered) return 0;
+    Span* all = new (std::nothrow) Span[n];
+    if (!all) return -1;
+    int k = 0, found = 0;
+    for (int i = 0; i < n; ++i)
+        if (sizes[i]) all[k++] = span(i);
+    std::sort(all, all + k);
+    for (int i = 1; i < k; ++i) found |= all[i].from < all[i - 1].to;
+    delete[] all;
+    return found;
+}
+
 }  // namespace rtfs
 
 using namespace rtfs;
@@ -163,6 +193,7 @@ int rtfs_clip_grad_norm(const long long* grads, const long long* sizes, const in
         if (types[i] < 0 || types[i] > 2 || sizes[i] < 0 || (sizes[i] && (!grads[i] || grads[i] % (types[i] == 0 ? 4 : 2)))) return RTFS_EINVAL;
         all += sizes[i] / kClipUnit + 2;  // at least its units
     }
+    if (clip_overlaps(grads, sizes, types, n)) return RTFS_EINVAL;
     ClipList list;
     // workgroups of a launch: its share of kClipParts by its units, so the partials of all launches stay in reach of one workgroup
     auto groups = [&](unsigned units) {

@@ -140,8 +140,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0):
     """torch.nn.utils.clip_grad_norm_ as HIP launches: the norm of all gradients of `parameters` (a tensor or an iterable of them; those without a gradient are
     passed over) taken as one vector, and every gradient scaled in place by min(1, max_norm / (norm + 1e-6)).
 
-    norm_type 2 or inf.  fp32, bf16 and fp16 gradients in any mix, dense in any order of their dimensions, without memory in common, on one device; the same
-    tensor listed twice counts once.  The norm's squares are summed in fp64 in a fixed order.  -> the norm before clipping, a 0-dim fp32 tensor on the gradients'
+    norm_type 2 or inf.  fp32, bf16 and fp16 gradients in any mix, dense in any order of their dimensions, without memory in common (refused), on one device; the
+    same tensor listed twice counts once.  The norm's squares are summed in fp64 in a fixed order.  -> the norm before clipping, a 0-dim fp32 tensor on the gradients'
     device (nothing is copied to the host; a norm that is not finite is not an error: a NaN goes through to every gradient).  Every gradient is written, also where
     the factor is 1."""
     max_norm, norm_type = float(max_norm), float(norm_type)
@@ -176,8 +176,14 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0):
     types = array.array("i", types)
     norm = torch.empty((), device=device)
     parts = torch.empty(2048 + len(grads) + (sum(sizes) >> 30), dtype=torch.float64, device=device)  # a tensor of over 2^30 elements is listed in pieces
-    lib.call("rtfs_clip_grad_norm", at.buffer_info()[0], sizes.buffer_info()[0], types.buffer_info()[0], len(grads), max_norm, 2 if norm_type == 2.0 else 0, parts,
-             parts.numel(), norm)
+    try:
+        lib.call("rtfs_clip_grad_norm", at.buffer_info()[0], sizes.buffer_info()[0], types.buffer_info()[0], len(grads), max_norm, 2 if norm_type == 2.0 else 0, parts,
+                 parts.numel(), norm)
+    except RuntimeError:
+        spans = sorted((a, a + g.nbytes) for a, g in zip(at, grads) if g.numel())
+        if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
+            raise ValueError("clip_grad_norm_: two gradients have memory in common") from None
+        raise
     torch.autograd.graph.increment_version(grads)  # written through their addresses
     return norm
 

@@ -184,3 +184,37 @@ def test_the_library_refuses_bad_lists():
     assert call(at, size, kind, 1, 1.0, 2, 0) == -1  # no room for the partial sums
     assert call((ctypes.c_longlong * 1)(4098), size, kind, 1, 1.0, 2, 4096) == -1  # not on an element boundary
     assert call(at, (ctypes.c_longlong * 1)(-1), kind, 1, 1.0, 2, 4096) == -1 and call(at, size, (ctypes.c_int * 1)(3), 1, 1.0, 2, 4096) == -1
+
+
+def test_the_library_refuses_tensors_that_overlap():
+    """before anything is launched (no device is touched): two workgroups would scale the same values at once"""
+    import ctypes
+
+    from rtfs_net_amd import lib
+
+    h = lib.load()
+
+    def call(*spans):  # address, size, type
+        n = len(spans)
+        at, size, kind = zip(*spans)
+        return h.rtfs_clip_grad_norm((ctypes.c_longlong * n)(*at), (ctypes.c_longlong * n)(*size), (ctypes.c_int * n)(*kind), n, 1.0, 2, 16, 4096, 16, None)
+
+    assert call((4096, 8, 0), (4124, 8, 0)) == -1  # the last value of the first is the first of the second
+    assert call((8192, 8, 0), (4096, 8, 1), (8194, 1, 1)) == -1 and call((4096, 100, 1), (4098, 1, 1), (8192, 1, 0)) == -1
+    assert call((4096, 8, 0), (0, 0, 0), (4096, 8, 0)) == -1
+
+
+@pytest.mark.gpu
+def test_gradients_that_overlap_are_refused():
+    from rtfs_net_amd.optim import clip_grad_norm_
+
+    flat = torch.randn(300, device="cuda")
+    held = flat.clone()
+    ps = params([(100,), (100,), (50,), (0,)], [torch.float32], "cuda")
+    ps[0].grad, ps[1].grad = flat[150:250], flat[51:151]
+    with pytest.raises(ValueError, match="memory in common"):
+        clip_grad_norm_(ps, 0.1)
+    assert torch.equal(flat, held)
+    ps[1].grad = flat[50:150]
+    check(ps, 0.1, 2.0)
+    assert torch.equal(flat[:50], held[:50]) and torch.equal(flat[250:], held[250:])
