@@ -575,7 +575,8 @@ int rtfs_ssm_step(const void* x, long long x_row, const void* dt, long long dt_r
 
 /* ---- global gradient norm and clipping for any optimizer (csrc/clip.hip): torch.nn.utils.clip_grad_norm_'s arithmetic over n tensors -------------------------------
  * grads / sizes / types: HOST arrays of device addresses, element counts and types (0 fp32, 1 bf16, 2 fp16); norm_kind 2 (root of the sum of squares, summed in
- * fp64) or 0 (largest magnitude); norm: one float; parts: n_parts >= 2048 + n doubles of workspace.  g *= min(1, max_norm / (norm + 1e-6)) in place.
+ * fp64) or 0 (largest magnitude); norm: one float; parts: n_parts >= 2561 + 512 * (m / 240) doubles of workspace,
+ * m = n and one more for every 2^30 elements of a tensor.  g *= min(1, max_norm / (norm + 1e-6)) in place.
  * Tensors with memory in common are refused (RTFS_EINVAL). */
 int rtfs_clip_grad_norm(const long long* grads, const long long* sizes, const int* types, int n, double max_norm, int norm_kind, double* parts, int n_parts,
                         float* norm, void* stream);

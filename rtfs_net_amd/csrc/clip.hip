@@ -5,9 +5,9 @@
 // 740 k numbers.  The tensor list therefore travels in the kernel arguments (240 entries of 16 bytes per launch, below the 4 KB of an argument block):
 // no table in device memory, no copy to it, and a captured graph holds all it needs.
 // Squares are summed in fp64 from the first add on: the sum can neither overflow nor depend on the order beyond fp64's rounding, and a workgroup leaves
-// ONE partial at a fixed place (no atomics), so the norm has the same bits on every run.  The scaling kernel sums the <= 2048 + launches partials again in
-// every workgroup (16 KB out of L2, ~1 us) instead of waiting for one more launch.
-// 300 M bf16 values in 291 tensors (1.8 GB read and written): 427 us, 4.2 TB/s.  RTFS-Net's 403 tensors: 25 us on the device, 175 us on the host that lists them.
+// ONE partial at a fixed place (no atomics), so the norm has the same bits on every run.  The scaling kernel sums the partials again in every workgroup (16 KB out
+// of L2, ~1 us) instead of waiting for one more launch; lists of some 2000 tensors and more, whose launches leave more partials than that, take the launch.
+// 300 M bf16 values in 291 tensors (1.8 GB read and written): 411 us, 4.4 TB/s; in 5000 tensors 651 us on the device, 2.2 ms on the host.  RTFS-Net's 403 tensors: 25 us on the device, 175 us on the host that lists them.
 #include <algorithm>
 #include <new>
 
@@ -16,7 +16,9 @@
 namespace rtfs {
 
 constexpr int kClipEntries = 240;       // tensors per launch
-constexpr int kClipParts = 2048;        // workgroups over all launches (8 per CU)
+constexpr int kClipParts = 2048;        // workgroups of the whole list (8 per CU), and the most of one launch
+constexpr int kClipLeast = 512;         // workgroups of a norm launch that has as many units, however long the list
+constexpr int kClipFold = 4096;         // more partials than these are summed once, not by every workgroup
 constexpr unsigned kClipUnit = 4096;    // elements a workgroup takes at a time
 constexpr long long kClipLong = 1 << 30;  // a longer tensor is listed in pieces: element counts stay below 2^31
 
@@ -132,6 +134,16 @@ __global__ __launch_bounds__(256) void clip_kernel(ClipList list, int entries, d
     }
 }
 
+// the partials of a long list as one, in a fixed order
+template <bool MAX>
+__global__ __launch_bounds__(256) void clip_fold_kernel(const double* __restrict__ parts, int n_parts, double* __restrict__ total) {
+    __shared__ double red[4];
+    double s = 0.0;
+    for (int i = threadIdx.x; i < n_parts; i += 256) s = clip_join(s, parts[i], MAX);
+    s = clip_reduce(s, MAX, red);
+    if (threadIdx.x == 0) *total = s;
+}
+
 // Lists the tensors launch by launch; f(list, entries, units) for each full or last list.
 template <typename F>
 static void clip_lists(const long long* grads, const long long* sizes, const int* types, int n, ClipList& list, F f) {
@@ -195,14 +207,16 @@ int rtfs_clip_grad_norm(const long long* grads, const long long* sizes, const in
     }
     if (clip_overlaps(grads, sizes, types, n)) return RTFS_EINVAL;
     ClipList list;
-    // workgroups of a launch: its share of kClipParts by its units, so the partials of all launches stay in reach of one workgroup
+    // Workgroups of a norm launch: its share of kClipParts by its units, so that a list of few launches leaves few partials, but never so few that the card runs
+    // empty (launches follow each other: 300 M bf16 values in 5000 tensors: 1880 us on the device by shares alone, 651 so).  A scaling launch leaves none and takes what it can use.
     auto groups = [&](unsigned units) {
-        const long long share = (long long)kClipParts * units / all;
-        return (int)(share < 1 ? 1 : share < units ? share : units);
+        const long long share = (long long)kClipParts * units / all, most = share < kClipLeast ? kClipLeast : share;
+        return (int)(most < units ? most : units);
     };
     int used = 0;
     clip_lists(grads, sizes, types, n, list, [&](const ClipList&, int, unsigned units) { used += groups(units); });
-    if (used == 0 || used > n_parts) return RTFS_EINVAL;
+    const bool fold = used > kClipFold;
+    if (used == 0 || used + fold > n_parts) return RTFS_EINVAL;
     int at = 0, failed = 0;
     clip_lists(grads, sizes, types, n, list, [&](const ClipList& l, int entries, unsigned units) {
         const dim3 grid(groups(units));
@@ -214,9 +228,15 @@ int rtfs_clip_grad_norm(const long long* grads, const long long* sizes, const in
         failed |= hipGetLastError() != hipSuccess;
     });
     if (failed) return RTFS_ELAUNCH;
+    if (fold) {
+        if (norm_kind == 2) hipLaunchKernelGGL(clip_fold_kernel<false>, dim3(1), dim3(256), 0, (hipStream_t)stream, parts, used, parts + used);
+        else hipLaunchKernelGGL(clip_fold_kernel<true>, dim3(1), dim3(256), 0, (hipStream_t)stream, parts, used, parts + used);
+        RTFS_LAUNCH_CHECK();
+        parts += used, used = 1;
+    }
     float* out = norm;  // the first launch writes it
     clip_lists(grads, sizes, types, n, list, [&](const ClipList& l, int entries, unsigned units) {
-        const dim3 grid(groups(units));
+        const dim3 grid(units < (unsigned)kClipParts ? units : (unsigned)kClipParts);
         if (norm_kind == 2)
             hipLaunchKernelGGL((clip_kernel<true, false>), grid, dim3(256), 0, (hipStream_t)stream, l, entries, parts, used, (float)max_norm, out);
         else

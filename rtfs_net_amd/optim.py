@@ -175,7 +175,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0):
     types = [_CLIP_TYPES[g.dtype] for g in grads] if len(kinds) > 1 else [_CLIP_TYPES[grads[0].dtype]] * len(grads)
     types = array.array("i", types)
     norm = torch.empty((), device=device)
-    parts = torch.empty(2048 + len(grads) + (sum(sizes) >> 30), dtype=torch.float64, device=device)  # a tensor of over 2^30 elements is listed in pieces
+    listed = len(grads) + (sum(sizes) >> 30)  # a tensor of over 2^30 elements is listed in pieces
+    parts = torch.empty(2561 + 512 * (listed // 240), dtype=torch.float64, device=device)
     try:
         lib.call("rtfs_clip_grad_norm", at.buffer_info()[0], sizes.buffer_info()[0], types.buffer_info()[0], len(grads), max_norm, 2 if norm_type == 2.0 else 0, parts,
                  parts.numel(), norm)

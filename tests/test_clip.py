@@ -218,3 +218,45 @@ def test_gradients_that_overlap_are_refused():
     ps[1].grad = flat[50:150]
     check(ps, 0.1, 2.0)
     assert torch.equal(flat[:50], held[:50]) and torch.equal(flat[250:], held[250:])
+
+
+def split_params(total, count):
+    flat, ps = torch.randn(total, device="cuda").bfloat16(), []
+    for g in flat.split(total // count):
+        p = torch.nn.Parameter(g.detach())
+        p.grad = g
+        ps.append(p)
+    return ps
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("norm", [2.0, math.inf])
+def test_lists_of_thousands(norm):
+    """so many launches that their partial sums are added up by one of their own"""
+    check(params([(n,) for n in range(8193, 8193 + 2900)], list(U), "cuda"), 0.5, norm)
+    check(params([(3,)] * 5000, [torch.float32], "cuda"), 0.5, norm)
+
+
+@pytest.mark.gpu
+def test_a_long_list_keeps_the_card_busy():
+    """the same values in 20 times as many tensors: 21 launches instead of one each way, and not the time of a card that stands mostly empty"""
+    from rtfs_net_amd.optim import clip_grad_norm_
+
+    times = []
+    for count in (240, 5000):
+        ps = split_params(240_000_000, count)
+        clip_grad_norm_(ps, 1.0)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            clip_grad_norm_(ps, 1.0)
+        best = math.inf
+        for _ in range(6):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            graph.replay()
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        times.append(best)
+    assert times[1] < 3 * times[0], times
