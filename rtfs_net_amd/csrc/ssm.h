@@ -366,11 +366,13 @@ __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_ex
 // by one wave for one chunk; `raw`: this lane's dt (with bias), `alive`: whether its token is within the row
 struct Decay {
     float step, hi, lo;  // of this lane's token
+    bool grows;          // whether any token of the chunk makes states larger
 };
 __device__ __forceinline__ Decay put_decays(Decays& o, float raw, bool alive, bool plus, float A) {
     const int lane = threadIdx.x & 63;
     Decay e;
     e.step = !alive ? 0.f : plus ? softplus(raw) : raw;
+    e.grows = __ballot(e.step * A > 0.f) != 0;
     chunk_decay(e.step, A, e.hi, e.lo);
     const float eh = lane_value(e.hi, 63), el = lane_value(e.lo, 63);
     o.hi[lane] = e.hi, o.lo[lane] = e.lo, o.step[lane] = e.step, o.to[lane] = exp2_fast((eh - e.hi) + (el - e.lo));
@@ -378,20 +380,42 @@ __device__ __forceinline__ Decay put_decays(Decays& o, float raw, bool alive, bo
     return e;
 }
 
-// e^{s[t]-s[j]} of tokens in different tiles of 16 as a product of two factors, with the last token r in front of t's tile between them: both are at most 1 where
-// states decay.  near[t] = e^{s[t]-s[r]}; to(tile of t)[j] = e^{s[r]-s[j]} weight[j], j <= r.
+// e^{s[t]-s[j]} of tokens in different tiles of 16 as a product of two factors with a decay s[r] between them: near[t] = e^{s[t]-s[r]} and
+// to(tile of t)[j] = e^{s[r]-s[j]} weight[j], j in front of t's tile.  Where states only decay, r is the last token in front of t's tile, and both are at most 1.  Where
+// they grow too, a factor could pass fp32's range though the product does not (0 times infinity): s[r] is halfway between the tile's largest s[t] and the smallest
+// s[j] in front of it then, so that a factor is infinite only if the largest decay between the two sides passes e^176, and products of e^-43 and more keep both.
 struct Factors {
     float near[kQ], far[16 + 32 + 48];  // far of the tiles 1, 2, 3 one behind the other
     __device__ __forceinline__ const float* to(int tile) const { return far + (tile == 1 ? 0 : tile == 2 ? 16 : 48); }
 };
+// the value of the lane BY places on, around this lane's row of 16
+template <int BY> __device__ __forceinline__ float turned(float v) {
+    const int bits = __builtin_bit_cast(int, v);
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(bits, bits, 0x120 + BY, 0xf, 0xf, false));  // row_ror
+}
 __device__ __forceinline__ void put_factors(Factors& o, const Decay& e, float weight) {
     const int lane = threadIdx.x & 63;
+    float rh[3], rl[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) rh[k] = lane_value(e.hi, 16 * k + 15), rl[k] = lane_value(e.lo, 16 * k + 15);
+    if (e.grows) {
+        float top = e.hi, low = e.hi;
+        top = fmaxf(top, turned<8>(top)), low = fminf(low, turned<8>(low));
+        top = fmaxf(top, turned<4>(top)), low = fminf(low, turned<4>(low));
+        top = fmaxf(top, turned<2>(top)), low = fminf(low, turned<2>(low));
+        top = fmaxf(top, turned<1>(top)), low = fminf(low, turned<1>(low));
+        float least = lane_value(low, 0);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            rh[k] = 0.5f * (lane_value(top, 16 * (k + 1)) + least), rl[k] = 0.f;
+            least = fminf(least, lane_value(low, 16 * (k + 1)));
+        }
+    }
     float nh = 0.f, nl = 0.f;
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
-        const float rh = lane_value(e.hi, 16 * k + 15), rl = lane_value(e.lo, 16 * k + 15);
-        if (lane <= 16 * k + 15) o.far[(k == 0 ? 0 : k == 1 ? 16 : 48) + lane] = exp2_fast((rh - e.hi) + (rl - e.lo)) * weight;
-        if (lane >> 4 == k + 1) nh = rh, nl = rl;
+        if (lane <= 16 * k + 15) o.far[(k == 0 ? 0 : k == 1 ? 16 : 48) + lane] = exp2_fast((rh[k] - e.hi) + (rl[k] - e.lo)) * weight;
+        if (lane >> 4 == k + 1) nh = rh[k], nl = rl[k];
     }
     o.near[lane] = exp2_fast((e.hi - nh) + (e.lo - nl));
 }

@@ -274,7 +274,7 @@ def selective_scan(x, dt, A, B, C, D=None, *, dt_bias=None, softplus=False, stat
     y[t] = S[t] C[t] + D x[t].
 
     x [B, L, H, P], B and C [B, L, G, N], fp32 or bf16 (head h uses group h // (H // G)); dt [B, L, H] of x's type or fp32; A, D, dt_bias [H] fp32, the rates in A
-    negative for a state that decays; state [B, H, P, N] fp32 in front of token 0 (None: zeros); lengths int32 [B].  P, N <= 128, B H < 2^22, H P < 2^23.
+    negative for a state that decays (without softplus a step may have either sign too; what lies between two tokens of a row may grow by e^88, fp32's range); state [B, H, P, N] fp32 in front of token 0 (None: zeros); lengths int32 [B].  P, N <= 128, B H < 2^22, H P < 2^23.
     -> y [B, L, H, P], or (y, last) with `return_state`: last [B, H, P, N], the state behind each row's end.  Differentiable in every tensor but lengths."""
     _first("selective_scan", x, 4)
     rows, L, H, P = x.shape

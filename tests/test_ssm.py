@@ -797,3 +797,54 @@ def test_gradients_without_tokens(B, L):
     none, empty = torch.zeros(2, 3, 0, device="cuda"), torch.zeros(0, 4, device="cuda", requires_grad=True)
     causal_conv(none, empty).sum().backward()
     assert empty.grad.shape == (0, 4)
+
+
+def swings(up, down):
+    """steps of both signs: six tokens that let states grow by e^up, twelve that let them fall by e^down, within one tile of 16 tokens and across three"""
+    v = scan_inputs(2, 150, 2, 1, 16, 16, torch.float32, seed=3)
+    v["A"], v["bias"] = torch.tensor([-1.0, -0.5]), torch.zeros(2)
+    dt = torch.full((2, 150, 2), 0.05)
+    for at in (8, 34, 118):
+        dt[:, at:at + 6], dt[:, at + 6:at + 18] = -up / 6, down / 12
+    v["dt"] = dt / -v["A"]
+    return v
+
+
+def per_token(got, want):
+    got, want = got.detach().double().cpu(), want.detach().double()
+    return (got - want).norm(dim=(2, 3)) / want.norm(dim=(2, 3))
+
+
+@gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("up,down", [(60, 200), (80, 80), (75, 90)])
+def test_steps_of_both_signs(kind, up, down):
+    """states that fall and grow within a chunk: every token by the definition, and the gradients.  Exponents of up to 300 (log2) are rounded to fp32: 4 tol."""
+    v = swings(up, down)
+    v = {k: t.to(kind) if k in ("x", "Bm", "C") else t for k, t in v.items()}
+    leaves = {k: t.double().requires_grad_() for k, t in v.items()}
+    want = ref_scan(*(leaves[k] for k in ("x", "dt", "A", "Bm", "C", "D", "bias")), False, leaves["state"], None)
+    here = cuda(v, leaf=True)
+    got = gpu_scan(here, softplus=False)
+    assert float(per_token(got[0], want[0]).max()) <= max(4 * tol(torch.float32), tol(kind, 1)) and off(got[1], want[1]) <= 4 * tol(kind)
+    dy = torch.randn(want[0].shape, generator=torch.Generator().manual_seed(2)).to(kind)
+    a = torch.autograd.grad(got[0], list(here.values()), dy.cuda())
+    b = torch.autograd.grad(want[0], list(leaves.values()), dy.double())
+    far = {}
+    for k, p, q in zip(v, a, b):  # (a rate's gradient is 1.04e39 at 80 up and 80 down, more than fp32's largest 3.4e38: its rounding is an infinity of its sign)
+        beyond = q.float().isinf()
+        assert torch.equal(p.cpu().float()[beyond], q.float()[beyond]) and (k == "A" or not beyond.any())
+        far[k] = off(p.cpu()[~beyond], q[~beyond])
+    assert max(far.values()) <= max(8 * tol(torch.float32), tol(kind, 1)), far
+
+
+@gpu
+def test_states_beyond_fp32_for_a_while():
+    """between tokens that are less than e^88 apart the outputs are right, also where the state passes fp32's range between them"""
+    v = swings(120, 144)
+    want, last = ref_scan(*(v[k].double() for k in ("x", "dt", "A", "Bm", "C", "D", "bias")), False, v["state"].double(), None)
+    y, s = gpu_scan(cuda(v), softplus=False)
+    far = per_token(y, want)
+    ok = want.abs().amax((2, 3)) < 1e34
+    assert ok[:, 60:118].all() and ok.float().mean() > 0.8
+    assert float(far[ok].max()) <= 4 * tol(torch.float32) and off(s, last) <= 4 * tol(torch.float32)
