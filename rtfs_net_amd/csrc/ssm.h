@@ -350,9 +350,10 @@ __device__ __forceinline__ double running_sum(double v) {
     v = dpp_add<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
     return dpp_add<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
 }
-// One wave, one token per lane: log2 decay (as two floats whose sum is the fp64 value to 48 bits).
+// One wave, one token per lane: log2 decay (as two floats whose sum is the fp64 value to 48 bits).  A single token's is held at -4096: states are 0 behind it all the
+// same (fp32 ends at -149), and the sums stay far from where fp32 ends, which rates of -1e38 would pass, and small enough that the decays behind it keep their bits.
 __device__ __forceinline__ void chunk_decay(float step, float A, float& hi, float& lo) {
-    const double s = running_sum((double)step * (double)A * 1.4426950408889634074);
+    const double v = (double)step * (double)A * 1.4426950408889634074, s = running_sum(v < -4096.0 ? -4096.0 : v);  // (a NaN goes through)
     hi = (float)s;
     lo = (float)(s - (double)hi);
 }

@@ -848,3 +848,28 @@ def test_states_beyond_fp32_for_a_while():
     ok = want.abs().amax((2, 3)) < 1e34
     assert ok[:, 60:118].all() and ok.float().mean() > 0.8
     assert float(far[ok].max()) <= 4 * tol(torch.float32) and off(s, last) <= 4 * tol(torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("rates", [(-1e38, -3e37), (-1e14, -1e9), (-3e38, -1.0)], ids=str)
+def test_rates_that_forget_at_once(rates):
+    """decays whose logarithms pass fp32's range, or leave no bits for the weaker ones behind them: prompt, gradients and single tokens by the definition"""
+    from rtfs_net_amd.ssm import selective_scan_step
+
+    v = scan_inputs(2, 70, 2, 1, 16, 16, torch.float32, seed=3)
+    v["A"] = torch.tensor(rates)
+    v["dt"][:, 1::2], v["bias"] = -200.0, torch.zeros(2)  # every other step is e^-200: 0 in fp32
+    v["dt"][:, 5::6] = v["dt"][:, 4::6][:, :v["dt"][:, 5::6].shape[1]] - 20  # and some are e^-20 of their neighbour's
+    leaves = {k: t.double().requires_grad_() for k, t in v.items()}
+    want = ref_scan(*(leaves[k] for k in ("x", "dt", "A", "Bm", "C", "D", "bias")), True, leaves["state"], None)
+    here = cuda(v, leaf=True)
+    got = gpu_scan(here)
+    assert off(got[0], want[0]) <= tol(torch.float32) and off(got[1], want[1]) <= tol(torch.float32)
+    dy = torch.randn(want[0].shape, generator=torch.Generator().manual_seed(2))
+    names = ("x", "Bm", "C", "D")
+    for k, p, q in zip(names, torch.autograd.grad(got[0], [here[k] for k in names], dy.cuda()), torch.autograd.grad(want[0], [leaves[k] for k in names], dy.double())):
+        assert off(p, q) <= tol(torch.float32), k
+    u = {k: t.detach() for k, t in here.items()}
+    state = u["state"].clone()
+    steps = [selective_scan_step(u["x"][:, t], u["dt"][:, t], u["A"], u["Bm"][:, t], u["C"][:, t], state, u["D"], dt_bias=u["bias"], softplus=True) for t in range(70)]
+    assert off(torch.stack(steps, 1), want[0]) <= tol(torch.float32) and off(state, want[1]) <= tol(torch.float32)
