@@ -204,6 +204,25 @@ template <int ROWS, int COLS, Kind KIND> struct Tile<__bf16, ROWS, COLS, KIND> {
     }
 };
 
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+// v += 0 x of all x of a Vec8
+__device__ __forceinline__ void times_zero(const Vec8<float>& x, float& v) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v = fmaf(x.a[j], 0.f, v), v = fmaf(x.b[j], 0.f, v);
+}
+__device__ __forceinline__ void times_zero(const Vec8<__bf16>& x, float& v) {
+    const bf16x2 zero = {(__bf16)0.f, (__bf16)0.f};
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) v = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{x.v[j], x.v[j + 1]}, zero, v, false);
+}
+__device__ __forceinline__ float value(const Vec8<float>& x, int j) { return j < 4 ? x.a[j] : x.b[j - 4]; }
+__device__ __forceinline__ float value(const Vec8<__bf16>& x, int j) { return (float)x.v[j]; }
+__device__ __forceinline__ void clear(Vec8<float>& x, int j) {
+    if (j < 4) x.a[j] = 0.f;
+    else x.b[j - 4] = 0.f;
+}
+__device__ __forceinline__ void clear(Vec8<__bf16>& x, int j) { x.v[j] = (__bf16)0.f; }
+
 // 8 values at byte offset `at`, the first `n` of them; bounds are below 2^31, so the offset of a value that is not wanted is set past them and reads as zero
 constexpr unsigned kNowhere = 0x80000000u;
 __device__ __forceinline__ void load8(Vec8<__bf16>& v, __amdgpu_buffer_rsrc_t r, unsigned at, int n) {
@@ -276,6 +295,26 @@ struct Load {
         asm volatile("" : "+v"(thread));
         if (how == kAnywhere && cols * (int)sizeof(T) >= 16) all(thread, [&](Vec8<T>& v, unsigned at, int n) { load8_anywhere(v, rsrc, at, n); });
         else all(thread, [&](Vec8<T>& v, unsigned at, int n) { load8_singly(v, rsrc, at, n); });
+    }
+    // whether this thread holds an infinity or a NaN: 0 times the sum of its values is not 0 then
+    __device__ __forceinline__ bool odd() const {
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) times_zero(r[k], v);
+        return v != v;
+    }
+    // infinities and NaN become zeros; the first token of each value that had one goes to `token` (LDS)
+    __device__ __forceinline__ void clear_odd(unsigned thread, int* token) {
+        asm volatile("" : "+v"(thread));
+#pragma unroll
+        for (int k = 0; k < kPer; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float v = value(r[k], j);
+                if (v - v == 0.f) continue;
+                atomicMin(token + thread % kVecs * 8 + j, (int)(thread / kVecs + k * (THREADS / kVecs)));
+                clear(r[k], j);
+            }
     }
     template <Kind KIND>
     __device__ __forceinline__ void put(unsigned thread, Tile<T, kQ, COLS, KIND>& tile) const {

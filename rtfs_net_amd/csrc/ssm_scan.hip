@@ -79,11 +79,14 @@ __device__ __forceinline__ void advance(f32x4 (&S)[R][C], const Tile<T, kQ, PW, 
 // two bf16 each, the second what rounding to the first leaves: they lose 2^-17 of a factor where y is rounded by 2^-9. As single bf16 they cost y 1.04 times its
 // rounding's error, and 33 us less of 273 on the prompt above. The weighted inputs that build the state are split in three (ssm.h), so the state that is handed on
 // has fp32's precision.
+// An infinity or a NaN in x would reach the tokens in front of it through scores of zero: it is replaced by zero on its way into LDS, and its value of the head
+// becomes a NaN from its token on (odd_from).  Finding none costs 2 %.  (Those of B, C and dt meet no zero: tiles that are masked are not multiplied but chosen.)
 // Up to kChain segments a row are chained by the kernel itself, from the own states of the segments in front: that reads each of them half kChain times on average,
 // where a launch that chains them reads and writes each and has it read once more (8 rows of four segments, 32 heads of 64 x 128: 16 us).
 constexpr int kChain = 8;
+constexpr float kNan = __builtin_nanf("");
 template <typename T, int NP, int PW> struct ScanShare {
-    static constexpr int kBytes = 2 * Tile<T, kQ, NP, kSwapped>::kBytes + 4 * (Tile<T, kQ, PW, kDownOnly>::kBytes + (int)(sizeof(Decays) + sizeof(Factors)));
+    static constexpr int kBytes = 2 * Tile<T, kQ, NP, kSwapped>::kBytes + 4 * (Tile<T, kQ, PW, kDownOnly>::kBytes + (int)(sizeof(Decays) + sizeof(Factors)) + PW * 4);
     // waves per SIMD: two (256 registers each) where a CU's LDS holds as many workgroups, else one
     static constexpr int kWavesPerSimd = kBytes * 2 <= 160 * 1024 ? 2 : 1;
 };
@@ -99,6 +102,7 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
     __shared__ __attribute__((aligned(16))) Tile<T, kQ, PW, kDownOnly> Xs[4];
     __shared__ __attribute__((aligned(16))) Decays decays[4];
     __shared__ __attribute__((aligned(16))) Factors factors[4];
+    __shared__ __attribute__((aligned(16))) int odd_from[4][PW];
     const int lane = threadIdx.x & 63, w = wave_index(), lc = lane & 15, g = lane >> 4;
     const Place at = scan_place(a, w);
     const int b = at.b, h = at.head, len = row_length(a.lengths, b, a.L), cols = a.P - at.p0;
@@ -169,7 +173,15 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
         const int t0 = c * kQ, rows = len - t0 < kQ ? len - t0 : kQ, all = a.L - t0 < kQ ? a.L - t0 : kQ;
         T* out = y + (((long long)b * a.L + t0) * a.H + h) * a.P + at.p0;
         __syncthreads();  // the chunk before has been read
-        lb.put(threadIdx.x, Bs), lcc.put(threadIdx.x, Cs), lx.put(lane, X);
+        lb.put(threadIdx.x, Bs), lcc.put(threadIdx.x, Cs);
+        const bool odd = __ballot(lx.odd()) != 0;
+        if (odd) {
+            int l = lane;
+            asm volatile("" : "+v"(l));
+            if (l < PW) odd_from[w][l] = kQ;
+            lx.clear_odd(l, odd_from[w]);
+        }
+        lx.put(lane, X);
         const Decay d = put_decays(e, raw, lane < rows, a.dt.softplus, A);
         put_factors(f, d, d.step);
         __syncthreads();
@@ -262,6 +274,17 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
                             acc[1][pt] = mma(xj, m[1][kk], acc[1][pt]);
                             if (kRest) acc[0][pt] = mma(xj, rest[0][kk], acc[0][pt]), acc[1][pt] = mma(xj, rest[1][kk], acc[1][pt]);
                         }
+                    if (odd) {
+                        int l = lane;
+                        asm volatile("" : "+v"(l));
+#pragma unroll
+                        for (int pt = 0; pt < kSome; ++pt)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int from = odd_from[w][16 * (p0 + pt) + 4 * (l >> 4) + i] - 32 * half - (l & 15);
+                                acc[0][pt][i] = from <= 0 ? kNan : acc[0][pt][i], acc[1][pt][i] = from <= 16 ? kNan : acc[1][pt][i];
+                            }
+                    }
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         const int t = 16 * (2 * half + r) + lc;
@@ -289,7 +312,19 @@ __global__ __launch_bounds__(256, (ScanShare<T, NP, PW>::kWavesPerSimd)) void sc
             }
         }
         if (c + 1 < c1) ask(c + 1);  // the registers of the products above are free again; the state's products hide the loads
-        if (at.works && (c + 1 < c1 || wanted)) advance<true>(S, X, Bs, e, false);
+        if (at.works && (c + 1 < c1 || wanted)) {
+            advance<true>(S, X, Bs, e, false);
+            if (odd) {
+                int l = lc;
+                asm volatile("" : "+v"(l));
+#pragma unroll
+                for (int pt = 0; pt < PT; ++pt) {
+                    const float v = odd_from[w][16 * pt + l] < kQ ? kNan : 0.f;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) S[nt][pt] += v;
+                }
+            }
+        }
     }
     if (!at.works) return;
     // chunks behind this row's end: nothing but zeros

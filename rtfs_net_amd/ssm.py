@@ -9,7 +9,8 @@ from, `lengths` (int32 [B], on the device) makes the batch a padded one - behind
 stays.  fp32 or bf16 (`x`, `B`, `C`; `dt` may be fp32 next to bf16); parameters and the scan's state are fp32.  Everything is channels-last; `x`, `dt`, `B` and `C`
 may be slices of wider tensors (the values of a token contiguous, rows and tokens at any pitch).  HIP kernels in csrc/ssm_*.hip, on torch's current stream; no
 workspace outlives a call, so captured graphs share none.  A backward pass may be captured too, but (as with every autograd function) not while an eager graph that
-holds the same leaves lives: torch ends the process.  A value that is not finite reaches tokens of its chunk of 64 in front of it too, never another row.
+holds the same leaves lives: torch ends the process.  A value that is not finite reaches the outputs that depend on it, from its token on (an infinity may
+arrive as a NaN), and every gradient of its row.
 CUDA tensors only: no CPU fallback."""
 from __future__ import annotations
 

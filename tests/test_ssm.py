@@ -873,3 +873,30 @@ def test_rates_that_forget_at_once(rates):
     state = u["state"].clone()
     steps = [selective_scan_step(u["x"][:, t], u["dt"][:, t], u["A"], u["Bm"][:, t], u["C"][:, t], state, u["D"], dt_bias=u["bias"], softplus=True) for t in range(70)]
     assert off(torch.stack(steps, 1), want[0]) <= tol(torch.float32) and off(state, want[1]) <= tol(torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(3, 130, 4, 2, 32, 32), (2, 200, 2, 1, 100, 33), (600, 130, 2, 1, 17, 5), (2, 70, 3, 1, 64, 128), (2, 140, 2, 1, 64, 64), (5, 90, 1, 1, 128, 128)], ids=str)
+def test_values_that_are_not_finite_go_forward_only(shape, kind):
+    """an infinity or a NaN changes what the definition says depends on it, from its token on; everything else keeps its bits, the rest of its chunk included"""
+    v = scan_inputs(*shape, kind, seed=7)
+    y0, s0 = (t.cpu() for t in gpu_scan(cuda(v)))
+    b, h = shape[0] - 1, shape[2] - 1
+    for name, t, bad in (("x", 0, "nan"), ("x", 37, "nan"), ("x", 64, "inf"), ("x", 69, "-inf"), ("Bm", 50, "nan"), ("Bm", 65, "inf"), ("C", 33, "nan"), ("C", 64, "-inf"), ("dt", 47, "nan"),
+                         ("dt", 66, "inf"), ("dt", 20, "-inf"), ("state", 0, "nan")):
+        w = {k: u.clone() for k, u in v.items()}
+        if name == "dt":
+            w[name][b, t, h] = float(bad)
+        elif name == "state":
+            w[name][b, h, -1, 0] = float(bad)
+        else:
+            w[name][b, t, -1, -1] = float(bad)
+        row = {k: u[b:b + 1] if k in ("x", "dt", "Bm", "C", "state") else u for k, u in w.items()}
+        y, s = (u.cpu() for u in gpu_scan(cuda(w)))
+        want, last = ref_scan(*(row[k].double() for k in ("x", "dt", "A", "Bm", "C", "D", "bias")), True, row["state"].double(), None)
+        for got, clean, ref in ((y, y0, want), (s, s0, last)):
+            assert torch.equal(got[:b], clean[:b]) and torch.equal(got[b].isfinite(), ref[0].isfinite()), (name, t, bad)
+        assert torch.equal(y[b, :t], y0[b, :t]), (name, t, bad)
+        if name == "x":  # another value's outputs never take part
+            assert torch.equal(y[b].flatten(1)[:, :-1], y0[b].flatten(1)[:, :-1]) and torch.equal(s[b].flatten(0, 1)[:-1], s0[b].flatten(0, 1)[:-1]), (t, bad)
