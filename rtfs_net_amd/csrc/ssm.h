@@ -389,6 +389,19 @@ __device__ __forceinline__ double running_sum(double v) {
     v = dpp_add<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
     return dpp_add<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
 }
+// Sums over the tokens from this lane's on, and those in front of it: of their own, not as what a sum over all leaves, which loses values 2^53 below the others
+__device__ __forceinline__ double running_sum_from(double v) {
+    v = row_sum_from(v);
+    const int row = (threadIdx.x & 63) >> 4;
+    const double t3 = lane_value(v, 48), t2 = lane_value(v, 32) + t3, t1 = lane_value(v, 16) + t2;
+    return v + (row == 0 ? t1 : row == 1 ? t2 : row == 2 ? t3 : 0.0);
+}
+__device__ __forceinline__ double running_sum_before(double v) {
+    v = running_sum(v);
+    const long long bits = __builtin_bit_cast(long long, v);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)bits, 0x138, 0xf, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, (int)(bits >> 32), 0x138, 0xf, 0xf, false);
+    return __builtin_bit_cast(double, (long long)(unsigned)lo | (long long)hi << 32);  // wave_shr:1
+}
 // One wave, one token per lane: log2 decay (as two floats whose sum is the fp64 value to 48 bits).  A single token's is held at -4096: states are 0 behind it all the
 // same (fp32 ends at -149), and the sums stay far from where fp32 ends, which rates of -1e38 would pass, and small enough that the decays behind it keep their bits.
 __device__ __forceinline__ void chunk_decay(float step, float A, float& hi, float& lo) {

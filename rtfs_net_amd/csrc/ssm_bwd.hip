@@ -328,8 +328,7 @@ __global__ __launch_bounds__((GradShare<T, NP, PP>::kThreads), (GradShare<T, NP,
             const float own = tile == 0 ? z0 : tile == 1 ? z1 : tile == 2 ? z2 : z3, left = tile == 0 ? 0.f : tile == 1 ? z0 : tile == 2 ? z0 + z1 : z0 + z1 + z2;
             const float past1 = wave_sum(tile > 1 ? z0 : 0.f), past2 = wave_sum(tile > 2 ? z0 + z1 : 0.f);  // rows behind tiles 1 and 2 of columns in front of them
             const double near = row_sum_from((double)left + ((double)own - (double)step * in)), below = (double)step * low;
-            const double us = running_sum((double)u), vs = running_sum((double)step * v);
-            const double over64 = (double)cross + (vs - (double)step * v) + (lane_value(us, 63) - (us - (double)u)) + near + (row_sum_to(below) - below);
+            const double over64 = (double)cross + running_sum_before((double)step * v) + running_sum_from((double)u) + near + (row_sum_to(below) - below);
             const float over = (float)(over64 + (double)(tile == 1 ? past1 : tile == 2 ? past2 : 0.f)), col = in + low;
             float dstep = lane < rows ? fmaf(A, over, col + s.diagZ[lane] + v) : 0.f;
             if (a.dt.softplus) dstep *= -expm1f(-step);  // softplus'(v) = 1 - e^{-softplus(v)}

@@ -900,3 +900,37 @@ def test_values_that_are_not_finite_go_forward_only(shape, kind):
         assert torch.equal(y[b, :t], y0[b, :t]), (name, t, bad)
         if name == "x":  # another value's outputs never take part
             assert torch.equal(y[b].flatten(1)[:, :-1], y0[b].flatten(1)[:, :-1]) and torch.equal(s[b].flatten(0, 1)[:-1], s0[b].flatten(0, 1)[:-1]), (t, bad)
+
+
+def scan_gradients(v, dy, ds):
+    """all gradients of a scan: the definition's and the kernels'"""
+    leaves = {k: t.double().requires_grad_() for k, t in v.items()}
+    out = ref_scan(*(leaves[k] for k in ("x", "dt", "A", "Bm", "C", "D", "bias")), True, leaves["state"], None)
+    want = torch.autograd.grad(out, list(leaves.values()), (dy.double(), ds.double()))
+    here = cuda(v, leaf=True)
+    got = torch.autograd.grad(gpu_scan(here), list(here.values()), (dy.cuda(), ds.cuda()))
+    return {k: (a, b) for k, a, b in zip(v, got, want)}
+
+
+@gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_sums_over_all_tokens(shape, kind):
+    """gradients of A and dt_bias are sums over B L tokens (those of a head's P values are summed in each), whose magnitudes add up to at most sqrt(B L) of the result
+    for random signs, an eighth of which the sums within a token have averaged out already; dt's own has no such sum"""
+    B, L, H, G, P, N = shape
+    v, r = scan_inputs(*shape, kind, seed=L + 1, fp32_dt=True), torch.Generator().manual_seed(2)
+    far = {k: off(a, b) for k, (a, b) in scan_gradients(v, torch.randn(B, L, H, P, generator=r).to(kind), torch.randn(B, H, P, N, generator=r)).items()}
+    assert max(far["A"], far["bias"]) <= tol(kind) * max(1.0, (B * L) ** 0.5 / 8) and far["dt"] <= tol(kind), far
+
+
+@gpu
+@pytest.mark.parametrize("A,bias", [((-2.0, -5.0), (40.0, -300.0)), ((0.05, 0.0), (0.0, 0.0)), ((-2.0, -5.0), (-60.0, -20.0))], ids=["forgets", "grows", "stands"])
+def test_gradients_of_strong_and_weak_steps(A, bias):
+    """states that are forgotten at once, steps that underflow to zero, states that grow or only add up, and steps whose softplus has no bits next to 1"""
+    v, r = scan_inputs(2, 200, 2, 1, 16, 16, torch.float32, seed=3), torch.Generator().manual_seed(2)
+    v["A"], v["bias"] = torch.tensor(A), torch.tensor(bias)
+    pairs = scan_gradients(v, torch.randn(2, 200, 2, 16, generator=r), torch.randn(2, 2, 16, 16, generator=r))
+    for k, (a, b) in pairs.items():
+        for h in range(2) if k in ("dt", "A", "bias") else (slice(None),):  # heads apart: one has far smaller gradients
+            assert off(a[..., h], b[..., h]) <= 4 * tol(torch.float32), (k, h)
