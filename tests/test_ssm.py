@@ -934,3 +934,20 @@ def test_gradients_of_strong_and_weak_steps(A, bias):
     for k, (a, b) in pairs.items():
         for h in range(2) if k in ("dt", "A", "bias") else (slice(None),):  # heads apart: one has far smaller gradients
             assert off(a[..., h], b[..., h]) <= 4 * tol(torch.float32), (k, h)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["x", "dt", "Bm", "C"])
+def test_gradients_of_other_rows_keep_their_bits(name):
+    v = scan_inputs(3, 700, 2, 1, 32, 32, torch.bfloat16, seed=2)
+    dy = torch.randn(3, 700, 2, 32, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16).cuda()
+
+    def once(v):
+        y, s = gpu_scan(v)
+        return torch.autograd.grad((y, s), [v[k] for k in ("x", "dt", "Bm", "C", "state")], (dy, torch.ones_like(s)))
+
+    w = {k: t.clone() for k, t in v.items()}
+    w[name][1, 300, 0] = float("nan")
+    pairs = list(zip(once(cuda(v, leaf=True)), once(cuda(w, leaf=True))))
+    assert all(torch.equal(p[0], q[0]) and torch.equal(p[2], q[2]) for p, q in pairs)
+    assert any(q[1].isnan().any() for _, q in pairs)
