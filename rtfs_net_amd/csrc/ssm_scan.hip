@@ -73,11 +73,11 @@ __device__ __forceinline__ void advance(f32x4 (&S)[R][C], const Tile<T, kQ, PW, 
 // A wave walks one segment of its slice and keeps the state in its accumulators from chunk to chunk: an accumulator tile is, as it lies, the operand of the
 // product with C, so the state never leaves registers.  So do the scores: C B^T of a pair of token tiles, times decay and step (D joins the diagonal), is the
 // operand of the product with x.  LDS holds B and C once for four waves and each wave's x; two barriers per chunk.
-// 32768 tokens, 32 heads of 64, N = 128, bf16: 167 us (and 82 + 13 us for the segments' starts); 2048 rows of 125 tokens, 4 heads of 32, N = 32, fp32: 149 us, 40 % of
+// 32768 tokens, 32 heads of 64, N = 128, bf16: 205 us (and 84 + 13 us for the segments' starts); 2048 rows of 125 tokens, 4 heads of 32, N = 32, fp32: 149 us, 40 % of
 // it fp32 matrix instructions.  Per wave, vector instructions take as long as the matrix ones, and the LDS holds no third wave per SIMD to run under them.
 // Roundings (bf16): y's own alone counts. The scores times decay and step (with D on the diagonal) and the state as it enters the product with C are operands of
 // two bf16 each, the second what rounding to the first leaves: they lose 2^-17 of a factor where y is rounded by 2^-9. As single bf16 they cost y 1.04 times its
-// rounding's error, and 33 us less of 273 on the prompt above. The weighted inputs that build the state are split in three (ssm.h), so the state that is handed on
+// rounding's error, and 33 us less of the 205 above. The weighted inputs that build the state are split in three (ssm.h), so the state that is handed on
 // has fp32's precision.
 // An infinity or a NaN in x would reach the tokens in front of it through scores of zero: it is replaced by zero on its way into LDS, and its value of the head
 // becomes a NaN from its token on (odd_from).  Finding none costs 2 %.  (Those of B, C and dt meet no zero: tiles that are masked are not multiplied but chosen.)
@@ -555,6 +555,8 @@ int scan_walks(const ScanArgs& a0, const WalkOut& o0, const ScanArgs& a1, const 
 
 // A wave takes 64, 32 or 16 columns of P: the widest that leaves a group's heads four waves of work (the scores of a head are formed by each of its waves), and
 // whose state of N values each fits a wave's registers next to the loads in flight (64 columns of 128 spilled).
+// Both sides where N <= 64, 32 heads of 64: 32768 tokens, N = 64, bf16 201 us in 64 columns, 207 in 32; 8 rows of 2048 tokens, N = 64, bf16 114 and 109 us.  fp32, whose
+// tiles of 64 columns leave a CU one workgroup, would be better off with 32: 540 and 462 us for the former, 279 and 230 us for the latter; the rule does not look at types.
 // Rows are cut into segments, each walked by workgroups of its own, and into no more than 256: a segment's own state is walked first then (B, x and dt read twice,
 // the state's products done twice) and the segments' states are chained (about 0.1 us each).  A prompt is cut until every CU has two workgroups (seven rows of
 // eight chunks, 6 heads of 48, fp32: 94 us uncut, 75 us in segments of four chunks, 34 us in segments of one).  The gradients' walks, both directions in one
