@@ -260,3 +260,21 @@ def test_a_long_list_keeps_the_card_busy():
             best = min(best, a.elapsed_time(b))
         times.append(best)
     assert times[1] < 3 * times[0], times
+
+
+@pytest.mark.gpu
+def test_captured_long_list_replays():
+    from rtfs_net_amd.optim import clip_grad_norm_
+
+    a, b = (split_params(24_000_007, 2500) for _ in range(2))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = clip_grad_norm_(a, 1.0)
+    for i in range(4):
+        for p, q in zip(a, b):
+            q.grad.normal_()
+            p.grad.copy_(q.grad)
+        graph.replay()
+        want = clip_grad_norm_(b, 1.0)
+        torch.cuda.synchronize()
+        assert torch.equal(norm, want) and all(torch.equal(p.grad, q.grad) for p, q in zip(a, b)), i
