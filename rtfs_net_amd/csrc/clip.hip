@@ -7,7 +7,8 @@
 // Squares are summed in fp64 from the first add on: the sum can neither overflow nor depend on the order beyond fp64's rounding, and a workgroup leaves
 // ONE partial at a fixed place (no atomics), so the norm has the same bits on every run.  The scaling kernel sums the partials again in every workgroup (16 KB out
 // of L2, ~1 us) instead of waiting for one more launch; lists of some 2000 tensors and more, whose launches leave more partials than that, take the launch.
-// 300 M bf16 values in 291 tensors (1.8 GB read and written): 411 us, 4.4 TB/s; in 5000 tensors 651 us on the device, 2.2 ms on the host.  RTFS-Net's 403 tensors: 25 us on the device, 175 us on the host that lists them.
+// 300 M bf16 values in 291 tensors (1.8 GB read and written): 405 us, 4.4 TB/s; in 5000 tensors 651 us on the device, 2.1 ms on the
+// host.  RTFS-Net's 403 tensors: 25 us on the device, 175 us on the host that lists them.
 #include <algorithm>
 #include <new>
 
@@ -208,7 +209,8 @@ int rtfs_clip_grad_norm(const long long* grads, const long long* sizes, const in
     if (clip_overlaps(grads, sizes, types, n)) return RTFS_EINVAL;
     ClipList list;
     // Workgroups of a norm launch: its share of kClipParts by its units, so that a list of few launches leaves few partials, but never so few that the card runs
-    // empty (launches follow each other: 300 M bf16 values in 5000 tensors: 1880 us on the device by shares alone, 651 so).  A scaling launch leaves none and takes what it can use.
+    // empty: launches follow each other (300 M bf16 values in 5000 tensors: 1880 us on the device by shares alone, 651 so).  A scaling launch leaves none and takes
+    // what it can use.
     auto groups = [&](unsigned units) {
         const long long share = (long long)kClipParts * units / all, most = share < kClipLeast ? kClipLeast : share;
         return (int)(most < units ? most : units);

@@ -269,7 +269,8 @@ __device__ __forceinline__ void load8_singly(Vec8<float>& v, __amdgpu_buffer_rsr
 // zero and never read (a padded batch may hold anything there).  Buffer loads throughout: their bounds check supplies the zeros without a branch, and code
 // without branches lets the loads stay in flight until put() - a tile is asked for ahead of the work on the one before.  `how` the rows lie:
 enum { kAligned = 0, kAnywhere = 1, kShort = 2 };  // on 16 bytes, `cols` a multiple of them; rows of at least 16 bytes; shorter ones (and what a slice leaves of one), value by value
-// ANEW: offsets of aligned rows are formed at every call too, a dozen registers fewer over the chunk loop (bf16 prompts, which spill otherwise: 290 us, 274 with it).
+// ANEW: offsets of aligned rows are formed at every call too, a dozen registers fewer over the chunk loop (prompts in bf16, which spill otherwise: 32768 tokens, 32 heads
+// of 64, N = 128: 290 us, 274 with it; fp32 gradients of 2048 rows of 125 tokens, 4 heads of 32, which do not: 565 us, 556 without).
 template <typename T, int COLS, int THREADS, bool ANEW = false>
 struct Load {
     static constexpr int kVecs = COLS / 8, kUnits = kQ * kVecs, kPer = (kUnits + THREADS - 1) / THREADS;

@@ -31,7 +31,8 @@ struct GradArgs {
 // time likewise: on one wave they were a third of a head's time.  x and dy are asked for one block ahead.
 // 8 rows of 2048 tokens, 32 heads of 64, N = 128, bf16: 350 us; 2048 rows of 125 tokens, 4 heads of 32, N = 32, fp32: 330 us.  About 1100 vector instructions per head
 // and wave, spread evenly (the products with H and G a tenth, the per-token sums 13 %, the stores of dx 5 %), are what bounds it, with the matrix instructions
-// a third of the time (the forms of P > 32 run out of registers besides: 2 to 35 of 256 go through scratch, in bf16 and with N > 64); smaller rings for a third wave per SIMD were slower.
+// a third of the time (the forms of P > 32 run out of registers besides: 2 to 35 of 256 go through scratch, in bf16 and with N > 64); smaller rings for a third wave
+// per SIMD were slower.
 // What a and d(step) need is summed in fp32 from products of split operands (ssm.h), and so is what dB and dC take from the states. The scores that dB and dC are
 // formed of, the weights of dx and G in its product are two bf16 each, the second what rounding to the first leaves: 2^-17 of a factor is lost, next to the results'
 // own 2^-9 (dx's as single bf16: 1.12 times its rounding's error; 18 us less of 662 at 8 x 2048 tokens).

@@ -555,8 +555,8 @@ int scan_walks(const ScanArgs& a0, const WalkOut& o0, const ScanArgs& a1, const 
 
 // A wave takes 64, 32 or 16 columns of P: the widest that leaves a group's heads four waves of work (the scores of a head are formed by each of its waves), and
 // whose state of N values each fits a wave's registers next to the loads in flight (64 columns of 128 spilled).
-// Both sides where N <= 64, 32 heads of 64: 32768 tokens, N = 64, bf16 201 us in 64 columns, 207 in 32; 8 rows of 2048 tokens, N = 64, bf16 114 and 109 us.  fp32, whose
-// tiles of 64 columns leave a CU one workgroup, would be better off with 32: 540 and 462 us for the former, 279 and 230 us for the latter; the rule does not look at types.
+// Both sides, 32 heads of 64, N = 64: 32768 tokens, bf16 201 us in 64 columns, 207 in 32; 8 rows of 2048 tokens, bf16 114 and 109 us.  The rule does not look at types:
+// fp32, whose tiles of 64 columns leave a CU one workgroup, takes 540 and 279 us, and 462 and 230 in 32 columns.
 // Rows are cut into segments, each walked by workgroups of its own, and into no more than 256: a segment's own state is walked first then (B, x and dt read twice,
 // the state's products done twice) and the segments' states are chained (about 0.1 us each).  A prompt is cut until every CU has two workgroups (seven rows of
 // eight chunks, 6 heads of 48, fp32: 94 us uncut, 75 us in segments of four chunks, 34 us in segments of one).  The gradients' walks, both directions in one

@@ -10,7 +10,7 @@ stays.  fp32 or bf16 (`x`, `B`, `C`; `dt` may be fp32 next to bf16); parameters 
 may be slices of wider tensors (the values of a token contiguous, rows and tokens at any pitch).  HIP kernels in csrc/ssm_*.hip, on torch's current stream; no
 workspace outlives a call, so captured graphs share none.  A backward pass may be captured too, but (as with every autograd function) not while an eager graph that
 holds the same leaves lives: torch ends the process.  A value that is not finite reaches the outputs that depend on it, from its token on (an infinity may
-arrive as a NaN), and every gradient of its row.
+arrive as a NaN), and may reach every gradient of its row.
 CUDA tensors only: no CPU fallback."""
 from __future__ import annotations
 
@@ -275,7 +275,8 @@ def selective_scan(x, dt, A, B, C, D=None, *, dt_bias=None, softplus=False, stat
     y[t] = S[t] C[t] + D x[t].
 
     x [B, L, H, P], B and C [B, L, G, N], fp32 or bf16 (head h uses group h // (H // G)); dt [B, L, H] of x's type or fp32; A, D, dt_bias [H] fp32, the rates in A
-    negative for a state that decays (without softplus a step may have either sign too; what lies between two tokens of a row may grow by e^88, fp32's range); state [B, H, P, N] fp32 in front of token 0 (None: zeros); lengths int32 [B].  P, N <= 128, B H < 2^22, H P < 2^23.
+    negative for a state that decays (without softplus a step may have either sign too; what lies between two tokens of a row may grow by e^88, fp32's range);
+    state [B, H, P, N] fp32 in front of token 0 (None: zeros); lengths int32 [B].  P, N <= 128, B H < 2^22, H P < 2^23.
     -> y [B, L, H, P], or (y, last) with `return_state`: last [B, H, P, N], the state behind each row's end.  Differentiable in every tensor but lengths."""
     _first("selective_scan", x, 4)
     rows, L, H, P = x.shape
